@@ -53,6 +53,9 @@ LIBRARIES: Dict[str, tuple] = {
     "linear_state": ("linear_state.cu", []),
     "token_side": ("token_side.cu", []),
     "state_space": ("state_space.cu", []),
+    "page_append": ("page_append.cu", []),
+    "page_choice": ("page_choice.cu", []),
+    "attention_pages": ("attention_pages.cu", []),
     # host-side bookkeeping (page pools, cache manager, decode plans): plain C++, no CUDA
     "host_core": ("host_core.cpp", []),
 }
