@@ -6,20 +6,24 @@
 // A page named twice counts twice; a number outside the request's table, or a page the table does not hold, is no page; a token
 // that sees no key gets zeros; rows behind the last request's tokens are left as they are.  Scores, weights and sums in 32-bit.
 // What a token does not see is never multiplied, so that it may hold anything.
-#include "common.cuh"
+#include <cooperative_groups.h>
+
+#include "mma_tiles.cuh"
 
 using namespace dinfer;
+using namespace dinfer_mma;
 
 namespace {
 
+// The request of token t: the first whose tokens end behind it (every lane of a full warp asks; requests without tokens are passed
+// over), -1 where there is none.
 __device__ __forceinline__ int request_of(const int* cu, int num_reqs, int t) {
-  if (t >= cu[num_reqs] || t < cu[0]) return -1;
-  int lo = 0, hi = num_reqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+  int ended = 0;
+  for (int i0 = 0; i0 < num_reqs; i0 += 32) {
+    const int i = i0 + (threadIdx.x & 31);
+    ended += __popc(__ballot_sync(0xffffffffu, i < num_reqs && cu[i + 1] <= t));
   }
-  return lo;
+  return ended < num_reqs && t >= cu[0] ? ended : -1;
 }
 
 struct Pages {
@@ -117,18 +121,292 @@ int run(const void* q, void* out, const void* cache, const Pages& p, cudaStream_
   return cuda_status("attention_pages");
 }
 
+
+// ------------------------------------------------------------------------------------------------
+// Bfloat16, head sizes 64 and 128, pages of 16 to 128 tokens, groups of up to 16 heads: few tokens (decode steps).
+// A CTA owns a (token, key head) and, with splits, a share of its keys.  Tiles of 64 keys (a piece of a page or several pages) ride a
+// ring of cp.async stages; a warp takes 16 of a tile's keys as the rows of S^T = K Q^T (the group's heads are the columns, so
+// nothing of the product is spent on padding beyond 8 heads) and of O^T += V^T P^T, with a softmax of its own.  The four warps
+// meet in shared memory at the end, the CTAs of a (token, key head), a cluster, through distributed shared memory.
+constexpr int NT = 128, BN = 64, MAX_TOP = 1024;
+
+template <int D> __device__ __forceinline__ int swz(int row, int chunk) { return row * D + ((chunk ^ (row & 7)) << 3); }
+
+template <int D, int NH8, int STAGES>
+__global__ void __launch_bounds__(NT)
+pages_token_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restrict__ out, const __nv_bfloat16* __restrict__ cache,
+                   const Pages p, int splits) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __nv_bfloat16* sK = reinterpret_cast<__nv_bfloat16*>(smem_raw);          // [STAGES][BN][D]
+  __nv_bfloat16* sV = sK + STAGES * BN * D;                                // [STAGES][BN][D]
+  int2* s_page = reinterpret_cast<int2*>(sV + STAGES * BN * D);            // [top]: (page, keys the token sees of it)
+  __shared__ int s_count;
+  constexpr int NHEADS = NH8 * 8;
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
+  const int t = blockIdx.x / splits, split = blockIdx.x % splits, g = blockIdx.y;
+  const int r = request_of(p.cu, p.num_reqs, t);
+  if (r < 0) return;                                       // (the whole cluster alike)
+  const int group = p.H / p.Hkv, P = p.page_size;
+  if (warp == 0) {
+    const int pos = p.positions[t];
+    const int* chosen = p.chosen + ((int64_t)t * p.Hkv + g) * p.top;
+    int n = 0;
+    for (int i0 = 0; i0 < p.top; i0 += 32) {
+      const int j = i0 + lane < p.top ? chosen[i0 + lane] : -1;
+      int page = -1;
+      if (j >= 0 && j < p.width && (int64_t)j * P <= pos) page = p.table[(int64_t)r * p.width + j];
+      const bool ok = page >= 0 && page < p.num_pages;
+      const unsigned mask = __ballot_sync(0xffffffffu, ok);
+      if (ok) s_page[n + __popc(mask & ((1u << lane) - 1))] = make_int2(page, min(P, pos - j * P + 1));
+      n += __popc(mask);
+    }
+    if (lane == 0) s_count = n;
+  }
+  // Q^T as the B operand: head nt*8 + gr, elements ks*16 + {2tq, 2tq+1} and + 8
+  unsigned qb[D / 16][NH8][2];
+#pragma unroll
+  for (int nt = 0; nt < NH8; ++nt) {
+    const int head = nt * 8 + gr;
+    const __nv_bfloat16* row = q + (int64_t)t * p.ldq + (int64_t)(g * group + head) * D + 2 * tq;
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ++ks) {
+      qb[ks][nt][0] = head < group ? *reinterpret_cast<const unsigned*>(row + ks * 16) : 0u;
+      qb[ks][nt][1] = head < group ? *reinterpret_cast<const unsigned*>(row + ks * 16 + 8) : 0u;
+    }
+  }
+  __syncthreads();
+  const int n_pages = s_count;
+  const int p_log2 = 31 - __clz(P);
+  int tile = 0, tile_end = ((n_pages << p_log2) + BN - 1) / BN;
+  {
+    const int per = (tile_end + splits - 1) / splits;
+    tile = split * per;
+    tile_end = min(tile_end, tile + per);
+  }
+  const int n_tiles = max(0, tile_end - tile);
+  const int64_t plane = (int64_t)p.Hkv * P * D;
+  auto load_tile = [&](int i) {
+    constexpr int C = D / 8, ROWS = NT / C;                // a warp's copies cover whole rows
+    const int chunk = threadIdx.x % C;
+    __nv_bfloat16 *k = sK + (i % STAGES) * BN * D, *v = sV + (i % STAGES) * BN * D;
+#pragma unroll
+    for (int r0 = 0; r0 < BN; r0 += ROWS) {
+      const int row = r0 + threadIdx.x / C;
+      const int key = (tile + i) * BN + row;               // in the list's order
+      const int e = key >> p_log2, o = key & (P - 1);
+      const int2 entry = e < n_pages ? s_page[e] : make_int2(0, 0);
+      const bool ok = o < entry.y;
+      const __nv_bfloat16* src = cache + (ok ? (int64_t)entry.x * 2 * plane + ((int64_t)g * P + o) * D + chunk * 8 : 0);
+      cp_async16(k + swz<D>(row, chunk), src, ok);
+      cp_async16(v + swz<D>(row, chunk), ok ? src + plane : src, ok);
+    }
+  };
+#pragma unroll
+  for (int i = 0; i < STAGES - 1; ++i) {
+    if (i < n_tiles) load_tile(i);
+    cp_async_commit();
+  }
+  float ot[D / 16][NH8][4];
+#pragma unroll
+  for (int i = 0; i < D / 16; ++i)
+#pragma unroll
+    for (int nt = 0; nt < NH8; ++nt) ot[i][nt][0] = ot[i][nt][1] = ot[i][nt][2] = ot[i][nt][3] = 0.f;
+  float m_run[NH8][2], l_run[NH8][2];                      // heads nt*8 + 2tq + {0, 1}
+#pragma unroll
+  for (int nt = 0; nt < NH8; ++nt) { m_run[nt][0] = m_run[nt][1] = -INFINITY; l_run[nt][0] = l_run[nt][1] = 0.f; }
+  const float scale_log2 = p.scale * 1.4426950408889634f;
+  const int key_off = warp * 16;
+
+  for (int i = 0; i < n_tiles; ++i) {
+    cp_async_wait<STAGES - 2>();
+    __syncthreads();                                       // tile i is here, and everyone is done with tile i - 1
+    if (i + STAGES - 1 < n_tiles) load_tile(i + STAGES - 1);
+    cp_async_commit();
+    const __nv_bfloat16 *kt = sK + (i % STAGES) * BN * D, *vt = sV + (i % STAGES) * BN * D;
+    // the warp's 16 keys lie in one page (pages hold a multiple of 16 keys)
+    const int key = (tile + i) * BN + key_off, e = key >> p_log2, o = key & (P - 1);
+    const int seen = e < n_pages ? s_page[e].y - o : 0;
+    if (seen <= 0) continue;
+    const bool vis0 = gr < seen, vis1 = gr + 8 < seen;
+    float st[NH8][4], st2[NH8][4];                         // two accumulators: half the dependent chain
+#pragma unroll
+    for (int nt = 0; nt < NH8; ++nt) {
+      st[nt][0] = st[nt][1] = st[nt][2] = st[nt][3] = 0.f;
+      st2[nt][0] = st2[nt][1] = st2[nt][2] = st2[nt][3] = 0.f;
+    }
+#pragma unroll
+    for (int ks = 0; ks < D / 16; ks += 2) {
+      unsigned a[4], b[4];
+      ldmatrix_x4(a, kt + swz<D>(key_off + (lane & 15), ks * 2 + (lane >> 4)));
+      ldmatrix_x4(b, kt + swz<D>(key_off + (lane & 15), (ks + 1) * 2 + (lane >> 4)));
+#pragma unroll
+      for (int nt = 0; nt < NH8; ++nt) {
+        mma_bf16(st[nt], a[0], a[1], a[2], a[3], qb[ks][nt][0], qb[ks][nt][1]);
+        mma_bf16(st2[nt], b[0], b[1], b[2], b[3], qb[ks + 1][nt][0], qb[ks + 1][nt][1]);
+      }
+    }
+    bool rescale = false;
+    float alpha[NH8][2];
+    unsigned pb[NH8][2];
+#pragma unroll
+    for (int nt = 0; nt < NH8; ++nt) {
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const float s0 = vis0 ? (st[nt][c] + st2[nt][c]) * scale_log2 : -INFINITY;
+        const float s1 = vis1 ? (st[nt][c + 2] + st2[nt][c + 2]) * scale_log2 : -INFINITY;
+        float mx = fmaxf(s0, s1);
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 4));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 8));
+        mx = fmaxf(mx, __shfl_xor_sync(0xffffffffu, mx, 16));
+        const float m_new = fmaxf(m_run[nt][c], mx), m_use = m_new == -INFINITY ? 0.f : m_new;
+        alpha[nt][c] = fast_exp2(m_run[nt][c] - m_use);
+        rescale |= m_new != m_run[nt][c];
+        const float p0 = fast_exp2(s0 - m_use), p1 = fast_exp2(s1 - m_use);
+        l_run[nt][c] = l_run[nt][c] * alpha[nt][c] + p0 + p1;
+        m_run[nt][c] = m_new;
+        st[nt][c] = p0;
+        st[nt][c + 2] = p1;
+      }
+      // the weights are rounded to bfloat16 for the second product (2^-9 of each; their sum is taken before)
+      pb[nt][0] = movmatrix_trans(pack_bf16(st[nt][0], st[nt][1]));
+      pb[nt][1] = movmatrix_trans(pack_bf16(st[nt][2], st[nt][3]));
+    }
+    if (__any_sync(0xffffffffu, rescale)) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int nt = 0; nt < NH8; ++nt) {
+          ot[d][nt][0] *= alpha[nt][0]; ot[d][nt][1] *= alpha[nt][1];
+          ot[d][nt][2] *= alpha[nt][0]; ot[d][nt][3] *= alpha[nt][1];
+        }
+    }
+#pragma unroll
+    for (int d = 0; d < D / 16; ++d) {
+      unsigned a[4];
+      ldmatrix_x4_trans(a, vt + swz<D>(key_off + (lane & 7) + ((lane >> 4) << 3), d * 2 + ((lane >> 3) & 1)));
+#pragma unroll
+      for (int nt = 0; nt < NH8; ++nt) mma_bf16(ot[d][nt], a[0], a[1], a[2], a[3], pb[nt][0], pb[nt][1]);
+    }
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+
+  // ---- the four warps come together: sums relative to the CTA's maximum, in shared memory
+  float* w_o = reinterpret_cast<float*>(smem_raw);         // [4][NHEADS][D]
+  float* w_m = w_o + 4 * NHEADS * D;                       // [4][NHEADS]
+  float* w_l = w_m + 4 * NHEADS;
+  float* c_o = w_l + 4 * NHEADS;                           // [NHEADS][D]
+  float* c_ml = c_o + NHEADS * D;                          // [NHEADS][2]
+#pragma unroll
+  for (int nt = 0; nt < NH8; ++nt) {
+#pragma unroll
+    for (int c = 0; c < 2; ++c) {
+      float l = l_run[nt][c];
+      l += __shfl_xor_sync(0xffffffffu, l, 4);
+      l += __shfl_xor_sync(0xffffffffu, l, 8);
+      l += __shfl_xor_sync(0xffffffffu, l, 16);
+      const int head = nt * 8 + 2 * tq + c;
+      if (gr == 0) { w_m[warp * NHEADS + head] = m_run[nt][c]; w_l[warp * NHEADS + head] = l; }
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d) {
+        w_o[(warp * NHEADS + head) * D + d * 16 + gr] = ot[d][nt][c];
+        w_o[(warp * NHEADS + head) * D + d * 16 + gr + 8] = ot[d][nt][c + 2];
+      }
+    }
+  }
+  __syncthreads();
+  const int64_t orow = (int64_t)t * p.ldo + (int64_t)g * group * D;
+  for (int idx = threadIdx.x; idx < group * D; idx += NT) {
+    const int head = idx / D, d = idx % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = fmaxf(M, w_m[w * NHEADS + head]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc = 0.f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+      const float f = fast_exp2(w_m[w * NHEADS + head] - base);
+      L += w_l[w * NHEADS + head] * f;
+      acc += w_o[(w * NHEADS + head) * D + d] * f;
+    }
+    if (splits == 1) {
+      out[orow + idx] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+    } else {
+      c_o[idx] = acc;
+      if (d == 0) { c_ml[head * 2] = M; c_ml[head * 2 + 1] = L; }
+    }
+  }
+  if (splits == 1) return;
+
+  // ---- the CTAs of the cluster come together: each writes its share of the outputs
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int share = (group * D + splits - 1) / splits;
+  for (int idx = split * share + threadIdx.x; idx < min(group * D, (split + 1) * share); idx += NT) {
+    const int head = idx / D;
+    float M = -INFINITY;
+    for (int s = 0; s < splits; ++s) M = fmaxf(M, cluster.map_shared_rank(c_ml, s)[head * 2]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, acc = 0.f;
+    for (int s = 0; s < splits; ++s) {
+      const float* ml = cluster.map_shared_rank(c_ml, s) + head * 2;
+      const float f = fast_exp2(ml[0] - base);
+      L += ml[1] * f;
+      acc += cluster.map_shared_rank(c_o, s)[idx] * f;
+    }
+    out[orow + idx] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+  }
+  cluster.sync();                                          // nobody leaves while another reads its memory
+}
+
+template <int D, int NH8>
+int run_token(const void* q, void* out, const void* cache, const Pages& p, int splits, cudaStream_t stream) {
+  constexpr int STAGES = 3;
+  const size_t tiles = (size_t)STAGES * 2 * BN * D * 2 + (size_t)p.top * sizeof(int2);
+  const size_t fold = (size_t)(4 * (NH8 * 8) * (D + 2) + NH8 * 8 * (D + 2)) * 4;
+  const size_t smem = tiles > fold ? tiles : fold;
+  auto kernel = pages_token_kernel<D, NH8, STAGES>;
+  static thread_local int set_for = -1;                    // the attribute belongs to the device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (set_for != dev) {
+    const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, STAGES * 2 * BN * D * 2 + MAX_TOP * 8);
+    if (e != cudaSuccess) return cuda_status("attention_pages: shared memory");
+    set_for = dev;
+  }
+  launch_pdl_cluster(kernel, dim3((unsigned)(p.T * splits), p.Hkv), dim3(NT), dim3(splits), smem, stream, (const __nv_bfloat16*)q,
+                     (__nv_bfloat16*)out, (const __nv_bfloat16*)cache, p, splits);
+  return cuda_status("attention_pages (tokens)");
+}
+
+// Whether the tensor-core kernels take the call: rows that 16-byte loads and pair stores address, sizes they are made for.
+bool tensor_cores(const void* q, const void* out, const void* cache, const Pages& p) {
+  const int group = p.H / p.Hkv;
+  return (p.D == 64 || p.D == 128) && p.page_size >= 16 && p.page_size <= 128 && !(p.page_size & (p.page_size - 1)) && group <= 16 &&
+         p.top <= MAX_TOP && p.ldq % 8 == 0 && p.ldo % 2 == 0 && (uintptr_t)q % 16 == 0 && (uintptr_t)cache % 16 == 0 &&
+         (uintptr_t)out % 4 == 0 && p.Hkv <= 65535;
+}
 }  // namespace
 
 // chosen int32 [T, Hkv, top]; cache [num_pages, 2, Hkv, page_size, D].
 DINFER_API int dinfer_attention_pages(const void* q, int64_t ldq, void* out, int64_t ldo, const void* cache, int num_pages,
                                       const int* table, int width, const int* cu_seqlens, int num_reqs, const int* positions,
                                       const int* chosen, int top, int T, int H, int Hkv, int D, int page_size, float scale,
-                                      int dtype, cudaStream_t stream) {
+                                      int sms, int dtype, cudaStream_t stream) {
   if (T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 512 || page_size <= 0 || num_reqs <= 0 || top <= 0 || width < 0)
     return refuse(DINFER_BAD_ARGUMENT, "attention_pages: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d", T, H, Hkv, D, page_size, top);
   if ((H + WARPS - 1) / WARPS > 65535) return refuse(DINFER_BAD_ARGUMENT, "attention_pages: %d heads", H);
   if (T == 0) return DINFER_OK;
   const Pages p{ldq, ldo, num_pages, table, width, cu_seqlens, num_reqs, positions, chosen, top, T, H, Hkv, D, page_size, scale};
+  // CTAs that share a token's keys: as far as all run at the same time (two an SM), each with a tile of its own at least
+  int splits = 1;
+  while (splits < 8 && (int64_t)T * Hkv * splits * 2 <= 2 * sms && splits * 2 * BN <= (int64_t)top * page_size) splits *= 2;
+  if (dtype == DINFER_BF16 && tensor_cores(q, out, cache, p)) {
+    if (D == 128) return H / Hkv <= 8 ? run_token<128, 1>(q, out, cache, p, splits, stream) : run_token<128, 2>(q, out, cache, p, splits, stream);
+    return H / Hkv <= 8 ? run_token<64, 1>(q, out, cache, p, splits, stream) : run_token<64, 2>(q, out, cache, p, splits, stream);
+  }
   DINFER_DISPATCH_DTYPE(dtype, E, { return run<E>(q, out, cache, p, stream); });
 }
 

@@ -17,7 +17,7 @@ from typing import Optional
 
 import torch
 
-from .lib import DTYPE_CODE, KernelError, check, dtype_code, ptr, require_cuda, stream_handle
+from .lib import DTYPE_CODE, KernelError, check, dtype_code, num_sms, ptr, require_cuda, stream_handle
 from .ops import _fn
 
 
@@ -186,8 +186,8 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
         raise KernelError(f"{what}: chosen int32 [T, Hkv, top] with top > 0")
     lib, f = _fn("attention_pages", "dinfer_attention_pages",
                  [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                  c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_void_p])
+                  c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p])
     check(lib, f(ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(cache), num_pages, ptr(block_table), block_table.shape[1],
                  ptr(cu_seqlens), block_table.shape[0], ptr(positions), ptr(chosen), chosen.shape[2], T, num_heads, Hkv, D, page_size,
-                 scale, DTYPE_CODE[q.dtype], stream_handle()), what)
+                 scale, num_sms(), DTYPE_CODE[q.dtype], stream_handle()), what)
     return out
