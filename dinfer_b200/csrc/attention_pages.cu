@@ -381,6 +381,390 @@ int run_token(const void* q, void* out, const void* cache, const Pages& p, int s
   return cuda_status("attention_pages (tokens)");
 }
 
+// ------------------------------------------------------------------------------------------------
+// The same sizes, many tokens (portions of prompts).  Token by token every page would be read once for each token that chose it; here
+// the work is turned round: for every (request, key head, page) the tokens that chose it are listed, and a tile of up to 128 rows
+// (tokens of the list x the group's heads) meets the page's keys once, on the tensor cores.  What a tile makes for a (token, page)
+// pair is a partial result: the sum of weights times values relative to the pair's own maximum, that maximum and the sum of weights,
+// in 32 bits; a last kernel joins the partial results of each token in the order of its list.  Lists are filled with atomic
+// counters, so a token's place in a tile varies from run to run, but no row of a tile depends on the others, and results do not vary.
+//
+// The partial results are the traffic that bounds it (top x D x 4 bytes a token and head, written and read once).  The step is therefore
+// cut into slabs, key heads x runs of tokens, whose partial results fit the L2 together (SLAB_BYTES), one after the other.
+constexpr int64_t SLAB_BYTES = 64ll << 20;
+constexpr int ROWS = 128, PORTION_NT = 256;
+constexpr int64_t MAX_COUNTERS = 1 << 24;   // lists of all slabs (requests x table width x key heads x runs of tokens): 64 MB of counters
+
+struct Slabs {
+  int heads, tokens, chunks, count;     // key heads and tokens of a slab, runs of tokens, slabs (key-head part slowest)
+  int keys;                             // counters of a slab: heads x requests x table width, to a multiple of 32
+  int tile_tokens;                      // tokens of a tile
+  int64_t list, tiles;                  // room of a slab: list entries, tiles
+  int *counts, *cursors, *rank, *base, *entries;   // cursors [count][2]: list entries and tiles given out
+  int4* desc;                           // a tile: (key, first entry, tokens, -)
+  float *part, *ml;                     // [heads][tokens][top][group][D], and (maximum in log2 units, sum of weights)
+  int64_t bytes, zeroed;                // the workspace; what must be zero at the start (from counts on)
+};
+
+Slabs slabs_of(const Pages& p, unsigned char* at) {
+  Slabs s;
+  const int group = p.H / p.Hkv;
+  const int64_t per_token = (int64_t)group * p.top * p.D * 4;             // of one key head
+  s.tokens = p.T;
+  s.chunks = 1;
+  while (s.tokens * per_token > SLAB_BYTES && s.tokens > ROWS) {
+    ++s.chunks;
+    s.tokens = ((p.T + s.chunks - 1) / s.chunks + 31) / 32 * 32;
+  }
+  s.chunks = (p.T + s.tokens - 1) / s.tokens;
+  s.heads = (int)(SLAB_BYTES / (s.tokens * per_token));
+  s.heads = s.heads < 1 ? 1 : s.heads > p.Hkv ? p.Hkv : s.heads;
+  const int parts = (p.Hkv + s.heads - 1) / s.heads;
+  s.heads = (p.Hkv + parts - 1) / parts;
+  s.count = parts * s.chunks;
+  const int64_t keys = ((int64_t)s.heads * p.num_reqs * p.width + 31) / 32 * 32;
+  s.keys = (int)(keys > INT32_MAX / 2 ? INT32_MAX / 2 : keys);
+  s.tile_tokens = ROWS / group;
+  s.list = (int64_t)s.heads * s.tokens * p.top;
+  s.tiles = s.list / s.tile_tokens + (s.list < keys ? s.list : keys) + 1;
+  unsigned char* start = at;
+  auto take = [&](int64_t bytes) { unsigned char* x = at; at += (bytes + 255) / 256 * 256; return x; };
+  s.counts = (int*)take((int64_t)s.count * s.keys * 4);
+  s.cursors = (int*)take((int64_t)s.count * 2 * 4);
+  s.zeroed = at - start;
+  s.base = (int*)take((int64_t)s.count * s.keys * 4);
+  s.rank = (int*)take((int64_t)p.T * p.Hkv * p.top * 4);
+  s.entries = (int*)take((int64_t)s.count * s.list * 4);
+  s.desc = (int4*)take((int64_t)s.count * s.tiles * 16);
+  s.part = (float*)take(s.list * group * p.D * 4);
+  s.ml = (float*)take(s.list * group * 8);
+  s.bytes = at - start;
+  return s;
+}
+
+__device__ __forceinline__ int slab_of(const Slabs& s, int t, int g) { return g / s.heads * s.chunks + t / s.tokens; }
+
+// How often each (request, page) of a slab was chosen, and the place of every choice in its list; -1 for what is no page, -2 in the
+// rows behind the last request.
+__global__ void __launch_bounds__(256)
+pages_count_kernel(const Pages p, const Slabs s) {
+  pdl_enter();
+  const int t = blockIdx.x;
+  const int r = request_of(p.cu, p.num_reqs, t);
+  const int pos = r < 0 ? -1 : p.positions[t];
+  for (int i = threadIdx.x; i < p.Hkv * p.top; i += 256) {
+    const int64_t at = (int64_t)t * p.Hkv * p.top + i;
+    const int g = i / p.top, j = p.chosen[at];
+    int rank = r < 0 ? -2 : -1;
+    if (r >= 0 && j >= 0 && j < p.width && (int64_t)j * p.page_size <= pos) {
+      const int page = p.table[(int64_t)r * p.width + j];
+      if (page >= 0 && page < p.num_pages)
+        rank = atomicAdd(s.counts + (int64_t)slab_of(s, t, g) * s.keys + ((int64_t)(g % s.heads) * p.num_reqs + r) * p.width + j, 1);
+    }
+    s.rank[at] = rank;
+  }
+}
+
+// A list and tiles for every (request, page) that was chosen: a warp adds up its 32 and takes room once.
+__global__ void __launch_bounds__(256)
+pages_lists_kernel(const Pages p, const Slabs s) {
+  pdl_enter();
+  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  const int lane = threadIdx.x & 31;
+  const bool in = i < (int64_t)s.count * s.keys;
+  const int slab = in ? (int)(i / s.keys) : 0, key = in ? (int)(i % s.keys) : 0;     // (the same slab in a whole warp)
+  const int c = in ? s.counts[i] : 0, tiles = (c + s.tile_tokens - 1) / s.tile_tokens;
+  int c_sum = c, t_sum = tiles;
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) {
+    const int a = __shfl_up_sync(0xffffffffu, c_sum, o), b = __shfl_up_sync(0xffffffffu, t_sum, o);
+    if (lane >= o) { c_sum += a; t_sum += b; }
+  }
+  int c_at = 0, t_at = 0;
+  if (lane == 31 && c_sum > 0) {
+    c_at = atomicAdd(s.cursors + slab * 2, c_sum);
+    t_at = atomicAdd(s.cursors + slab * 2 + 1, t_sum);
+  }
+  c_at = __shfl_sync(0xffffffffu, c_at, 31) + c_sum - c;
+  t_at = __shfl_sync(0xffffffffu, t_at, 31) + t_sum - tiles;
+  if (!in || c == 0) return;
+  s.base[i] = c_at;
+  for (int k = 0; k < tiles; ++k)
+    s.desc[(int64_t)slab * s.tiles + t_at + k] = make_int4(key, c_at + k * s.tile_tokens, min(s.tile_tokens, c - k * s.tile_tokens), 0);
+}
+
+__global__ void __launch_bounds__(256)
+pages_fill_kernel(const Pages p, const Slabs s) {
+  pdl_enter();
+  const int t = blockIdx.x;
+  int r = -1;
+  for (int i = threadIdx.x; i < p.Hkv * p.top; i += 256) {
+    const int64_t at = (int64_t)t * p.Hkv * p.top + i;
+    const int rank = s.rank[at];
+    if (rank < 0) continue;
+    if (r < 0) {                                            // (once a thread; lanes may differ here, so no vote)
+      int lo = 0, hi = p.num_reqs - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi + 1) >> 1;
+        if (p.cu[mid] <= t) lo = mid; else hi = mid - 1;
+      }
+      r = lo;
+    }
+    const int g = i / p.top, slab = slab_of(s, t, g);
+    const int base = s.base[(int64_t)slab * s.keys + ((int64_t)(g % s.heads) * p.num_reqs + r) * p.width + p.chosen[at]];
+    s.entries[(int64_t)slab * s.list + base + rank] = (t % s.tokens) * p.top + i % p.top;
+  }
+}
+
+// 0 where a packed bfloat16 is not a number or infinite
+__device__ __forceinline__ unsigned finite2(unsigned x) {
+  if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
+  if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
+  return x;
+}
+__device__ __forceinline__ bool odd2(unsigned x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
+
+// One tile: a warp owns 16 rows.  Q comes from memory straight into fragments: the order of the elements of a product's sum is free,
+// so a lane takes 16 bytes of its rows and of the keys' at the same places, two steps of 16 elements at once.
+template <int D, int P>
+__global__ void __launch_bounds__(PORTION_NT, 2)
+pages_portion_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ cache, const Pages p, const Slabs s, int slab) {
+  extern __shared__ __align__(128) unsigned char smem_raw[];
+  __nv_bfloat16* sK = reinterpret_cast<__nv_bfloat16*>(smem_raw);          // [P][D], 16-byte pieces exchanged by (key & 1) * 4
+  __nv_bfloat16* sV = sK + P * D;                                          // [P][D], by key & 7
+  pdl_enter();
+  if ((int)blockIdx.x >= s.cursors[slab * 2 + 1]) return;
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
+  const int4 d = s.desc[(int64_t)slab * s.tiles + blockIdx.x];
+  const int j = d.x % p.width, r = d.x / p.width % p.num_reqs, gl = d.x / p.width / p.num_reqs;
+  const int g = slab / s.chunks * s.heads + gl, t0 = slab % s.chunks * s.tokens, group = p.H / p.Hkv;
+  const int64_t plane = (int64_t)p.Hkv * P * D;
+  const __nv_bfloat16* keys = cache + (int64_t)p.table[(int64_t)r * p.width + j] * 2 * plane + (int64_t)g * P * D;
+  constexpr int C = D / 8;
+  for (int i = threadIdx.x; i < P * C; i += PORTION_NT) {
+    const int row = i / C, chunk = i % C;
+    cp_async16(sK + row * D + ((chunk ^ ((row & 1) << 2)) << 3), keys + (int64_t)row * D + chunk * 8, true);
+  }
+  cp_async_commit();
+  for (int i = threadIdx.x; i < P * C; i += PORTION_NT) {
+    const int row = i / C, chunk = i % C;
+    cp_async16(sV + row * D + ((chunk ^ (row & 7)) << 3), keys + plane + (int64_t)row * D + chunk * 8, true);
+  }
+  cp_async_commit();
+  // this lane's two rows
+  const int rows = d.z * group;
+  const bool active = warp * 16 < rows;
+  int64_t part[2];                                          // [pair][head] of the partial results, -1: no row
+  int seen[2];
+  const __nv_bfloat16* qr[2];
+#pragma unroll
+  for (int u = 0; u < 2; ++u) {
+    const int row = warp * 16 + gr + 8 * u;
+    part[u] = -1;
+    seen[u] = P;
+    qr[u] = q;
+    if (row < rows) {
+      const int e = s.entries[(int64_t)slab * s.list + d.y + row / group];
+      const int t = t0 + e / p.top, h = row % group;
+      part[u] = ((int64_t)gl * s.tokens * p.top + e) * group + h;
+      seen[u] = min(P, p.positions[t] - j * P + 1);
+      qr[u] = q + (int64_t)t * p.ldq + (int64_t)(g * group + h) * D;
+    }
+  }
+  float st[P / 8][4];
+#pragma unroll
+  for (int n = 0; n < P / 8; ++n) st[n][0] = st[n][1] = st[n][2] = st[n][3] = 0.f;
+  uint4 qa[D / 32][2];
+  if (active) {
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        qa[k][u] = part[u] >= 0 ? *reinterpret_cast<const uint4*>(qr[u] + k * 32 + tq * 8) : make_uint4(0, 0, 0, 0);
+  }
+  cp_async_wait<1>();
+  __syncthreads();
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+  unsigned pa[P / 16][4];
+  if (active) {
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+      for (int n = 0; n < P / 8; ++n) {
+        const int row = n * 8 + gr;
+        const uint4 b = *reinterpret_cast<const uint4*>(sK + row * D + (((k * 4 + tq) ^ ((row & 1) << 2)) << 3));
+        mma_bf16(st[n], qa[k][0].x, qa[k][1].x, qa[k][0].y, qa[k][1].y, b.x, b.y);
+        mma_bf16(st[n], qa[k][0].z, qa[k][1].z, qa[k][0].w, qa[k][1].w, b.z, b.w);
+      }
+    const float scale_log2 = p.scale * 1.4426950408889634f;
+#pragma unroll
+    for (int n = 0; n < P / 8; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        st[n][c] = n * 8 + 2 * tq + (c & 1) < seen[c >> 1] ? st[n][c] * scale_log2 : -INFINITY;
+        m[c >> 1] = fmaxf(m[c >> 1], st[n][c]);
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 1));
+      m[u] = fmaxf(m[u], __shfl_xor_sync(0xffffffffu, m[u], 2));
+    }
+    const float base[2] = {m[0] == -INFINITY ? 0.f : m[0], m[1] == -INFINITY ? 0.f : m[1]};
+#pragma unroll
+    for (int n = 0; n < P / 8; ++n)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        st[n][c] = fast_exp2(st[n][c] - base[c >> 1]);
+        l[c >> 1] += st[n][c];
+      }
+#pragma unroll
+    for (int u = 0; u < 2; ++u) {
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
+      l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
+    }
+    // the weights are rounded to bfloat16 for the second product (2^-9 of each; their sum is taken before)
+#pragma unroll
+    for (int k = 0; k < P / 16; ++k) {
+      pa[k][0] = pack_bf16(st[2 * k][0], st[2 * k][1]);
+      pa[k][1] = pack_bf16(st[2 * k][2], st[2 * k][3]);
+      pa[k][2] = pack_bf16(st[2 * k + 1][0], st[2 * k + 1][1]);
+      pa[k][3] = pack_bf16(st[2 * k + 1][2], st[2 * k + 1][3]);
+    }
+    if (tq == 0)
+#pragma unroll
+      for (int u = 0; u < 2; ++u)
+        if (part[u] >= 0) *reinterpret_cast<float2*>(s.ml + part[u] * 2) = make_float2(m[u], l[u]);
+  }
+  cp_async_wait<0>();
+  __syncthreads();
+  // A value that is not a finite number, in a page that some row sees in part: a weight of zero would carry it into rows that do not
+  // see it.  Those products are then made without such values, and rows that see them get them one by one.
+  bool odd = false;
+  if (__syncthreads_or(seen[0] < P || seen[1] < P)) {
+    for (int i = threadIdx.x; i < P * C; i += PORTION_NT) {
+      const uint4 v = *reinterpret_cast<const uint4*>(sV + i * 8);
+      odd |= odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w);
+    }
+    odd = __syncthreads_or(odd);
+  }
+  if (!active) return;
+#pragma unroll
+  for (int db = 0; db < D / 16; ++db) {
+    float o[2][4] = {};
+#pragma unroll
+    for (int k = 0; k < P / 16; ++k) {
+      unsigned b[4];
+      const int row = k * 16 + (lane & 15);
+      ldmatrix_x4_trans(b, sV + row * D + (((db * 2 + (lane >> 4)) ^ (row & 7)) << 3));
+      if (odd)
+#pragma unroll
+        for (int x = 0; x < 4; ++x) b[x] = finite2(b[x]);
+      mma_bf16(o[0], pa[k][0], pa[k][1], pa[k][2], pa[k][3], b[0], b[1]);
+      mma_bf16(o[1], pa[k][0], pa[k][1], pa[k][2], pa[k][3], b[2], b[3]);
+    }
+    if (odd) {
+#pragma unroll
+      for (int k = 0; k < P / 16; ++k)
+        for (int x = 0; x < 16; ++x) {
+          const int key = k * 16 + x, from = (lane & ~3) | ((x & 7) >> 1);
+          const unsigned w0 = __shfl_sync(0xffffffffu, x < 8 ? pa[k][0] : pa[k][2], from);
+          const unsigned w1 = __shfl_sync(0xffffffffu, x < 8 ? pa[k][1] : pa[k][3], from);
+          const float w[2] = {__uint_as_float(x & 1 ? w0 & 0xffff0000u : w0 << 16), __uint_as_float(x & 1 ? w1 & 0xffff0000u : w1 << 16)};
+#pragma unroll
+          for (int n = 0; n < 2; ++n)
+#pragma unroll
+            for (int c = 0; c < 4; ++c) {
+              const int col = db * 16 + n * 8 + 2 * tq + (c & 1);
+              const float v = __bfloat162float(sV[key * D + (((col >> 3) ^ (key & 7)) << 3) + (col & 7)]);
+              if (!isfinite(v) && key < seen[c >> 1]) o[n][c] += w[c >> 1] * v;
+            }
+        }
+    }
+#pragma unroll
+    for (int u = 0; u < 2; ++u)
+      if (part[u] >= 0) {
+        float* dst = s.part + part[u] * D + db * 16 + 2 * tq;
+        *reinterpret_cast<float2*>(dst) = make_float2(o[0][2 * u], o[0][2 * u + 1]);
+        *reinterpret_cast<float2*>(dst + 8) = make_float2(o[1][2 * u], o[1][2 * u + 1]);
+      }
+  }
+}
+
+// A warp per (token, head) of a slab: the partial results of the token's pages, in the order of its list.
+template <int D>
+__global__ void __launch_bounds__(256)
+pages_join_kernel(__nv_bfloat16* __restrict__ out, const Pages p, const Slabs s, int slab) {
+  pdl_enter();
+  constexpr int E = D / 32;                                 // elements a lane
+  const int lane = threadIdx.x & 31, group = p.H / p.Hkv;
+  const int g0 = slab / s.chunks * s.heads, t0 = slab % s.chunks * s.tokens;
+  const int heads = min(s.heads, p.Hkv - g0) * group;
+  const int64_t w = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
+  const int tl = (int)(w / heads), hl = (int)(w % heads), t = t0 + tl;
+  if (tl >= s.tokens || t >= p.T) return;
+  const int gl = hl / group, h = hl % group;
+  const int* rank = s.rank + ((int64_t)t * p.Hkv + g0 + gl) * p.top;
+  const int64_t pair0 = ((int64_t)gl * s.tokens + tl) * p.top;
+  if (rank[0] == -2) return;                                // behind the last request
+  float M = -INFINITY;
+  for (int i = lane; i < p.top; i += 32)
+    if (rank[i] >= 0) M = fmaxf(M, s.ml[((pair0 + i) * group + h) * 2]);
+  M = warp_max(M);
+  const float base = M == -INFINITY ? 0.f : M;
+  float L = 0.f, acc[E] = {};
+  for (int i0 = 0; i0 < p.top; i0 += 32) {
+    float f = 0.f, l = 0.f;
+    const bool in = i0 + lane < p.top && rank[i0 + lane] >= 0;
+    if (in) {
+      const float2 ml = *reinterpret_cast<const float2*>(s.ml + ((pair0 + i0 + lane) * group + h) * 2);
+      f = fast_exp2(ml.x - base);
+      l = f * ml.y;
+    }
+    L += warp_sum(l);
+    unsigned mask = __ballot_sync(0xffffffffu, in);
+    const float* src = s.part + ((pair0 + i0) * group + h) * D + lane * E;
+#pragma unroll 8
+    for (; mask; mask &= mask - 1) {
+      const int i = __ffs(mask) - 1;
+      const float w_i = __shfl_sync(0xffffffffu, f, i);
+      struct alignas(E * 4) Vec { float v[E]; };
+      const Vec x = *reinterpret_cast<const Vec*>(src + (int64_t)i * group * D);
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[e] = fmaf(w_i, x.v[e], acc[e]);
+    }
+  }
+  const float inv = L == 0.f ? 0.f : 1.f / L;
+  __nv_bfloat16* dst = out + (int64_t)t * p.ldo + (int64_t)(g0 + gl) * group * D + (int64_t)h * D + lane * E;
+#pragma unroll
+  for (int e = 0; e < E; e += 2) *reinterpret_cast<unsigned*>(dst + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+}
+
+template <int D, int P>
+int run_portions(const void* q, void* out, const void* cache, const Pages& p, const Slabs& s, cudaStream_t stream) {
+  auto kernel = pages_portion_kernel<D, P>;
+  constexpr int smem = 2 * P * D * 2;
+  if (smem > 48 * 1024) {
+    static thread_local int set_for = -1;
+    int dev = 0;
+    cudaGetDevice(&dev);
+    if (set_for != dev) {
+      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+        return cuda_status("attention_pages: shared memory");
+      set_for = dev;
+    }
+  }
+  if (cudaMemsetAsync(s.counts, 0, s.zeroed, stream) != cudaSuccess) return cuda_status("attention_pages: counters");
+  launch_pdl(pages_count_kernel, dim3(p.T), dim3(256), 0, stream, p, s);
+  launch_pdl(pages_lists_kernel, dim3((unsigned)(((int64_t)s.count * s.keys + 255) / 256)), dim3(256), 0, stream, p, s);
+  launch_pdl(pages_fill_kernel, dim3(p.T), dim3(256), 0, stream, p, s);
+  const int64_t joined = ((int64_t)s.tokens * s.heads * (p.H / p.Hkv) + 7) / 8;
+  for (int i = 0; i < s.count; ++i) {
+    launch_pdl(kernel, dim3((unsigned)s.tiles), dim3(PORTION_NT), smem, stream, (const __nv_bfloat16*)q, (const __nv_bfloat16*)cache, p, s, i);
+    launch_pdl(pages_join_kernel<D>, dim3((unsigned)joined), dim3(256), 0, stream, (__nv_bfloat16*)out, p, s, i);
+  }
+  return cuda_status("attention_pages (portions)");
+}
+
 // Whether the tensor-core kernels take the call: rows that 16-byte loads and pair stores address, sizes they are made for.
 bool tensor_cores(const void* q, const void* out, const void* cache, const Pages& p) {
   const int group = p.H / p.Hkv;
@@ -390,20 +774,37 @@ bool tensor_cores(const void* q, const void* out, const void* cache, const Pages
 }
 }  // namespace
 
+// Bytes of workspace with which the call takes its portions' form (any smaller one: token by token).
+DINFER_API int64_t dinfer_attention_pages_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D) {
+  if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > 16 || top <= 0 || width <= 0 || num_reqs <= 0 || D <= 0) return 0;
+  Pages p{};
+  p.width = width; p.num_reqs = num_reqs; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.D = D;
+  if ((int64_t)Hkv * num_reqs * width > MAX_COUNTERS) return 0;
+  const Slabs s = slabs_of(p, nullptr);
+  return (int64_t)s.count * s.keys > MAX_COUNTERS ? 0 : s.bytes;
+}
+
 // chosen int32 [T, Hkv, top]; cache [num_pages, 2, Hkv, page_size, D].
 DINFER_API int dinfer_attention_pages(const void* q, int64_t ldq, void* out, int64_t ldo, const void* cache, int num_pages,
                                       const int* table, int width, const int* cu_seqlens, int num_reqs, const int* positions,
                                       const int* chosen, int top, int T, int H, int Hkv, int D, int page_size, float scale,
-                                      int sms, int dtype, cudaStream_t stream) {
+                                      void* workspace, int64_t workspace_bytes, int sms, int dtype, cudaStream_t stream) {
   if (T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 512 || page_size <= 0 || num_reqs <= 0 || top <= 0 || width < 0)
     return refuse(DINFER_BAD_ARGUMENT, "attention_pages: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d", T, H, Hkv, D, page_size, top);
   if ((H + WARPS - 1) / WARPS > 65535) return refuse(DINFER_BAD_ARGUMENT, "attention_pages: %d heads", H);
   if (T == 0) return DINFER_OK;
   const Pages p{ldq, ldo, num_pages, table, width, cu_seqlens, num_reqs, positions, chosen, top, T, H, Hkv, D, page_size, scale};
-  // CTAs that share a token's keys: as far as all run at the same time (two an SM), each with a tile of its own at least
-  int splits = 1;
-  while (splits < 8 && (int64_t)T * Hkv * splits * 2 <= 2 * sms && splits * 2 * BN <= (int64_t)top * page_size) splits *= 2;
   if (dtype == DINFER_BF16 && tensor_cores(q, out, cache, p)) {
+    const int64_t need = workspace ? dinfer_attention_pages_workspace(num_reqs, width, top, T, H, Hkv, D) : 0;
+    if (need > 0 && workspace_bytes >= need) {
+      const Slabs s = slabs_of(p, (unsigned char*)workspace);
+#define DINFER_PAGES(P_) case P_: return D == 128 ? run_portions<128, P_>(q, out, cache, p, s, stream) : run_portions<64, P_>(q, out, cache, p, s, stream)
+      switch (page_size) { DINFER_PAGES(16); DINFER_PAGES(32); DINFER_PAGES(64); DINFER_PAGES(128); }
+#undef DINFER_PAGES
+    }
+    // CTAs that share a token's keys: as far as all run at the same time (two an SM), each with a tile of its own at least
+    int splits = 1;
+    while (splits < 8 && (int64_t)T * Hkv * splits * 2 <= 2 * sms && splits * 2 * BN <= (int64_t)top * page_size) splits *= 2;
     if (D == 128) return H / Hkv <= 8 ? run_token<128, 1>(q, out, cache, p, splits, stream) : run_token<128, 2>(q, out, cache, p, splits, stream);
     return H / Hkv <= 8 ? run_token<64, 1>(q, out, cache, p, splits, stream) : run_token<64, 2>(q, out, cache, p, splits, stream);
   }

@@ -17,8 +17,19 @@ from typing import Optional
 
 import torch
 
-from .lib import DTYPE_CODE, KernelError, check, dtype_code, num_sms, ptr, require_cuda, stream_handle
+from .lib import DTYPE_CODE, KernelError, check, dtype_code, library, num_sms, ptr, require_cuda, stream_handle
 from .ops import _fn
+
+
+# Steps of at least so many tokens turn the attention round: pages meet the tokens that chose them, through a workspace.
+PORTION_TOKENS = 64
+
+
+def _workspace(num_reqs: int, width: int, top: int, T: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
+    """Bytes that the portions' form needs (0: it does not take these sizes)."""
+    f = library("attention_pages").dinfer_attention_pages_workspace
+    f.argtypes, f.restype = [c_int] * 7, c_int64
+    return f(num_reqs, width, top, T, num_heads, num_kv_heads, head_dim)
 
 
 def _here(what: str, *tensors) -> None:
@@ -184,10 +195,16 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     _ints(what, chosen=chosen)
     if chosen.dim() != 3 or tuple(chosen.shape[:2]) != (T, Hkv) or chosen.shape[2] == 0:
         raise KernelError(f"{what}: chosen int32 [T, Hkv, top] with top > 0")
+    top = chosen.shape[2]
+    size, work = 0, None
+    if T >= PORTION_TOKENS and q.dtype == torch.bfloat16:
+        size = _workspace(block_table.shape[0], block_table.shape[1], top, T, num_heads, Hkv, D)
+        if size > 0:
+            work = torch.empty(size, dtype=torch.uint8, device=q.device)
     lib, f = _fn("attention_pages", "dinfer_attention_pages",
                  [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                  c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_int, c_int, c_void_p])
+                  c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int, c_int, c_void_p])
     check(lib, f(ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(cache), num_pages, ptr(block_table), block_table.shape[1],
-                 ptr(cu_seqlens), block_table.shape[0], ptr(positions), ptr(chosen), chosen.shape[2], T, num_heads, Hkv, D, page_size,
-                 scale, num_sms(), DTYPE_CODE[q.dtype], stream_handle()), what)
+                 ptr(cu_seqlens), block_table.shape[0], ptr(positions), ptr(chosen), top, T, num_heads, Hkv, D, page_size,
+                 scale, ptr(work), size, num_sms(), DTYPE_CODE[q.dtype], stream_handle()), what)
     return out
