@@ -6,21 +6,49 @@
 // Choice: per (token, key head) the first `first` pages, the last `recent` ones up to the token's own, and of the pages between
 // the best-scored, `top` in all; of equal scores the lower page, what is not a number behind every number.  Ascending, -1 behind
 // the last.
-#include "common.cuh"
+#include "mma_tiles.cuh"
 
 using namespace dinfer;
+using namespace dinfer_mma;
 
 namespace {
 
-// last r with cu_seqlens[r] <= t (requests without tokens are passed over), -1 behind the last request's tokens
+// The request of token t: the first whose tokens end behind it (every lane of a full warp asks; requests without tokens are passed
+// over), -1 where there is none.
 __device__ __forceinline__ int request_of(const int* cu, int num_reqs, int t) {
-  if (t >= cu[num_reqs] || t < cu[0]) return -1;
-  int lo = 0, hi = num_reqs - 1;
-  while (lo < hi) {
-    const int mid = (lo + hi + 1) >> 1;
-    if (cu[mid] <= t) lo = mid; else hi = mid - 1;
+  int ended = 0;
+  for (int i0 = 0; i0 < num_reqs; i0 += 32) {
+    const int i = i0 + (threadIdx.x & 31);
+    ended += __popc(__ballot_sync(0xffffffffu, i < num_reqs && cu[i + 1] <= t));
   }
-  return lo;
+  return ended < num_reqs && t >= cu[0] ? ended : -1;
+}
+
+// The token tile `y` of a batch whose requests are cut into runs of up to `tile` tokens: its request, first token and tokens (every
+// lane of a full warp asks); request -1 beyond the last tile.
+__device__ __forceinline__ int3 token_tile(const int* cu, int num_reqs, int tile, int y) {
+  const int lane = threadIdx.x & 31;
+  int before = 0;
+  for (int i0 = 0; i0 < num_reqs; i0 += 32) {
+    const int i = i0 + lane;
+    const int begin = i < num_reqs ? cu[i] : 0, tokens = i < num_reqs ? cu[i + 1] - begin : 0;
+    const int n = (tokens + tile - 1) / tile;
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, y >= before + incl - n && y < before + incl);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int at = y - before - __shfl_sync(0xffffffffu, incl - n, src);
+      const int b = __shfl_sync(0xffffffffu, begin, src), k = __shfl_sync(0xffffffffu, tokens, src);
+      return make_int3(i0 + src, b + at * tile, min(tile, k - at * tile));
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return make_int3(-1, 0, 0);
 }
 
 constexpr int WARPS = 8;
@@ -52,6 +80,99 @@ page_scores_kernel(const T* __restrict__ q, int64_t ldq, const T* __restrict__ m
       }
     }
     if (lane == 0) row[j] = best;
+  }
+}
+
+__device__ __forceinline__ float max_nan(float a, float b) {        // NaN where one of the two is
+  float r;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(r) : "f"(a), "f"(b));
+  return r;
+}
+
+// Bfloat16, head sizes 64 and 128, groups of up to 16 heads: a warp holds the means of 32 pages of a (request, key head) as the
+// A operand of mma.sync and runs the tokens of its tile past them, eight columns (tokens x heads, the group filled up to a power of two
+// with its last head) at a time.  Both operands go from memory straight into registers: the order of the elements of a sum is free, so a lane
+// takes 16 bytes of its rows at the same places, two steps of 16 elements at once.  The maximum over the heads is taken in the columns.
+constexpr int TILE_TOKENS = 64;
+
+template <int D, int GP>             // GP: the group, filled up to a power of two
+__global__ void __launch_bounds__(WARPS * 32)
+page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const __nv_bfloat16* __restrict__ means, int num_pages,
+                       const int* __restrict__ table, int width, const int* __restrict__ cu, int num_reqs,
+                       const int* __restrict__ positions, float* __restrict__ out, int64_t ldt, int64_t ldg, int group, int Hkv,
+                       int page_size, int pages) {
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
+  const int g = blockIdx.y, j0 = (blockIdx.z * WARPS + warp) * 32;
+  if (j0 >= pages) return;
+  const int3 tile = token_tile(cu, num_reqs, TILE_TOKENS, blockIdx.x);
+  if (tile.x < 0) return;
+  constexpr int NT8 = GP > 8 ? GP / 8 : 1;                 // products of eight columns a step
+  constexpr int STEP = GP > 8 ? 1 : 8 / GP;                // tokens of a step
+  // rows gr + {0, 8, 16, 24}: pages j0 + ...; a page that is not held scores -inf
+  unsigned held = 0;
+  uint4 a[4][D / 32];
+#pragma unroll
+  for (int u = 0; u < 4; ++u) {
+    const int j = j0 + gr + 8 * u;
+    const int page = j < pages ? table[(int64_t)tile.x * width + j] : -1;
+    const bool ok = page >= 0 && page < num_pages;
+    const __nv_bfloat16* row = means + ((int64_t)(ok ? page : 0) * Hkv + g) * D + tq * 8;
+#pragma unroll
+    for (int k = 0; k < D / 32; ++k) a[u][k] = ok ? *reinterpret_cast<const uint4*>(row + k * 32) : make_uint4(0, 0, 0, 0);
+    held |= (ok ? 1u : 0u) << u;
+  }
+  auto load_q = [&](int i, uint4 (&b)[NT8][D / 32]) {
+    const int t = tile.y + min(i + gr / GP, tile.z - 1);
+#pragma unroll
+    for (int n = 0; n < NT8; ++n) {
+      const int h = min(GP > 8 ? n * 8 + gr : gr % GP, group - 1);
+      const __nv_bfloat16* row = q + (int64_t)t * ldq + (int64_t)(g * group + h) * D + tq * 8;
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k) b[n][k] = *reinterpret_cast<const uint4*>(row + k * 32);
+    }
+  };
+  uint4 b[NT8][D / 32];
+  load_q(0, b);
+  for (int i = 0; i < tile.z; i += STEP) {
+    float c[2][4];
+#pragma unroll
+    for (int n = 0; n < NT8; ++n) {
+      float d[2][4] = {};
+#pragma unroll
+      for (int k = 0; k < D / 32; ++k)
+#pragma unroll
+        for (int m = 0; m < 2; ++m) {
+          mma_bf16(d[m], a[2 * m][k].x, a[2 * m + 1][k].x, a[2 * m][k].y, a[2 * m + 1][k].y, b[n][k].x, b[n][k].y);
+          mma_bf16(d[m], a[2 * m][k].z, a[2 * m + 1][k].z, a[2 * m][k].w, a[2 * m + 1][k].w, b[n][k].z, b[n][k].w);
+        }
+#pragma unroll
+      for (int m = 0; m < 2; ++m)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) c[m][e] = n == 0 ? d[m][e] : max_nan(c[m][e], d[m][e]);
+    }
+    if (i + STEP < tile.z) load_q(i + STEP, b);
+    // columns 2tq and 2tq + 1 -> tokens
+    constexpr int MINE = GP == 1 ? 2 : 1;                  // tokens a lane writes
+#pragma unroll
+    for (int w = 0; w < MINE; ++w) {
+      const int at = i + (GP >= 8 ? 0 : 2 * tq / GP) + w;
+      const int t = tile.y + min(at, tile.z - 1);
+      const int full = min(positions[t] / page_size, pages);
+      const bool writes = at < tile.z && (GP >= 8 ? tq == 0 : 2 * tq % GP == 0);
+      float* row = out + (int64_t)t * ldt + (int64_t)g * ldg + j0;
+#pragma unroll
+      for (int v = 0; v < 4; ++v) {                        // rows gr + 8 v
+        float x = c[v / 2][2 * (v & 1) + w];
+        if (GP > 1) {
+          x = max_nan(x, c[v / 2][2 * (v & 1) + 1]);
+          if (GP >= 4) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, 1));
+          if (GP >= 8) x = max_nan(x, __shfl_xor_sync(0xffffffffu, x, 2));
+        }
+        const int j = gr + 8 * v;
+        if (writes && j0 + j < pages) row[j] = (held >> v & 1) && j0 + j < full ? x : -INFINITY;
+      }
+    }
   }
 }
 
@@ -110,6 +231,196 @@ choose_pages_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
   for (int i = at + lane; i < top; i += 32) dst[i] = -1;
 }
 
+// Up to 2048 pages: a warp per (token, key head) with the candidates' orders in registers (page lo + 32 i + lane), read once.
+// Wanted is the order of the last pick.  Up to 32 picks: the picks-th largest of the lanes' own maxima is a bound that few
+// candidates reach; those are ranked against one another in shared memory.  Where many reach it (or more picks are wanted) the order
+// is found bit by bit, counting.  The picks then come out in ascending order, candidates of the last pick's order from the lowest on.
+constexpr int SHORT_LIST = 64;
+
+template <int NPL>
+__global__ void __launch_bounds__(WARPS * 32)
+choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, const int* __restrict__ positions, int page_size,
+                        int first, int recent, int top, int pages, int* __restrict__ out, int64_t rows, int Hkv) {
+  __shared__ __align__(16) unsigned s_list[WARPS][SHORT_LIST];
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = (int64_t)blockIdx.x * WARPS + warp;
+  if (row >= rows) return;
+  const int t = (int)(row / Hkv), g = (int)(row % Hkv);
+  const int pos = positions[t];
+  const int own = pos < 0 ? -1 : min(pos / page_size, pages - 1);
+  const int lo = min(first, own + 1), hi = max(own + 1 - recent, lo);   // candidates are [lo, hi)
+  const int picks = min(top - lo - (own + 1 - hi), hi - lo);
+  int* dst = out + row * top;
+  unsigned last = 0;                                         // the order of the last pick
+  int equal = 0;                                             // picks of just that order
+  unsigned key[NPL];
+  const bool all = picks == hi - lo;
+  if (!all && picks > 0) {
+    const float* s = scores + (int64_t)t * ldt + (int64_t)g * ldg;
+    float x[NPL];
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) x[i] = lo + 32 * i + lane < hi ? s[lo + 32 * i + lane] : 0.f;
+    unsigned best = 0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      key[i] = lo + 32 * i + lane < hi ? order_of(x[i]) + 1u : 0u;       // 0: no candidate
+      best = max(best, key[i]);
+    }
+    bool found = false;
+    if (picks <= 32) {
+      // how many lanes have a larger maximum (or an equal one and a lower number); the picks-th gives the bound
+      int before = 0;
+#pragma unroll
+      for (int o = 1; o < 32; ++o) {
+        const unsigned other = __shfl_sync(0xffffffffu, best, (lane + o) & 31);
+        before += other > best || (other == best && ((lane + o) & 31) < lane);
+      }
+      const unsigned bound = __shfl_sync(0xffffffffu, best, __ffs(__ballot_sync(0xffffffffu, before == picks - 1)) - 1);
+      int n = 0;
+      if (bound > 0) {
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) {
+          const unsigned in = __ballot_sync(0xffffffffu, key[i] >= bound);
+          const int at = n + __popc(in & ((1u << lane) - 1));
+          if (key[i] >= bound && at < SHORT_LIST) s_list[warp][at] = key[i];
+          n += __popc(in);
+        }
+        found = n <= SHORT_LIST;
+      }
+      if (found) {
+        for (int i = n + lane; i < (n + 3) / 4 * 4; i += 32) s_list[warp][i] = 0;
+        __syncwarp();
+        const unsigned a = lane < n ? s_list[warp][lane] : 0, b = lane + 32 < n ? s_list[warp][lane + 32] : 0;
+        int above_a = 0, above_b = 0, same_a = 0, same_b = 0;
+        for (int i = 0; i < n; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(&s_list[warp][i]);
+          above_a += (v.x > a) + (v.y > a) + (v.z > a) + (v.w > a);
+          same_a += (v.x == a) + (v.y == a) + (v.z == a) + (v.w == a);
+          above_b += (v.x > b) + (v.y > b) + (v.z > b) + (v.w > b);
+          same_b += (v.x == b) + (v.y == b) + (v.z == b) + (v.w == b);
+        }
+        const bool is_a = a && above_a < picks && above_a + same_a >= picks, is_b = b && above_b < picks && above_b + same_b >= picks;
+        const unsigned ma = __ballot_sync(0xffffffffu, is_a), mb = __ballot_sync(0xffffffffu, is_b);
+        const int src = __ffs(ma ? ma : mb) - 1;
+        last = __shfl_sync(0xffffffffu, ma ? a : b, src);
+        equal = picks - __shfl_sync(0xffffffffu, ma ? above_a : above_b, src);
+      }
+    }
+    if (!found) {                                            // the largest order that at least `picks` candidates reach
+#pragma unroll 1
+      for (int bit = 31; bit >= 0; --bit) {
+        const unsigned tried = last | (1u << bit);
+        int n = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) n += key[i] >= tried;
+        if ((int)__reduce_add_sync(0xffffffffu, (unsigned)n) >= picks) last = tried;
+      }
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) above += key[i] > last;
+      equal = picks - (int)__reduce_add_sync(0xffffffffu, (unsigned)above);
+    }
+  }
+  // ascending: the first pages, the picks, the recent pages
+  for (int j = lane; j < lo; j += 32) dst[j] = j;
+  int at = lo;
+  if (all) {
+    for (int j = lo + lane; j < hi; j += 32) dst[j] = j;
+    at = hi;
+  } else if (picks > 0) {
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const unsigned same = __ballot_sync(0xffffffffu, key[i] == last);
+      const bool in = key[i] > last || (key[i] == last && __popc(same & ((1u << lane) - 1)) < equal);
+      equal = max(0, equal - __popc(same));
+      const unsigned mask = __ballot_sync(0xffffffffu, in);
+      if (in) dst[at + __popc(mask & ((1u << lane) - 1))] = lo + 32 * i + lane;
+      at += __popc(mask);
+    }
+  }
+  for (int j = hi + lane; j <= own; j += 32) dst[at + j - hi] = j;
+  at += own + 1 - hi;
+  for (int i = at + lane; i < top; i += 32) dst[i] = -1;
+}
+
+// More pages, up to 8192: a block per (token, key head), the order of the last pick bit by bit.
+template <int NPL>
+__global__ void __launch_bounds__(WARPS * 32)
+choose_block_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, const int* __restrict__ positions, int page_size,
+                    int first, int recent, int top, int pages, int* __restrict__ out, int Hkv) {
+  __shared__ int s_count[2][WARPS];
+  pdl_enter();
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int64_t row = blockIdx.x;
+  const int t = (int)(row / Hkv), g = (int)(row % Hkv);
+  const int pos = positions[t];
+  const int own = pos < 0 ? -1 : min(pos / page_size, pages - 1);
+  const int lo = min(first, own + 1), hi = max(own + 1 - recent, lo);
+  const int picks = min(top - lo - (own + 1 - hi), hi - lo);
+  int* dst = out + row * top;
+  const float* s = scores + (int64_t)t * ldt + (int64_t)g * ldg;
+  int turn = 0;
+  auto total = [&](int n, int* before) {                     // of the block; before: of the warps below
+    n = (int)__reduce_add_sync(0xffffffffu, (unsigned)n);
+    if (lane == 0) s_count[turn][warp] = n;
+    __syncthreads();
+    int sum = 0, below = 0;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      if (w == warp) below = sum;
+      sum += s_count[turn][w];
+    }
+    if (before) *before = below;
+    turn ^= 1;                                               // (the next sum's writes meet nobody still reading this one's)
+    return sum;
+  };
+  for (int j = threadIdx.x; j < lo; j += WARPS * 32) dst[j] = j;
+  int at = lo;
+  if (picks == hi - lo) {
+    for (int j = lo + threadIdx.x; j < hi; j += WARPS * 32) dst[j] = j;
+    at = hi;
+  } else if (picks > 0) {
+    unsigned key[NPL];
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const int j = lo + i * WARPS * 32 + threadIdx.x;
+      key[i] = j < hi ? order_of(s[j]) + 1u : 0u;
+    }
+    unsigned last = 0;
+#pragma unroll 1
+    for (int bit = 31; bit >= 0; --bit) {
+      const unsigned tried = last | (1u << bit);
+      int n = 0;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) n += key[i] >= tried;
+      if (total(n, nullptr) >= picks) last = tried;
+    }
+    int above = 0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) above += key[i] > last;
+    int equal = picks - total(above, nullptr);
+#pragma unroll 1
+    for (int i0 = 0; i0 < NPL; ++i0) {
+      unsigned k = 0;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) k = i == i0 ? key[i] : k;
+      int below;
+      const unsigned same = __ballot_sync(0xffffffffu, k == last);
+      const int sames = total(lane == 0 ? __popc(same) : 0, &below);
+      const bool in = k > last || (k == last && below + __popc(same & ((1u << lane) - 1)) < equal);
+      equal = max(0, equal - sames);
+      const unsigned mask = __ballot_sync(0xffffffffu, in);
+      const int ins = total(lane == 0 ? __popc(mask) : 0, &below);
+      if (in) dst[at + below + __popc(mask & ((1u << lane) - 1))] = lo + i0 * WARPS * 32 + threadIdx.x;
+      at += ins;
+    }
+  }
+  for (int j = hi + threadIdx.x; j <= own; j += WARPS * 32) dst[at + j - hi] = j;
+  at += own + 1 - hi;
+  for (int i = at + threadIdx.x; i < top; i += WARPS * 32) dst[i] = -1;
+}
+
 }  // namespace
 
 // out[t * ldt + g * ldg + j] for j < pages; rows behind the last request's tokens are left as they are.
@@ -121,6 +432,23 @@ DINFER_API int dinfer_page_scores(const void* q, int64_t ldq, const void* means,
                   page_size, pages, width);
   if (T == 0 || pages == 0) return DINFER_OK;
   if (Hkv > 65535) return refuse(DINFER_BAD_ARGUMENT, "page_scores: %d key heads", Hkv);
+  const int group = H / Hkv;
+  const int64_t z = (pages + WARPS * 32 - 1) / (WARPS * 32);
+  if (dtype == DINFER_BF16 && (D == 64 || D == 128) && group <= 16 && ldq % 8 == 0 && ((uintptr_t)q | (uintptr_t)means) % 16 == 0 && z <= 65535) {
+    const int64_t tiles = (int64_t)T / TILE_TOKENS + (num_reqs < T ? num_reqs : T);     // of every way the tokens may be dealt out
+    const dim3 grid((unsigned)tiles, Hkv, (unsigned)z);
+#define DINFER_SCORES(GP)                                                                                                       \
+  launch_pdl(D == 64 ? page_scores_mma_kernel<64, GP> : page_scores_mma_kernel<128, GP>, grid, dim3(WARPS * 32), 0, stream,   \
+             (const __nv_bfloat16*)q, ldq, (const __nv_bfloat16*)means, num_pages, table, width, cu_seqlens, num_reqs,       \
+             positions, out, ldt, ldg, group, Hkv, page_size, pages)
+    if (group == 1) DINFER_SCORES(1);
+    else if (group == 2) DINFER_SCORES(2);
+    else if (group <= 4) DINFER_SCORES(4);
+    else if (group <= 8) DINFER_SCORES(8);
+    else DINFER_SCORES(16);
+#undef DINFER_SCORES
+    return cuda_status("page_scores");
+  }
   DINFER_DISPATCH_DTYPE(dtype, E, {
     launch_pdl(page_scores_kernel<E>, dim3(T, Hkv, min((pages + WARPS - 1) / WARPS, 64)), dim3(WARPS * 32), 0, stream, (const E*)q,
                ldq, (const E*)means, num_pages, table, width, cu_seqlens, num_reqs, positions, out, ldt, ldg, H, Hkv, D,
@@ -137,6 +465,20 @@ DINFER_API int dinfer_choose_pages(const float* scores, int64_t ldt, int64_t ldg
                   page_size, pages, first, recent, top);
   if (T == 0) return DINFER_OK;
   const int64_t rows = (int64_t)T * Hkv;
+  if (pages > 2048 && pages <= 8192 && rows <= 0x7fffffff) {
+    auto kernel = pages <= 4096 ? choose_block_kernel<16> : choose_block_kernel<32>;
+    launch_pdl(kernel, dim3((unsigned)rows), dim3(WARPS * 32), 0, stream, scores, ldt, ldg, positions, page_size, first, recent, top,
+               pages, out, Hkv);
+    return cuda_status("choose_pages");
+  }
+  if (pages <= 2048) {
+    auto kernel = pages <= 128 ? choose_registers_kernel<4> : pages <= 256 ? choose_registers_kernel<8>
+                  : pages <= 512 ? choose_registers_kernel<16> : pages <= 1024 ? choose_registers_kernel<32>
+                  : choose_registers_kernel<64>;
+    launch_pdl(kernel, dim3((unsigned)((rows + WARPS - 1) / WARPS)), dim3(WARPS * 32), 0, stream, scores, ldt, ldg, positions,
+               page_size, first, recent, top, pages, out, rows, Hkv);
+    return cuda_status("choose_pages");
+  }
   launch_pdl(choose_pages_kernel, dim3((unsigned)((rows + WARPS - 1) / WARPS)), dim3(WARPS * 32), 0, stream, scores, ldt, ldg,
              positions, page_size, first, recent, top, pages, out, rows, Hkv);
   return cuda_status("choose_pages");
