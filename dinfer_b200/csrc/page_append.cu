@@ -118,56 +118,49 @@ append_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW* __re
   }
 }
 
-// ---- head sizes 64 and 128, rows on 16-byte boundaries: a lane owns eight consecutive elements of a head (16 lanes a head of
-// 128, 8 a head of 64), the warp takes the token's next heads in turn and has asked for all of them before it works on the first.
-// A rotation partner rot/2 further on is another lane's (one exchange an element), a neighbour the lane's own.  Half of the
-// blocks, the first to start, only make means: a block whose token does not fill a page leaves at once, so that the long ones do not
-// start last.
-// Bound by memory (rows in, rows out).  4096 tokens of 32 + 8 + 8 heads of 128: @APPEND@
-template <typename T> __device__ __forceinline__ void load8(const T* p, float (&v)[8]);
-template <> __device__ __forceinline__ void load8<float>(const float* p, float (&v)[8]) {
-  const float4 a = *reinterpret_cast<const float4*>(p), b = *reinterpret_cast<const float4*>(p + 4);
-  v[0] = a.x; v[1] = a.y; v[2] = a.z; v[3] = a.w; v[4] = b.x; v[5] = b.y; v[6] = b.z; v[7] = b.w;
+// ---- head sizes 64 and 128, rows on 16-byte boundaries, a rotation over a multiple of 8 elements.  A lane owns eight elements of a head
+// (16 lanes a head of 128, 8 a head of 64) as two runs of four, chosen so that the pairs it turns are its own: of the turned part of a
+// neox head elements 4 l + {0..3} and their partners rot/2 further on, elsewhere eight in a row.  A warp asks for several heads
+// before it works on the first.  Bound by memory: the rows once in and once out.  @APPEND@
+template <typename T> struct alignas(4 * sizeof(T)) Vec4 { alignas(4 * sizeof(T)) T v[4]; };
+template <typename T> struct Lane8 { Vec4<T> a, b; };
+template <typename T> __device__ __forceinline__ Lane8<T> load_lane(const T* row, int a, int b) {
+  return {*reinterpret_cast<const Vec4<T>*>(row + a), *reinterpret_cast<const Vec4<T>*>(row + b)};
 }
-template <> __device__ __forceinline__ void load8<__nv_bfloat16>(const __nv_bfloat16* p, float (&v)[8]) {
-  const uint4 x = *reinterpret_cast<const uint4*>(p);
-  const __nv_bfloat162* h = reinterpret_cast<const __nv_bfloat162*>(&x);
-#pragma unroll
-  for (int j = 0; j < 4; ++j) { const float2 f = __bfloat1622float2(h[j]); v[2 * j] = f.x; v[2 * j + 1] = f.y; }
+template <typename T> __device__ __forceinline__ void store_lane(T* row, int a, int b, const Lane8<T>& x) {
+  *reinterpret_cast<Vec4<T>*>(row + a) = x.a;
+  *reinterpret_cast<Vec4<T>*>(row + b) = x.b;
 }
-template <typename T> struct alignas(16) Vec8 { T v[8]; };
-template <typename T> __device__ __forceinline__ void widen8(const Vec8<T>& x, float (&v)[8]) {
+template <typename T> __device__ __forceinline__ void widen(const Lane8<T>& x, float (&v)[8]) {
 #pragma unroll
-  for (int j = 0; j < 8; ++j) v[j] = to_f32<T>(x.v[j]);
+  for (int j = 0; j < 4; ++j) { v[j] = to_f32<T>(x.a.v[j]); v[4 + j] = to_f32<T>(x.b.v[j]); }
 }
-template <typename T> __device__ __forceinline__ Vec8<T> narrow8(const float (&v)[8]) {
-  Vec8<T> x;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) x.v[j] = from_f32<T>(v[j]);
+template <typename T> __device__ __forceinline__ Lane8<T> narrow(const float (&v)[8]);
+template <> __device__ __forceinline__ Lane8<float> narrow<float>(const float (&v)[8]) {
+  return {{v[0], v[1], v[2], v[3]}, {v[4], v[5], v[6], v[7]}};
+}
+template <> __device__ __forceinline__ Lane8<__nv_bfloat16> narrow<__nv_bfloat16>(const float (&v)[8]) {
+  Lane8<__nv_bfloat16> x;                                      // two at a time
+  __nv_bfloat162 *a = reinterpret_cast<__nv_bfloat162*>(x.a.v), *b = reinterpret_cast<__nv_bfloat162*>(x.b.v);
+  a[0] = __floats2bfloat162_rn(v[0], v[1]); a[1] = __floats2bfloat162_rn(v[2], v[3]);
+  b[0] = __floats2bfloat162_rn(v[4], v[5]); b[1] = __floats2bfloat162_rn(v[6], v[7]);
   return x;
 }
 
-// What a lane holds of the rotation of its eight elements: value * c + partner * s (the sign of the pair's first element in s).
-struct Turn { float c[8], s[8]; };
-
-// `l` the lane's place among the head's lanes.
-__device__ __forceinline__ void load_turn(const float* cs, int rot, int interleaved, int l, Turn& t) {
-  const int half = rot >> 1;
-#pragma unroll
-  for (int j = 0; j < 8; ++j) {
-    const int e = l * 8 + j;
-    const bool in = e < rot;
-    const int i = interleaved ? e >> 1 : (e < half ? e : e - half);
-    const bool first = interleaved ? !(e & 1) : e < half;
-    t.c[j] = in ? cs[i] : 1.f;
-    const float s = in ? cs[half + i] : 0.f;
-    t.s[j] = first ? -s : s;
-  }
+// Where lane l of a head's lanes finds its elements, and the four angles of its pairs.
+struct Place { int a, b; bool turns, neox; };
+__device__ __forceinline__ Place place_of(const Append& p, int l) {
+  const bool turns = l * 8 < p.rot, neox = turns && !p.interleaved;
+  return {neox ? 4 * l : 8 * l, neox ? 4 * l + (p.rot >> 1) : 8 * l + 4, turns, neox};
+}
+__device__ __forceinline__ void load_turn(const float* cs, const Place& at, int rot, int l, float4& c, float4& s) {
+  if (!at.turns) return;                                       // (angles 4 l .. 4 l + 3 in either layout)
+  c = *reinterpret_cast<const float4*>(cs + 4 * l);
+  s = *reinterpret_cast<const float4*>(cs + (rot >> 1) + 4 * l);
 }
 
-// v: the lane's elements (32-bit); w: its norm weights; LANES: lanes of a head
 template <int LANES>
-__device__ __forceinline__ void finish8(float (&v)[8], bool norm, const float (&w)[8], float eps, const Turn& t, int rot, int interleaved) {
+__device__ __forceinline__ void finish(float (&v)[8], bool norm, const float (&w)[8], float eps, const Place& at, const float4& c, const float4& s) {
   if (norm) {
     float ss = 0.f;
 #pragma unroll
@@ -178,120 +171,165 @@ __device__ __forceinline__ void finish8(float (&v)[8], bool norm, const float (&
 #pragma unroll
     for (int j = 0; j < 8; ++j) v[j] = v[j] * rinv * w[j];
   }
-  if (rot == 0) return;
-  const int lane = threadIdx.x & 31, l = lane % LANES;
-  if (interleaved) {
-#pragma unroll
-    for (int j = 0; j < 8; j += 2) {
-      const float a = v[j], b = v[j + 1];
-      if (l * 8 + j >= rot) break;
-      v[j] = fmaf(b, t.s[j], a * t.c[j]);
-      v[j + 1] = fmaf(a, t.s[j + 1], b * t.c[j + 1]);
-    }
+  if (!at.turns) return;
+  auto turn = [](float& x, float& y, float co, float si) {
+    const float a = x, b = y;
+    x = fmaf(a, co, -b * si);
+    y = fmaf(b, co, a * si);
+  };
+  if (at.neox) {
+    turn(v[0], v[4], c.x, s.x); turn(v[1], v[5], c.y, s.y); turn(v[2], v[6], c.z, s.z); turn(v[3], v[7], c.w, s.w);
   } else {
-    const int hop = rot / 16;                                // lanes to the partner
-    const int from = l < hop ? lane + hop : l < 2 * hop ? lane - hop : lane;
-#pragma unroll
-    for (int j = 0; j < 8; ++j) {
-      const float other = __shfl_sync(0xffffffffu, v[j], from);
-      if (l < 2 * hop) v[j] = fmaf(other, t.s[j], v[j] * t.c[j]);
-    }
+    turn(v[0], v[1], c.x, s.x); turn(v[2], v[3], c.y, s.y); turn(v[4], v[5], c.z, s.z); turn(v[6], v[7], c.w, s.w);
   }
 }
 
 constexpr int MAX_PAGE = 128;        // tokens of a page
+constexpr int FEW_TOKENS = 512;
 
-template <typename TA, typename TW, int D>
-__global__ void __launch_bounds__(WARPS * 32)
-append_lanes_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW* __restrict__ q_weight,
-                    const TW* __restrict__ k_weight, TA* cache, TA* __restrict__ means, const Append p) {
-  constexpr int LANES = D / 8, PER = 32 / LANES, AHEAD = 3;     // lanes of a head, heads of a warp at once, turns asked for ahead
-  pdl_enter();
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, side = lane / LANES;
-  const int slot = p.slots[t];
-  const bool kept = slot >= 0 && slot / p.page_size < p.num_pages;
-  const int page = kept ? slot / p.page_size : 0, off = kept ? slot % p.page_size : 0;
-  const int64_t plane = (int64_t)p.Hkv * p.page_size * D;
-  const bool norm = q_weight != nullptr;
-  Turn turn;
-  if (blockIdx.y == 0) {
-    if (!kept || off != p.page_size - 1) return;
-    // the page becomes full: a warp per key head, its groups of lanes take the offsets in turn
-    unsigned brought[MAX_PAGE / 32];                         // offsets whose key this step brings, by distance to the last
+// Of eight tokens from t0 on, those whose slot is a page's last.
+__device__ __forceinline__ unsigned page_ends(const Append& p, int t0, int T, int& slot) {
+  const int lane = threadIdx.x & 31, t = t0 + (lane & 7);
+  slot = t < T ? p.slots[t] : -1;
+  return __ballot_sync(0xffffffffu, lane < 8 && slot >= 0 && slot % p.page_size == p.page_size - 1 && slot / p.page_size < p.num_pages);
+}
+
+// The means of key head g of the pages that the eight tokens from t0 on fill, by a block: its warps' groups of lanes take the offsets
+// in turn and come together in an order that depends on nothing but the page size.  ROWS: keys that this step brings are made again from
+// its rows; else all come from the cache (behind the launch that wrote them).
+template <typename TA, typename TW, int D, bool ROWS>
+__device__ __forceinline__ void make_means(const TA* qkv, const TW* k_weight, const TA* cache, TA* means, int t0, int g, int T, const Append& p) {
+  constexpr int LANES = D / 8, PER = 32 / LANES, AHEAD = 4;
+  __shared__ float s_sum[WARPS][D];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, side = lane / LANES;
+  int slots;
+  unsigned ends = page_ends(p, t0, T, slots);
+  if (!ends) return;
+  const Place at = place_of(p, l);
+  const bool norm = k_weight != nullptr;
+  for (; ends; ends &= ends - 1) {
+    const int from = __ffs(ends) - 1, t = t0 + from, slot = __shfl_sync(0xffffffffu, slots, from), page = slot / p.page_size;
+    const TA* cached = cache + ((int64_t)page * 2 * p.Hkv + g) * p.page_size * D;
+    float sum[8] = {};
+    for (int o0 = warp * PER; o0 < p.page_size; o0 += WARPS * PER * AHEAD) {
+      Lane8<TA> in[AHEAD];
+      bool now[AHEAD];
 #pragma unroll
-    for (int i = 0; i < MAX_PAGE / 32; ++i) {
-      const int back = i * 32 + lane;
-      brought[i] = __ballot_sync(0xffffffffu, back < p.page_size && t - back >= 0 && p.slots[max(t - back, 0)] == slot - back);
-    }
-    float w[8];
-    if (norm) load8<TW>(k_weight + l * 8, w);
-    for (int g = warp; g < p.Hkv; g += WARPS) {
-      float sum[8] = {};
-      const TA* cached = cache + (int64_t)page * 2 * plane + (int64_t)g * p.page_size * D + l * 8;
-#pragma unroll 2
-      for (int o0 = 0; o0 < p.page_size; o0 += PER) {
-        const int o = o0 + side, back = p.page_size - 1 - o;
-        const bool in = o < p.page_size;
-        unsigned word = brought[0];
+      for (int u = 0; u < AHEAD; ++u) {                      // (no branch between the loads: they go out together)
+        const int o = o0 + u * WARPS * PER + side, back = p.page_size - 1 - o;
+        now[u] = ROWS && back >= 0 && t - back >= 0 && p.slots[max(t - max(back, 0), 0)] == slot - back;
+      }
 #pragma unroll
-        for (int i = 1; i < MAX_PAGE / 32; ++i) word = back >> 5 == i ? brought[i] : word;
-        const bool now = in && (word >> (back & 31) & 1);
-        const int u = now ? t - back : t;
-        const TA* src = !in || now ? qkv + (int64_t)u * p.ld + (int64_t)(p.H + g) * D + l * 8 : cached + (int64_t)o * D;
+      for (int u = 0; u < AHEAD; ++u) {
+        const int o = min(o0 + u * WARPS * PER + side, p.page_size - 1);
+        in[u] = load_lane<TA>(now[u] ? qkv + (int64_t)(t - (p.page_size - 1 - o)) * p.ld + (int64_t)(p.H + g) * D : cached + o * D, at.a, at.b);
+      }
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u) {
+        const int o = o0 + u * WARPS * PER + side;
         float v[8];
-        load8<TA>(src, v);
-        if (__any_sync(0xffffffffu, now)) {
-          float x[8];
+        widen<TA>(in[u], v);
+        if (ROWS && __any_sync(0xffffffffu, now[u])) {
+          float w[8], x[8];
+          if (norm) widen<TW>(load_lane<TW>(k_weight, at.a, at.b), w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = v[j];
-          if (p.rot) load_turn(angles(p, u), p.rot, p.interleaved, l, turn);
-          finish8<LANES>(x, norm, w, p.eps, turn, p.rot, p.interleaved);
+          float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+          if (p.rot) load_turn(angles(p, now[u] ? t - (p.page_size - 1 - o) : t), at, p.rot, l, c, s);
+          finish<LANES>(x, norm, w, p.eps, at, c, s);
+          float y[8];
+          widen<TA>(narrow<TA>(x), y);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = now ? to_f32<TA>(from_f32<TA>(x[j])) : v[j];
+          for (int j = 0; j < 8; ++j) v[j] = now[u] ? y[j] : v[j];
         }
+        if (o < p.page_size)
 #pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += in ? v[j] : 0.f;
+          for (int j = 0; j < 8; ++j) sum[j] += v[j];
       }
-#pragma unroll
-      for (int o = LANES; o < 32; o <<= 1)
-#pragma unroll
-        for (int j = 0; j < 8; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
-#pragma unroll
-      for (int j = 0; j < 8; ++j) sum[j] /= (float)p.page_size;
-      if (side == 0) *reinterpret_cast<Vec8<TA>*>(means + ((int64_t)page * p.Hkv + g) * D + l * 8) = narrow8<TA>(sum);
     }
+#pragma unroll
+    for (int o = LANES; o < 32; o <<= 1)
+#pragma unroll
+      for (int j = 0; j < 8; ++j) sum[j] += __shfl_xor_sync(0xffffffffu, sum[j], o);
+    if (side == 0) {
+      *reinterpret_cast<float4*>(&s_sum[warp][at.a]) = make_float4(sum[0], sum[1], sum[2], sum[3]);
+      *reinterpret_cast<float4*>(&s_sum[warp][at.b]) = make_float4(sum[4], sum[5], sum[6], sum[7]);
+    }
+    __syncthreads();
+    if (threadIdx.x < D) {
+      float all = 0.f;
+#pragma unroll
+      for (int w = 0; w < WARPS; ++w) all += s_sum[w][threadIdx.x];
+      means[((int64_t)page * p.Hkv + g) * D + threadIdx.x] = from_f32<TA>(all / (float)p.page_size);
+    }
+    __syncthreads();
+  }
+}
+
+template <typename TA, int D>
+__global__ void __launch_bounds__(WARPS * 32)
+page_means_kernel(const TA* __restrict__ cache, TA* __restrict__ means, int T, const Append p) {
+  pdl_enter();
+  make_means<TA, TA, D, false>(nullptr, nullptr, cache, means, blockIdx.x * 8, blockIdx.y, T, p);
+}
+
+// WPT: warps that share a token's heads.  MEANS: the first `mean_blocks` blocks make the means, from this step's rows and the cache.
+template <typename TA, typename TW, int D, int WPT, bool MEANS>
+__global__ void __launch_bounds__(WARPS * 32, MEANS ? 2 : 4)
+append_lanes_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW* __restrict__ q_weight,
+                    const TW* __restrict__ k_weight, TA* cache, TA* __restrict__ means, int T, int mean_blocks, const Append p) {
+  // lanes of a head, heads of a warp at once, heads asked for ahead
+  constexpr int LANES = D / 8, PER = 32 / LANES, AHEAD = 3;
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, side = lane / LANES;
+  const int64_t plane = (int64_t)p.Hkv * p.page_size * D;
+  const bool norm = q_weight != nullptr;
+  const Place at = place_of(p, l);
+  float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
+  if (MEANS && (int)blockIdx.x < mean_blocks) {
+    make_means<TA, TW, D, true>(qkv, k_weight, cache, means, blockIdx.x / p.Hkv * 8, blockIdx.x % p.Hkv, T, p);
     return;
   }
+  const int t = ((int)blockIdx.x - mean_blocks) * (WARPS / WPT) + warp / WPT;
+  if (t >= T) return;
+  // everything that waits for nothing goes out first: slot, position, the first heads, the weights; then the angles
+  const int slot = p.slots[t], pos = p.rot ? p.positions[t] : 0;
   const int heads = p.H + 2 * p.Hkv;
-  const TA* row = qkv + (int64_t)t * p.ld + l * 8;
-  float wq[8], wk[8];
-  if (norm) { load8<TW>(q_weight + l * 8, wq); load8<TW>(k_weight + l * 8, wk); }
-  if (p.rot) load_turn(angles(p, t), p.rot, p.interleaved, l, turn);
-  for (int h0 = warp * PER; h0 < heads; h0 += WARPS * PER * AHEAD) {
-    Vec8<TA> in[AHEAD];
+  const TA* row = qkv + (int64_t)t * p.ld;
+  const int first = warp % WPT * PER + side;
+  Lane8<TA> in[AHEAD];
+  auto load = [&](int h0) {
+#pragma unroll
+    for (int u = 0; u < AHEAD; ++u)                            // (no branch between the loads)
+      in[u] = load_lane<TA>(row + min(h0 + u * WPT * PER, heads - 1) * D, at.a, at.b);
+  };
+  load(first);
+  Lane8<TW> wq, wk;
+  if (norm) {
+    wq = load_lane<TW>(q_weight, at.a, at.b);
+    wk = load_lane<TW>(k_weight, at.a, at.b);
+  }
+  if (p.rot) load_turn(p.cos_sin + (int64_t)(pos >= 0 && pos < p.table_rows ? pos : 0) * p.rot, at, p.rot, l, c, s);
+  const int page = slot / p.page_size, off = slot - page * p.page_size;
+  const bool kept = slot >= 0 && page < p.num_pages;
+  TA* q_row = q_out + (int64_t)t * p.ldq;
+  TA* c_row = cache + (kept ? (int64_t)page * 2 * plane + (int64_t)off * D : 0);
+  const int head_step = p.page_size * D;                       // (the values follow the keys as key heads Hkv on)
+  for (int h0 = first; h0 - side < heads; h0 += WPT * PER * AHEAD) {
+    if (h0 != first) load(h0);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int head = h0 + u * WARPS * PER + side;
-      if (head < heads) in[u] = *reinterpret_cast<const Vec8<TA>*>(row + (int64_t)head * D);
-    }
-#pragma unroll
-    for (int u = 0; u < AHEAD; ++u) {
-      if (h0 + u * WARPS * PER >= heads) break;              // (the whole warp alike)
-      const int head = h0 + u * WARPS * PER + side;
-      float v[8];
-      widen8<TA>(in[u], v);
-      float w[8];
-#pragma unroll
-      for (int j = 0; j < 8; ++j) w[j] = head < p.H ? wq[j] : wk[j];
-      finish8<LANES>(v, norm, w, p.eps, turn, p.rot, p.interleaved);
-      if (head < p.H) {
-        *reinterpret_cast<Vec8<TA>*>(q_out + (int64_t)t * p.ldq + (int64_t)head * D + l * 8) = narrow8<TA>(v);
-      } else if (head < heads && kept) {
-        const bool key = head < p.H + p.Hkv;
-        const int g = key ? head - p.H : head - p.H - p.Hkv;
-        TA* dst = cache + ((int64_t)page * 2 + (key ? 0 : 1)) * plane + ((int64_t)g * p.page_size + off) * D + l * 8;
-        *reinterpret_cast<Vec8<TA>*>(dst) = key ? narrow8<TA>(v) : in[u];
+      const int head = h0 + u * WPT * PER;
+      if (head - side >= heads) break;                         // (the whole warp alike)
+      if (head - side < p.H + p.Hkv) {                         // values are left as they are
+        float v[8], w[8];
+        widen<TA>(in[u], v);
+        if (norm) widen<TW>(head < p.H ? wq : wk, w);
+        finish<LANES>(v, norm, w, p.eps, at, c, s);
+        if (head < p.H + p.Hkv) in[u] = narrow<TA>(v);
       }
+      if (head < p.H) store_lane<TA>(q_row + head * D, at.a, at.b, in[u]);
+      else if (head < heads && kept) store_lane<TA>(c_row + (int64_t)(head - p.H) * head_step, at.a, at.b, in[u]);
     }
   }
 }
@@ -299,12 +337,20 @@ append_lanes_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW
 template <typename TA, typename TW>
 int run(const void* qkv, void* q_out, const void* qw, const void* kw, void* cache, void* means, const Append& p, int T,
         cudaStream_t stream) {
-  const bool aligned = ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)qw | (uintptr_t)kw | (uintptr_t)cache | (uintptr_t)means) % 16 == 0 &&
+  const bool aligned = ((uintptr_t)qkv | (uintptr_t)q_out | (uintptr_t)qw | (uintptr_t)kw | (uintptr_t)cache | (uintptr_t)means | (uintptr_t)p.cos_sin) % 16 == 0 &&
                        p.ld % 8 == 0 && p.ldq % 8 == 0;
-  if (aligned && (p.D == 64 || p.D == 128) && p.page_size <= MAX_PAGE && (p.interleaved || p.rot % 16 == 0)) {
-    auto kernel = p.D == 64 ? append_lanes_kernel<TA, TW, 64> : append_lanes_kernel<TA, TW, 128>;
-    launch_pdl(kernel, dim3(T, 2), dim3(WARPS * 32), 0, stream, (const TA*)qkv, (TA*)q_out, (const TW*)qw, (const TW*)kw,
-               (TA*)cache, (TA*)means, p);
+  if (aligned && (p.D == 64 || p.D == 128) && p.page_size <= MAX_PAGE && p.rot % 8 == 0 && p.Hkv <= 65535) {
+    // few tokens: a block each, so that a token's heads are all under way at once; many: a warp's start (slot, angles, weights) is
+    // paid for a quarter of a token's heads
+    const bool few = T <= FEW_TOKENS;
+    auto kernel = few ? (p.D == 64 ? append_lanes_kernel<TA, TW, 64, 8, true> : append_lanes_kernel<TA, TW, 128, 8, true>)
+                      : (p.D == 64 ? append_lanes_kernel<TA, TW, 64, 4, false> : append_lanes_kernel<TA, TW, 128, 4, false>);
+    const int mean_blocks = few ? (T + 7) / 8 * p.Hkv : 0, per = few ? 1 : WARPS / 4;
+    launch_pdl(kernel, dim3(mean_blocks + (T + per - 1) / per), dim3(WARPS * 32), 0, stream, (const TA*)qkv, (TA*)q_out, (const TW*)qw,
+               (const TW*)kw, (TA*)cache, (TA*)means, T, mean_blocks, p);
+    if (!few)
+      launch_pdl(p.D == 64 ? page_means_kernel<TA, 64> : page_means_kernel<TA, 128>, dim3((T + 7) / 8, p.Hkv), dim3(WARPS * 32), 0, stream,
+                 (const TA*)cache, (TA*)means, T, p);
     return cuda_status("page_append");
   }
   launch_pdl(append_kernel<TA, TW>, dim3(T), dim3(WARPS * 32), 0, stream, (const TA*)qkv, (TA*)q_out, (const TW*)qw,

@@ -178,9 +178,9 @@ page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const _
 
 // Scores as whole numbers of the same order; 0 for what is not a number, 1 for -inf.
 __device__ __forceinline__ unsigned order_of(float s) {
-  if (s != s) return 0u;
-  const unsigned b = __float_as_uint(s + 0.f);                // -0 counts as 0
-  return (b & 0x80000000u ? ~b : b | 0x80000000u) - 0x007fffffu + 1u;
+  const int b = __float_as_int(s + 0.f);                      // -0 counts as 0
+  const unsigned k = (unsigned)(b ^ ((b >> 31) | (int)0x80000000)) - 0x007ffffeu;
+  return s == s ? k : 0u;
 }
 
 // Any sizes: a warp per (token, key head), the best of the rest again and again.
@@ -232,113 +232,117 @@ choose_pages_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
 }
 
 // Up to 2048 pages: a warp per (token, key head) with the candidates' orders in registers (page lo + 32 i + lane), read once.
-// Wanted is the order of the last pick.  Up to 32 picks: the picks-th largest of the lanes' own maxima is a bound that few
-// candidates reach; those are ranked against one another in shared memory.  Where many reach it (or more picks are wanted) the order
-// is found bit by bit, counting.  The picks then come out in ascending order, candidates of the last pick's order from the lowest on.
+// First a bound that few more candidates reach than there are picks, to the upper 16 bits: up to 32 picks by the lanes' own maxima
+// (as many lanes as picks reach it), else counted over all.  The candidates that reach it go to a list in shared memory in ascending
+// order and are ranked against one another; a pick's place among the picks is its place in the list.  Where too many reach the bound
+// (equal scores) the order of the last pick is found bit by bit, and of the candidates of that order the lowest are taken.
+// Bound by instructions: @CHOOSE@
 constexpr int SHORT_LIST = 64;
 
 template <int NPL>
 __global__ void __launch_bounds__(WARPS * 32)
 choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, const int* __restrict__ positions, int page_size,
-                        int first, int recent, int top, int pages, int* __restrict__ out, int64_t rows, int Hkv) {
-  __shared__ __align__(16) unsigned s_list[WARPS][SHORT_LIST];
+                        int first, int recent, int top, int pages, int* __restrict__ out, int rows, int Hkv) {
+  __shared__ __align__(16) unsigned s_key[WARPS][SHORT_LIST];
+  __shared__ int s_page[WARPS][SHORT_LIST];
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-  const int64_t row = (int64_t)blockIdx.x * WARPS + warp;
+  const int row = blockIdx.x * WARPS + warp;
   if (row >= rows) return;
-  const int t = (int)(row / Hkv), g = (int)(row % Hkv);
+  const int t = row / Hkv, g = row % Hkv;
   const int pos = positions[t];
   const int own = pos < 0 ? -1 : min(pos / page_size, pages - 1);
   const int lo = min(first, own + 1), hi = max(own + 1 - recent, lo);   // candidates are [lo, hi)
   const int picks = min(top - lo - (own + 1 - hi), hi - lo);
-  int* dst = out + row * top;
-  unsigned last = 0;                                         // the order of the last pick
-  int equal = 0;                                             // picks of just that order
-  unsigned key[NPL];
-  const bool all = picks == hi - lo;
-  if (!all && picks > 0) {
-    const float* s = scores + (int64_t)t * ldt + (int64_t)g * ldg;
-    float x[NPL];
+  int* dst = out + (int64_t)row * top;
+  const unsigned below = (1u << lane) - 1;
+  int at = lo;
+  for (int j = lane; j < lo; j += 32) dst[j] = j;
+  if (picks == hi - lo) {
+    for (int j = lo + lane; j < hi; j += 32) dst[j] = j;
+    at = hi;
+  } else if (picks > 0) {
+    const float* s = scores + (int64_t)t * ldt + (int64_t)g * ldg + lo + lane;
+    unsigned key[NPL], best = 0;                             // 0: no candidate
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) x[i] = lo + 32 * i + lane < hi ? s[lo + 32 * i + lane] : 0.f;
-    unsigned best = 0;
+    for (int i = 0; i < NPL; ++i) key[i] = __float_as_uint(lo + 32 * i + lane < hi ? s[32 * i] : 0.f);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      key[i] = lo + 32 * i + lane < hi ? order_of(x[i]) + 1u : 0u;       // 0: no candidate
+      key[i] = lo + 32 * i + lane < hi ? order_of(__uint_as_float(key[i])) + 1u : 0u;
       best = max(best, key[i]);
     }
-    bool found = false;
+    unsigned bound = 0;
     if (picks <= 32) {
-      // how many lanes have a larger maximum (or an equal one and a lower number); the picks-th gives the bound
-      int before = 0;
 #pragma unroll
-      for (int o = 1; o < 32; ++o) {
-        const unsigned other = __shfl_sync(0xffffffffu, best, (lane + o) & 31);
-        before += other > best || (other == best && ((lane + o) & 31) < lane);
+      for (int bit = 31; bit >= 16; --bit) {
+        const unsigned tried = bound | (1u << bit);
+        if (__popc(__ballot_sync(0xffffffffu, best >= tried)) >= picks) bound = tried;
       }
-      const unsigned bound = __shfl_sync(0xffffffffu, best, __ffs(__ballot_sync(0xffffffffu, before == picks - 1)) - 1);
-      int n = 0;
-      if (bound > 0) {
-#pragma unroll
-        for (int i = 0; i < NPL; ++i) {
-          const unsigned in = __ballot_sync(0xffffffffu, key[i] >= bound);
-          const int at = n + __popc(in & ((1u << lane) - 1));
-          if (key[i] >= bound && at < SHORT_LIST) s_list[warp][at] = key[i];
-          n += __popc(in);
-        }
-        found = n <= SHORT_LIST;
-      }
-      if (found) {
-        for (int i = n + lane; i < (n + 3) / 4 * 4; i += 32) s_list[warp][i] = 0;
-        __syncwarp();
-        const unsigned a = lane < n ? s_list[warp][lane] : 0, b = lane + 32 < n ? s_list[warp][lane + 32] : 0;
-        int above_a = 0, above_b = 0, same_a = 0, same_b = 0;
-        for (int i = 0; i < n; i += 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(&s_list[warp][i]);
-          above_a += (v.x > a) + (v.y > a) + (v.z > a) + (v.w > a);
-          same_a += (v.x == a) + (v.y == a) + (v.z == a) + (v.w == a);
-          above_b += (v.x > b) + (v.y > b) + (v.z > b) + (v.w > b);
-          same_b += (v.x == b) + (v.y == b) + (v.z == b) + (v.w == b);
-        }
-        const bool is_a = a && above_a < picks && above_a + same_a >= picks, is_b = b && above_b < picks && above_b + same_b >= picks;
-        const unsigned ma = __ballot_sync(0xffffffffu, is_a), mb = __ballot_sync(0xffffffffu, is_b);
-        const int src = __ffs(ma ? ma : mb) - 1;
-        last = __shfl_sync(0xffffffffu, ma ? a : b, src);
-        equal = picks - __shfl_sync(0xffffffffu, ma ? above_a : above_b, src);
-      }
-    }
-    if (!found) {                                            // the largest order that at least `picks` candidates reach
+    } else {
 #pragma unroll 1
-      for (int bit = 31; bit >= 0; --bit) {
-        const unsigned tried = last | (1u << bit);
+      for (int bit = 31; bit >= 16; --bit) {
+        const unsigned tried = bound | (1u << bit);
         int n = 0;
 #pragma unroll
         for (int i = 0; i < NPL; ++i) n += key[i] >= tried;
-        if ((int)__reduce_add_sync(0xffffffffu, (unsigned)n) >= picks) last = tried;
+        if ((int)__reduce_add_sync(0xffffffffu, (unsigned)n) >= picks) bound = tried;
+      }
+    }
+    bound = max(bound, 1u);
+    int n = 0;
+#pragma unroll
+    for (int i = 0; i < NPL; ++i) {
+      const unsigned in = __ballot_sync(0xffffffffu, key[i] >= bound);
+      if (in) {
+        const int k = n + __popc(in & below);
+        if (key[i] >= bound && k < SHORT_LIST) { s_key[warp][k] = key[i]; s_page[warp][k] = lo + 32 * i + lane; }
+        n += __popc(in);
+      }
+    }
+    if (n <= SHORT_LIST) {
+      if (lane < (-n & 3)) s_key[warp][n + lane] = 0;
+      __syncwarp();
+#pragma unroll
+      for (int half = 0; half < 2; ++half) {
+        const int me = lane + 32 * half;
+        if (32 * half >= n) break;
+        const unsigned a = me < n ? s_key[warp][me] : 0u;
+        int above = 0;                                       // larger ones, and equal ones lower down
+        for (int i = 0; i < n; i += 4) {
+          const uint4 v = *reinterpret_cast<const uint4*>(&s_key[warp][i]);
+          above += (v.x > a - (i < me)) + (v.y > a - (i + 1 < me)) + (v.z > a - (i + 2 < me)) + (v.w > a - (i + 3 < me));
+        }
+        const bool in = me < n && above < picks;
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        if (in) dst[at + __popc(mask & below)] = s_page[warp][me];
+        at += __popc(mask);
+      }
+    } else {
+      unsigned last = 0;                                     // the largest order that at least `picks` candidates reach
+#pragma unroll 1
+      for (int bit = 31; bit >= 0; --bit) {
+        const unsigned tried = last | (1u << bit);
+        int c = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) c += key[i] >= tried;
+        if ((int)__reduce_add_sync(0xffffffffu, (unsigned)c) >= picks) last = tried;
       }
       int above = 0;
 #pragma unroll
       for (int i = 0; i < NPL; ++i) above += key[i] > last;
-      equal = picks - (int)__reduce_add_sync(0xffffffffu, (unsigned)above);
-    }
-  }
-  // ascending: the first pages, the picks, the recent pages
-  for (int j = lane; j < lo; j += 32) dst[j] = j;
-  int at = lo;
-  if (all) {
-    for (int j = lo + lane; j < hi; j += 32) dst[j] = j;
-    at = hi;
-  } else if (picks > 0) {
+      int equal = picks - (int)__reduce_add_sync(0xffffffffu, (unsigned)above);
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) {
-      const unsigned same = __ballot_sync(0xffffffffu, key[i] == last);
-      const bool in = key[i] > last || (key[i] == last && __popc(same & ((1u << lane) - 1)) < equal);
-      equal = max(0, equal - __popc(same));
-      const unsigned mask = __ballot_sync(0xffffffffu, in);
-      if (in) dst[at + __popc(mask & ((1u << lane) - 1))] = lo + 32 * i + lane;
-      at += __popc(mask);
+      for (int i = 0; i < NPL; ++i) {
+        const unsigned same = __ballot_sync(0xffffffffu, key[i] == last);
+        const bool in = key[i] > last || (key[i] == last && __popc(same & below) < equal);
+        equal = max(0, equal - __popc(same));
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        if (in) dst[at + __popc(mask & below)] = lo + 32 * i + lane;
+        at += __popc(mask);
+      }
     }
   }
+  // behind the picks the recent pages
   for (int j = hi + lane; j <= own; j += 32) dst[at + j - hi] = j;
   at += own + 1 - hi;
   for (int i = at + lane; i < top; i += 32) dst[i] = -1;
@@ -471,12 +475,12 @@ DINFER_API int dinfer_choose_pages(const float* scores, int64_t ldt, int64_t ldg
                pages, out, Hkv);
     return cuda_status("choose_pages");
   }
-  if (pages <= 2048) {
+  if (pages <= 2048 && rows <= 0x7fffffff - WARPS) {
     auto kernel = pages <= 128 ? choose_registers_kernel<4> : pages <= 256 ? choose_registers_kernel<8>
                   : pages <= 512 ? choose_registers_kernel<16> : pages <= 1024 ? choose_registers_kernel<32>
                   : choose_registers_kernel<64>;
     launch_pdl(kernel, dim3((unsigned)((rows + WARPS - 1) / WARPS)), dim3(WARPS * 32), 0, stream, scores, ldt, ldg, positions,
-               page_size, first, recent, top, pages, out, rows, Hkv);
+               page_size, first, recent, top, pages, out, (int)rows, Hkv);
     return cuda_status("choose_pages");
   }
   launch_pdl(choose_pages_kernel, dim3((unsigned)((rows + WARPS - 1) / WARPS)), dim3(WARPS * 32), 0, stream, scores, ldt, ldg,

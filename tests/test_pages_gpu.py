@@ -98,14 +98,14 @@ def test_append(size, dtype, form):
 def test_means_do_not_depend_on_the_portions(D, dtype):
     """One prompt whole, token by token and in odd portions: the same cache and the same means, bit by bit."""
     from dinfer_b200.kernels import page_ops
-    P, H, G, n = 32, 4, 2, 150
+    P, H, G, n = 32, 4, 2, 650
     g = gen(3)
     whole = Batch([(0, n)], P, seed=2)
     x = torch.randn(n, (H + 2 * G) * D, generator=g).to(dtype).cuda()
     w = (1 + 0.1 * torch.randn(D, generator=g)).to(dtype).cuda()
     table, slots, positions = angles(n, D).cuda(), c(whole.slots), c(whole.positions)
     got = []
-    for cuts in ([n], [1] * n, [31, 2, 30, 1, 40, 46]):
+    for cuts in ([n], [1] * n, [31, 2, 30, 1, 40, 46, 500]):
         cache = torch.zeros(whole.num_pages, 2, G, P, D, dtype=dtype, device="cuda")
         means = torch.zeros(whole.num_pages, G, D, dtype=dtype, device="cuda")
         q = torch.empty(n, H * D, dtype=dtype, device="cuda")
