@@ -381,446 +381,6 @@ int run_token(const void* q, void* out, const void* cache, const Pages& p, int s
   return cuda_status("attention_pages (tokens)");
 }
 
-// ------------------------------------------------------------------------------------------------
-// The same sizes, many tokens (portions of prompts).  Token by token every page would be read once for each token that chose it; here
-// the work is turned round: for every (request, key head, page) the tokens that chose it are listed, and a tile of up to 128 rows
-// (tokens of the list x the group's heads) meets the page's keys once, on the tensor cores.  What a tile makes for a (token, page)
-// pair is a partial result: the sum of weights times values relative to the pair's own maximum, that maximum and the sum of weights,
-// in 32 bits; a last kernel joins the partial results of each token in the order of its list.  Lists are filled with atomic
-// counters, so a token's place in a tile varies from run to run, but no row of a tile depends on the others, and results do not vary.
-//
-// The partial results are the traffic that bounds it (top x D x 4 bytes a token and head, written and read once).  The step is therefore
-// cut into slabs, key heads x runs of tokens, one after the other, whose partial results take SLAB_BYTES at most.
-#ifndef SLAB_MB
-#define SLAB_MB 128
-#endif
-constexpr int64_t SLAB_BYTES = (int64_t)SLAB_MB << 20;
-constexpr int ROWS = 128;
-constexpr int64_t MAX_COUNTERS = 1 << 24;   // lists of all slabs (requests x table width x key heads x runs of tokens): 64 MB of counters
-
-struct Slabs {
-  int heads, tokens, chunks, count;     // key heads and tokens of a slab, runs of tokens, slabs (key-head part slowest)
-  int keys;                             // counters of a slab: heads x requests x table width, to a multiple of 32
-  int tile_tokens;                      // tokens of a tile
-  int64_t list, tiles;                  // room of a slab: list entries, tiles
-  int *counts, *cursors, *base;         // cursors [count][2]: list entries and tiles given out
-  int2 *place;                          // of every choice: its list (-1: no page, -2: behind the last request) and its place there
-  int2 *entries;                        // of a list: token with the keys it sees of the page in the upper 8 bits, and its pair
-  int4* desc;                           // a tile: page, first entry, tokens, key head in the slab
-  float *part, *ml;                     // [heads][tokens][top][group][D], and (maximum in log2 units, sum of weights)
-  int64_t bytes, zeroed;                // the workspace; what must be zero at the start (from counts on)
-};
-
-Slabs slabs_of(const Pages& p, unsigned char* at) {
-  Slabs s;
-  const int group = p.H / p.Hkv;
-  const int64_t per_token = (int64_t)group * p.top * p.D * 4;             // of one key head
-  s.tokens = p.T;
-  s.chunks = 1;
-  while (s.tokens * per_token > SLAB_BYTES && s.tokens > ROWS) {
-    ++s.chunks;
-    s.tokens = ((p.T + s.chunks - 1) / s.chunks + 31) / 32 * 32;
-  }
-  s.chunks = (p.T + s.tokens - 1) / s.tokens;
-  s.heads = (int)(SLAB_BYTES / (s.tokens * per_token));
-  s.heads = s.heads < 1 ? 1 : s.heads > p.Hkv ? p.Hkv : s.heads;
-  const int parts = (p.Hkv + s.heads - 1) / s.heads;
-  s.heads = (p.Hkv + parts - 1) / parts;
-  s.count = parts * s.chunks;
-  const int64_t keys = ((int64_t)s.heads * p.num_reqs * p.width + 31) / 32 * 32;
-  s.keys = (int)(keys > INT32_MAX / 2 ? INT32_MAX / 2 : keys);
-  s.tile_tokens = ROWS / group;
-  s.list = (int64_t)s.heads * s.tokens * p.top;
-  s.tiles = s.list / s.tile_tokens + (s.list < keys ? s.list : keys) + 1;
-  unsigned char* start = at;
-  auto take = [&](int64_t bytes) { unsigned char* x = at; at += (bytes + 255) / 256 * 256; return x; };
-  s.counts = (int*)take((int64_t)s.count * s.keys * 4);
-  s.cursors = (int*)take((int64_t)s.count * 2 * 4);
-  s.zeroed = at - start;
-  s.base = (int*)take((int64_t)s.count * s.keys * 4);
-  s.place = (int2*)take((int64_t)p.T * p.Hkv * p.top * 8);
-  s.entries = (int2*)take((int64_t)s.count * s.list * 8);
-  s.desc = (int4*)take((int64_t)s.count * s.tiles * 16);
-  s.part = (float*)take(s.list * group * p.D * 4);
-  s.ml = (float*)take(s.list * group * 8);
-  s.bytes = at - start;
-  return s;
-}
-
-__device__ __forceinline__ int slab_of(const Slabs& s, int t, int g) { return g / s.heads * s.chunks + t / s.tokens; }
-
-__global__ void __launch_bounds__(256) pages_clear_kernel(int4* at, int64_t n) {
-  pdl_enter();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  if (i < n) at[i] = make_int4(0, 0, 0, 0);
-}
-
-// How often each (request, page) of a slab was chosen, and the place of every choice in its list.  A warp takes 32 tokens of a key head;
-// those whose next choice is the same page count together (neighbours choose much the same pages).
-__global__ void __launch_bounds__(128)
-pages_count_kernel(const Pages p, const Slabs s) {
-  pdl_enter();
-  const int lane = threadIdx.x & 31, t = blockIdx.x * 32 + lane, g = blockIdx.y * 4 + (threadIdx.x >> 5);
-  if (g >= p.Hkv) return;
-  int r = -1;
-  if (t < p.T && t >= p.cu[0] && t < p.cu[p.num_reqs]) {     // the first request whose tokens end behind it
-    int lo = 0, hi = p.num_reqs - 1;
-    while (lo < hi) {
-      const int mid = (lo + hi) >> 1;
-      if (p.cu[mid + 1] > t) hi = mid; else lo = mid + 1;
-    }
-    r = lo;
-  }
-  const int pos = r < 0 ? -1 : p.positions[t];
-  const int64_t at = ((int64_t)t * p.Hkv + g) * p.top;
-  const int slab = slab_of(s, min(t, p.T - 1), g), row = (g % s.heads * p.num_reqs + r) * p.width;
-#pragma unroll 4
-  for (int i = 0; i < p.top; ++i) {
-    const int j = r >= 0 ? p.chosen[at + i] : -1;
-    int key = r < 0 ? -2 : -1;
-    if (j >= 0 && j < p.width && (int64_t)j * p.page_size <= pos) {
-      const int page = p.table[(int64_t)r * p.width + j];
-      if (page >= 0 && page < p.num_pages) key = row + j;
-    }
-    // (the 32 tokens may lie in two slabs: those count apart)
-    const unsigned long long id = key >= 0 ? (unsigned long long)slab << 32 | (unsigned)key : ~0ull;
-    const unsigned same = __match_any_sync(0xffffffffu, id);
-    int first = 0;
-    const int leader = __ffs(same) - 1;
-    if (key >= 0 && lane == leader) first = atomicAdd(s.counts + (int64_t)slab * s.keys + key, __popc(same));
-    first = __shfl_sync(0xffffffffu, first, leader);
-    if (t < p.T) s.place[at + i] = make_int2(key, first + __popc(same & ((1u << lane) - 1)));
-  }
-}
-
-// A list and tiles for every (request, page) that was chosen: a warp adds up its 32 and takes room once.
-__global__ void __launch_bounds__(256)
-pages_lists_kernel(const Pages p, const Slabs s) {
-  pdl_enter();
-  const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-  const int lane = threadIdx.x & 31;
-  const bool in = i < (int64_t)s.count * s.keys;
-  const int slab = in ? (int)(i / s.keys) : 0, key = in ? (int)(i % s.keys) : 0;     // (the same slab in a whole warp)
-  const int c = in ? s.counts[i] : 0, tiles = (c + s.tile_tokens - 1) / s.tile_tokens;
-  int c_sum = c, t_sum = tiles;
-#pragma unroll
-  for (int o = 1; o < 32; o <<= 1) {
-    const int a = __shfl_up_sync(0xffffffffu, c_sum, o), b = __shfl_up_sync(0xffffffffu, t_sum, o);
-    if (lane >= o) { c_sum += a; t_sum += b; }
-  }
-  int c_at = 0, t_at = 0;
-  if (lane == 31 && c_sum > 0) {
-    c_at = atomicAdd(s.cursors + slab * 2, c_sum);
-    t_at = atomicAdd(s.cursors + slab * 2 + 1, t_sum);
-  }
-  c_at = __shfl_sync(0xffffffffu, c_at, 31) + c_sum - c;
-  t_at = __shfl_sync(0xffffffffu, t_at, 31) + t_sum - tiles;
-  if (!in || c == 0) return;
-  s.base[i] = c_at;
-  const int request_page = key % (p.num_reqs * p.width), gl = key / (p.num_reqs * p.width);
-  const int page = p.table[request_page];
-  for (int k = 0; k < tiles; ++k)
-    s.desc[(int64_t)slab * s.tiles + t_at + k] = make_int4(page, c_at + k * s.tile_tokens, min(s.tile_tokens, c - k * s.tile_tokens), gl);
-}
-
-__global__ void __launch_bounds__(128)
-pages_fill_kernel(const Pages p, const Slabs s) {
-  pdl_enter();
-  const int64_t at = (int64_t)blockIdx.x * 128 + threadIdx.x;
-  const int per = p.Hkv * p.top;
-  if (at >= (int64_t)p.T * per) return;
-  const int2 place = s.place[at];
-  if (place.x < 0) return;
-  const int t = (int)(at / per), i = (int)(at - (int64_t)t * per), g = i / p.top, slab = slab_of(s, t, g);
-  const int seen = min(p.page_size, p.positions[t] - p.chosen[at] * p.page_size + 1);
-  const int pair = (g % s.heads * s.tokens + t % s.tokens) * p.top + i - g * p.top;
-  s.entries[(int64_t)slab * s.list + s.base[(int64_t)slab * s.keys + place.x] + place.y] = make_int2(t | seen << 24, pair);
-}
-
-// 0 where a packed bfloat16 is not a number or infinite
-__device__ __forceinline__ unsigned finite2(unsigned x) {
-  if ((x & 0x7f80u) == 0x7f80u) x &= 0xffff0000u;
-  if ((x & 0x7f800000u) == 0x7f800000u) x &= 0x0000ffffu;
-  return x;
-}
-__device__ __forceinline__ bool odd2(unsigned x) { return (x & 0x7f80u) == 0x7f80u || (x & 0x7f800000u) == 0x7f800000u; }
-
-// Tiles of 128 rows, a warp owns 16.  A block takes tile after tile: while it works on one, the next one's keys and values are on their way
-// into the other half of its shared memory, and once the scores are made, the next one's rows of Q into the registers that held
-// this one's.  Q goes from memory straight into fragments: the order of the elements of a product's sum is free, so a lane takes 16 bytes of its
-// rows and of the keys' at the same places, two steps of 16 elements at once.
-constexpr int PORTION_NT = ROWS * 2;
-
-template <int D, int P>
-__global__ void __launch_bounds__(PORTION_NT, 2)
-pages_portion_kernel(const __nv_bfloat16* __restrict__ q, const __nv_bfloat16* __restrict__ cache, const Pages p, const Slabs s, int slab) {
-  extern __shared__ __align__(128) unsigned char smem_raw[];
-  // [2] x keys [P][D], 16-byte pieces exchanged by (key & 1) * 4, and values [P][D], by key & 7
-  __nv_bfloat16* smem = reinterpret_cast<__nv_bfloat16*>(smem_raw);
-  pdl_enter();
-  const int tiles = s.cursors[slab * 2 + 1];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, gr = lane >> 2, tq = lane & 3;
-  const int g0 = slab / s.chunks * s.heads, group = p.H / p.Hkv;
-  const int64_t plane = (int64_t)p.Hkv * P * D;
-  const int4* desc = s.desc + (int64_t)slab * s.tiles;
-  const int2* entries = s.entries + (int64_t)slab * s.list;
-  float *s_part = s.part, *s_ml = s.ml;
-  constexpr int C = D / 8;
-  auto load_tile = [&](const int4& d, int stage) {
-    const __nv_bfloat16* keys = cache + (int64_t)d.x * 2 * plane + (int64_t)(g0 + d.w) * P * D;
-    __nv_bfloat16* k = smem + stage * 2 * P * D;
-    const int chunk = threadIdx.x % C;
-#pragma unroll
-    for (int row = threadIdx.x / C; row < P; row += PORTION_NT / C) {
-      cp_async16(k + row * D + ((chunk ^ ((row & 1) << 2)) << 3), keys + row * D + chunk * 8, true);
-      cp_async16(k + P * D + row * D + ((chunk ^ (row & 7)) << 3), keys + plane + row * D + chunk * 8, true);
-    }
-  };
-  // this lane's two rows of every tile: a token of its list and a head of the group
-  int row_token[2], row_head[2];
-#pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int row = warp * 16 + gr + 8 * u;
-    row_token[u] = row / group;
-    row_head[u] = row - row_token[u] * group;
-  }
-  int2 entry[2];                                            // (of a tile; x < 0: no row)
-  auto load_entries = [&](const int4& d) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) entry[u] = row_token[u] < d.z ? entries[d.y + row_token[u]] : make_int2(-1, 0);
-  };
-  uint4 qa[D / 32][2];
-  int part[2], seen[2];                                     // (pair, head) of the partial results, -1: no row; keys that the row sees
-  auto load_rows = [&](const int4& d) {
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      const bool in = row_token[u] < d.z;
-      const int t = entry[u].x & 0xffffff;
-      part[u] = in ? entry[u].y * group + row_head[u] : -1;
-      seen[u] = in ? (unsigned)entry[u].x >> 24 : P;
-      const __nv_bfloat16* row = q + (in ? (int64_t)t * p.ldq + (int64_t)((g0 + d.w) * group + row_head[u]) * D + tq * 8 : 0);
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k) qa[k][u] = *reinterpret_cast<const uint4*>(row + k * 32);
-    }
-  };
-  int tile = blockIdx.x;
-  int4 d = tile < tiles ? desc[tile] : make_int4(0, 0, 0, 0), d_next = d;
-  if (tile < tiles) {
-    load_tile(d, 0);
-    load_entries(d);
-    load_rows(d);
-    if (tile + (int)gridDim.x < tiles) d_next = desc[tile + gridDim.x];
-  }
-  cp_async_commit();
-  const float scale_log2 = p.scale * 1.4426950408889634f;
-  for (int stage = 0; tile < tiles; stage ^= 1) {
-    const int next = tile + gridDim.x;
-    cp_async_wait<0>();
-    __syncthreads();                                        // the tile is here, and everyone is done with the one before
-    if (next < tiles) {
-      load_tile(d_next, stage ^ 1);
-      load_entries(d_next);
-    }
-    cp_async_commit();
-    const __nv_bfloat16 *sK = smem + stage * 2 * P * D, *sV = sK + P * D;
-    const int mine[2] = {part[0], part[1]}, sees[2] = {seen[0], seen[1]};
-    const bool active = warp * 16 < d.z * group;
-    unsigned pa[P / 16][4];
-    if (active) {
-      float st[P / 8][4];
-#pragma unroll
-      for (int n = 0; n < P / 8; ++n) st[n][0] = st[n][1] = st[n][2] = st[n][3] = 0.f;
-#pragma unroll
-      for (int k = 0; k < D / 32; ++k)
-#pragma unroll
-        for (int n = 0; n < P / 8; ++n) {
-          const int row = n * 8 + gr;
-          const uint4 b = *reinterpret_cast<const uint4*>(sK + row * D + (((k * 4 + tq) ^ ((row & 1) << 2)) << 3));
-          mma_bf16(st[n], qa[k][0].x, qa[k][1].x, qa[k][0].y, qa[k][1].y, b.x, b.y);
-          mma_bf16(st[n], qa[k][0].z, qa[k][1].z, qa[k][0].w, qa[k][1].w, b.z, b.w);
-        }
-      float mx[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
-#pragma unroll
-      for (int n = 0; n < P / 8; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          st[n][c] = n * 8 + 2 * tq + (c & 1) < sees[c >> 1] ? st[n][c] * scale_log2 : -INFINITY;
-          mx[c >> 1] = fmaxf(mx[c >> 1], st[n][c]);
-        }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 1));
-        mx[u] = fmaxf(mx[u], __shfl_xor_sync(0xffffffffu, mx[u], 2));
-      }
-      const float base[2] = {mx[0] == -INFINITY ? 0.f : mx[0], mx[1] == -INFINITY ? 0.f : mx[1]};
-#pragma unroll
-      for (int n = 0; n < P / 8; ++n)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) {
-          st[n][c] = fast_exp2(st[n][c] - base[c >> 1]);
-          l[c >> 1] += st[n][c];
-        }
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 1);
-        l[u] += __shfl_xor_sync(0xffffffffu, l[u], 2);
-      }
-      // the weights are rounded to bfloat16 for the second product (2^-9 of each; their sum is taken before)
-#pragma unroll
-      for (int k = 0; k < P / 16; ++k) {
-        pa[k][0] = pack_bf16(st[2 * k][0], st[2 * k][1]);
-        pa[k][1] = pack_bf16(st[2 * k][2], st[2 * k][3]);
-        pa[k][2] = pack_bf16(st[2 * k + 1][0], st[2 * k + 1][1]);
-        pa[k][3] = pack_bf16(st[2 * k + 1][2], st[2 * k + 1][3]);
-      }
-      if (tq == 0)
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (mine[u] >= 0) *reinterpret_cast<float2*>(s_ml + (int64_t)mine[u] * 2) = make_float2(mx[u], l[u]);
-    }
-    if (next < tiles) load_rows(d_next);
-    // A value that is not a finite number, in a page that some row sees in part: a weight of zero would carry it into rows that do not
-    // see it.  Those products are then made without such values, and rows that see them get them one by one.
-    bool odd = false;
-    if (active && __any_sync(0xffffffffu, sees[0] < P || sees[1] < P)) {
-      for (int i = lane; i < P * C; i += 32) {
-        const uint4 v = *reinterpret_cast<const uint4*>(sV + i * 8);
-        odd |= odd2(v.x) || odd2(v.y) || odd2(v.z) || odd2(v.w);
-      }
-      odd = __any_sync(0xffffffffu, odd);
-    }
-    if (active) {
-#pragma unroll 2
-      for (int db = 0; db < D / 16; ++db) {
-        float o[2][4] = {};
-#pragma unroll
-        for (int k = 0; k < P / 16; ++k) {
-          unsigned b[4];
-          const int row = k * 16 + (lane & 15);
-          ldmatrix_x4_trans(b, sV + row * D + (((db * 2 + (lane >> 4)) ^ (row & 7)) << 3));
-          if (odd)
-#pragma unroll
-            for (int x = 0; x < 4; ++x) b[x] = finite2(b[x]);
-          mma_bf16(o[0], pa[k][0], pa[k][1], pa[k][2], pa[k][3], b[0], b[1]);
-          mma_bf16(o[1], pa[k][0], pa[k][1], pa[k][2], pa[k][3], b[2], b[3]);
-        }
-        if (odd) {
-#pragma unroll
-          for (int k = 0; k < P / 16; ++k)
-            for (int x = 0; x < 16; ++x) {
-              const int key = k * 16 + x, from = (lane & ~3) | ((x & 7) >> 1);
-              const unsigned w0 = __shfl_sync(0xffffffffu, x < 8 ? pa[k][0] : pa[k][2], from);
-              const unsigned w1 = __shfl_sync(0xffffffffu, x < 8 ? pa[k][1] : pa[k][3], from);
-              const float w[2] = {__uint_as_float(x & 1 ? w0 & 0xffff0000u : w0 << 16), __uint_as_float(x & 1 ? w1 & 0xffff0000u : w1 << 16)};
-#pragma unroll
-              for (int n = 0; n < 2; ++n)
-#pragma unroll
-                for (int c = 0; c < 4; ++c) {
-                  const int col = db * 16 + n * 8 + 2 * tq + (c & 1);
-                  const float v = __bfloat162float(sV[key * D + (((col >> 3) ^ (key & 7)) << 3) + (col & 7)]);
-                  if (!isfinite(v) && key < sees[c >> 1]) o[n][c] += w[c >> 1] * v;
-                }
-            }
-        }
-#pragma unroll
-        for (int u = 0; u < 2; ++u)
-          if (mine[u] >= 0) {
-            float* dst = s_part + (int64_t)mine[u] * D + db * 16 + 2 * tq;
-            *reinterpret_cast<float2*>(dst) = make_float2(o[0][2 * u], o[0][2 * u + 1]);
-            *reinterpret_cast<float2*>(dst + 8) = make_float2(o[1][2 * u], o[1][2 * u + 1]);
-          }
-      }
-    }
-    tile = next;
-    d = d_next;
-    if (tile + (int)gridDim.x < tiles) d_next = desc[tile + gridDim.x];
-  }
-  cp_async_wait<0>();
-}
-
-// A warp per (token, head) of a slab: the partial results of the token's pages, in the order of its list.
-template <int D>
-__global__ void __launch_bounds__(256)
-pages_join_kernel(__nv_bfloat16* __restrict__ out, const Pages p, const Slabs s, int slab) {
-  pdl_enter();
-  constexpr int E = D / 32, AHEAD = 8;                      // elements a lane; partial results asked for at once
-  struct alignas(E * 4) Vec { float v[E]; };
-  const int lane = threadIdx.x & 31, group = p.H / p.Hkv;
-  const int g0 = slab / s.chunks * s.heads, t0 = slab % s.chunks * s.tokens;
-  const int heads = min(s.heads, p.Hkv - g0) * group;
-  const int w = blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int tl = w / heads, hl = w - tl * heads, t = t0 + tl;
-  if (tl >= s.tokens || t >= p.T) return;
-  const int gl = hl / group, h = hl - gl * group;
-  const int2* place = s.place + ((int64_t)t * p.Hkv + g0 + gl) * p.top;
-  const int pair0 = (gl * s.tokens + tl) * p.top;
-  const float2* ml = reinterpret_cast<const float2*>(s.ml) + h;
-  const float* part = s.part + (int64_t)h * D + lane * E;
-  float M = -INFINITY, L = 0.f, acc[E] = {};
-  for (int i0 = 0; i0 < p.top; i0 += 32) {
-    const int mine = i0 + lane < p.top ? place[i0 + lane].x : -1;
-    if (i0 == 0 && __shfl_sync(0xffffffffu, mine, 0) == -2) return;       // behind the last request
-    const float2 x = mine >= 0 ? ml[(pair0 + i0 + lane) * group] : make_float2(-INFINITY, 0.f);
-    const float m = fmaxf(M, warp_max(x.x)), base = m == -INFINITY ? 0.f : m;
-    const float f = mine >= 0 ? fast_exp2(x.x - base) : 0.f, again = fast_exp2(M - base);
-    M = m;
-    L = fmaf(L, again, warp_sum(f * x.y));
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[e] *= again;
-    // the pages there are, in the list's order, several asked for at once
-    unsigned mask = __ballot_sync(0xffffffffu, mine >= 0);
-    while (mask) {
-      Vec v[AHEAD];
-      float w_i[AHEAD];
-      unsigned rest = mask;
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {
-        const int i = rest ? __ffs(rest) - 1 : __ffs(mask) - 1;
-        w_i[u] = __shfl_sync(0xffffffffu, f, i);
-        v[u] = *reinterpret_cast<const Vec*>(part + (int64_t)(pair0 + i0 + i) * group * D);
-        if (!rest) w_i[u] = -1.f;
-        rest &= rest - 1;
-      }
-#pragma unroll
-      for (int u = 0; u < AHEAD; ++u)
-        if (w_i[u] >= 0.f || w_i[u] != w_i[u])
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[e] = fmaf(w_i[u], v[u].v[e], acc[e]);
-      mask = rest;
-    }
-  }
-  const float inv = L == 0.f ? 0.f : 1.f / L;
-  __nv_bfloat16* dst = out + (int64_t)t * p.ldo + (int64_t)(g0 + gl) * group * D + (int64_t)h * D + lane * E;
-#pragma unroll
-  for (int e = 0; e < E; e += 2) *reinterpret_cast<unsigned*>(dst + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
-}
-
-template <int D, int P>
-int run_portions(const void* q, void* out, const void* cache, const Pages& p, const Slabs& s, int sms, cudaStream_t stream) {
-  auto kernel = pages_portion_kernel<D, P>;
-  constexpr int smem = 2 * 2 * P * D * 2;
-  if (smem > 48 * 1024) {
-    static thread_local int set_for = -1;
-    int dev = 0;
-    cudaGetDevice(&dev);
-    if (set_for != dev) {
-      if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
-        return cuda_status("attention_pages: shared memory");
-      set_for = dev;
-    }
-  }
-  launch_pdl(pages_clear_kernel, dim3((unsigned)((s.zeroed / 16 + 255) / 256)), dim3(256), 0, stream, (int4*)s.counts, s.zeroed / 16);
-  launch_pdl(pages_count_kernel, dim3((p.T + 31) / 32, (p.Hkv + 3) / 4), dim3(128), 0, stream, p, s);
-  launch_pdl(pages_lists_kernel, dim3((unsigned)(((int64_t)s.count * s.keys + 255) / 256)), dim3(256), 0, stream, p, s);
-  launch_pdl(pages_fill_kernel, dim3((unsigned)(((int64_t)p.T * p.Hkv * p.top + 127) / 128)), dim3(128), 0, stream, p, s);
-  const int64_t joined = ((int64_t)s.tokens * s.heads * (p.H / p.Hkv) + 7) / 8;
-  for (int i = 0; i < s.count; ++i) {
-    launch_pdl(kernel, dim3((unsigned)(s.tiles < 2 * sms ? s.tiles : 2 * sms)), dim3(PORTION_NT), smem, stream, (const __nv_bfloat16*)q, (const __nv_bfloat16*)cache, p, s, i);
-    launch_pdl(pages_join_kernel<D>, dim3((unsigned)joined), dim3(256), 0, stream, (__nv_bfloat16*)out, p, s, i);
-  }
-  return cuda_status("attention_pages (portions)");
-}
-
 // Whether the tensor-core kernels take the call: rows that 16-byte loads and pair stores address, sizes they are made for.
 bool tensor_cores(const void* q, const void* out, const void* cache, const Pages& p) {
   const int group = p.H / p.Hkv;
@@ -830,34 +390,17 @@ bool tensor_cores(const void* q, const void* out, const void* cache, const Pages
 }
 }  // namespace
 
-// Bytes of workspace with which the call takes its portions' form (any smaller one: token by token).
-DINFER_API int64_t dinfer_attention_pages_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D) {
-  if (T <= 0 || T >= 1 << 24 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > 16 || top <= 0 || width <= 0 || num_reqs <= 0 || D <= 0) return 0;
-  Pages p{};
-  p.width = width; p.num_reqs = num_reqs; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.D = D;
-  if ((int64_t)Hkv * num_reqs * width > MAX_COUNTERS) return 0;
-  const Slabs s = slabs_of(p, nullptr);
-  return (int64_t)s.count * s.keys > MAX_COUNTERS ? 0 : s.bytes;
-}
-
 // chosen int32 [T, Hkv, top]; cache [num_pages, 2, Hkv, page_size, D].
 DINFER_API int dinfer_attention_pages(const void* q, int64_t ldq, void* out, int64_t ldo, const void* cache, int num_pages,
                                       const int* table, int width, const int* cu_seqlens, int num_reqs, const int* positions,
                                       const int* chosen, int top, int T, int H, int Hkv, int D, int page_size, float scale,
-                                      void* workspace, int64_t workspace_bytes, int sms, int dtype, cudaStream_t stream) {
+                                      int sms, int dtype, cudaStream_t stream) {
   if (T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 512 || page_size <= 0 || num_reqs <= 0 || top <= 0 || width < 0)
     return refuse(DINFER_BAD_ARGUMENT, "attention_pages: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d", T, H, Hkv, D, page_size, top);
   if ((H + WARPS - 1) / WARPS > 65535) return refuse(DINFER_BAD_ARGUMENT, "attention_pages: %d heads", H);
   if (T == 0) return DINFER_OK;
   const Pages p{ldq, ldo, num_pages, table, width, cu_seqlens, num_reqs, positions, chosen, top, T, H, Hkv, D, page_size, scale};
   if (dtype == DINFER_BF16 && tensor_cores(q, out, cache, p)) {
-    const int64_t need = workspace ? dinfer_attention_pages_workspace(num_reqs, width, top, T, H, Hkv, D) : 0;
-    if (need > 0 && workspace_bytes >= need) {
-      const Slabs s = slabs_of(p, (unsigned char*)workspace);
-#define DINFER_PAGES(P_) case P_: return D == 128 ? run_portions<128, P_>(q, out, cache, p, s, sms, stream) : run_portions<64, P_>(q, out, cache, p, s, sms, stream)
-      switch (page_size) { DINFER_PAGES(16); DINFER_PAGES(32); DINFER_PAGES(64); DINFER_PAGES(128); }
-#undef DINFER_PAGES
-    }
     // CTAs that share a token's keys: as far as all run at the same time (two an SM), each with a tile of its own at least
     int splits = 1;
     while (splits < 8 && (int64_t)T * Hkv * splits * 2 <= 2 * sms && splits * 2 * BN <= (int64_t)top * page_size) splits *= 2;

@@ -1,0 +1,648 @@
+// Attention over chosen pages for many tokens (portions of prompts) on the 5th-generation tensor cores (tcgen05 + TMEM + TMA):
+// bfloat16, head sizes 64 and 128, groups of up to 128 heads, pages of 16 to 128 tokens.  Token t at position p, head h of key head g's
+// group:
+//     out[t, h] = sum_i softmax_i(scale q[t, h] . k_i) v_i      over  { i <= p : i / page_size in chosen[t, g] }
+//
+// Neighbouring tokens choose much the same pages.  The tokens of a request are cut into row tiles of 128 (token, head) rows, two to a
+// block, and for every (pair of row tiles, key head) a first kernel collects the pages that any of its tokens chose, ascending, with one
+// bit per token that says whether it did.  The block then walks that list as the attention over a whole context walks its keys:
+//     S[128, 64]  = Q K^T          tcgen05.mma, Q and K K-major in shared memory, S in tensor memory (two buffers)
+//     P = softmax step             one thread per row (= TMEM lane): tcgen05.ld, keys of pages that the row's token did not choose
+//                                  (or that lie behind it) to -inf, exp2, P -> shared memory (bfloat16)
+//     O[128, D]  += P V            tcgen05.mma accumulating in tensor memory; O is rescaled in place only when a row's maximum grows
+//                                  by more than 2^8
+// A page is read once for the 256 rows, not once for each token that chose it, and no partial results leave the SM.  A warp none
+// of whose rows sees a tile passes it with zeros.
+//
+// Warp roles (384 threads): warp 0 brings Q (once) and K, warp 11 V, page by page through a map over the cache, each on a ring of its own;
+// warps 1 and 10 issue the products of the two row tiles; warps 2..9 are softmax and output, four per row tile.  Every mbarrier wait
+// is bounded.
+//
+// A weight of zero times a value that is not a finite number is not zero: such a value in any of a block's pages makes an element of every
+// row's result one that is not finite.  Where a row's result has one, the block's rows are made again at its end, key by key and
+// only from keys that they see.  The same goes for a block one of whose tokens names a page twice (it then counts twice, which a bit
+// cannot say).
+#include <cuda.h>
+
+#include "common.cuh"
+#include "umma_attention.cuh"
+
+using namespace dinfer;
+using namespace dinfer_umma;
+
+namespace {
+
+constexpr int BM = 128, BN = 64, STAGES = 3, NTHREADS = 384;    // BM rows of a row tile, two row tiles a block
+constexpr int MMA_WARP_B = 10, V_WARP = 11;                     // the second MMA issuer, the V producer
+constexpr int LIST_SLOTS = 1024;                                // entries of a list in shared memory (fewer where a row tile has more than 32 tokens)
+constexpr int TWICE = 1 << 30;                                  // in a list's count: some token names a page twice
+
+struct Params {
+  const __nv_bfloat16* q; int64_t ldq;
+  __nv_bfloat16* out; int64_t ldo;
+  const __nv_bfloat16* cache; int num_pages;
+  const int* table; int width;
+  const int* cu; int B;
+  const int* positions;
+  const int* chosen; int top;
+  int T, H, Hkv, group, page_size;
+  float scale, scale_log2;
+  int tile_tokens;                     // tokens of a row tile
+  int words;                           // 32-bit words of its bits
+  int unit, per_tile;                  // keys of a list entry (a page, or 64 of its keys), entries of a key tile
+  int cap;                             // entries that a list has room for (a multiple of per_tile)
+  int pairs;                           // pairs of row tiles that the grid counts
+  int* counts;                         // [pairs][Hkv]: entries, to a multiple of per_tile
+  int2* entries;                       // [pairs][Hkv][cap]: first row of the entry's keys in key head 0's share of the cache (-1: none), first position
+  unsigned* masks;                     // [pairs][Hkv][cap][2][words]
+  int* status;
+};
+
+// The pair of row tiles `y` of the batch (every lane of a full warp asks): request, first token, tokens; request -1 beyond the last.
+__device__ __forceinline__ int3 pair_of(const Params& p, int y) {
+  const int lane = threadIdx.x & 31, tile = 2 * p.tile_tokens;
+  int before = 0;
+  for (int i0 = 0; i0 < p.B; i0 += 32) {
+    const int i = i0 + lane;
+    const int begin = i < p.B ? p.cu[i] : 0, tokens = i < p.B ? p.cu[i + 1] - begin : 0;
+    const int n = (tokens + tile - 1) / tile;
+    int incl = n;
+#pragma unroll
+    for (int d = 1; d < 32; d <<= 1) {
+      const int v = __shfl_up_sync(0xffffffffu, incl, d);
+      if (lane >= d) incl += v;
+    }
+    const unsigned hit = __ballot_sync(0xffffffffu, y >= before + incl - n && y < before + incl);
+    if (hit) {
+      const int src = __ffs(hit) - 1;
+      const int at = y - before - __shfl_sync(0xffffffffu, incl - n, src);
+      const int b = __shfl_sync(0xffffffffu, begin, src), k = __shfl_sync(0xffffffffu, tokens, src);
+      return make_int3(i0 + src, b + at * tile, min(tile, k - at * tile));
+    }
+    before += __shfl_sync(0xffffffffu, incl, 31);
+  }
+  return make_int3(-1, 0, 0);
+}
+
+// The list of a pair of row tiles and key head: bits of the pages of a window in shared memory, then the pages that have any, in order.
+constexpr int LIST_NT = 256, WINDOW_WORDS = 8192;
+
+__global__ void __launch_bounds__(LIST_NT) page_lists_kernel(const Params p) {
+  __shared__ unsigned s_bits[WINDOW_WORDS];
+  __shared__ int s_warp[LIST_NT / 32];
+  pdl_enter();
+  const int g = blockIdx.x, y = blockIdx.y, lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int3 pair = pair_of(p, y);
+  if (pair.x < 0) return;
+  const int* table = p.table + (int64_t)pair.x * p.width;
+  const int64_t at = ((int64_t)y * p.Hkv + g);
+  int2* entries = p.entries + at * p.cap;
+  unsigned* masks = p.masks + at * p.cap * 2 * p.words;
+  const int per_page = p.page_size / p.unit, bits = 2 * p.words, window = WINDOW_WORDS / bits;
+  int n = 0, twice = 0;                                         // entries so far; whether a token names a page twice
+  int far = -1;                                                 // (a page behind the furthest token's own is seen by none)
+  for (int tl = lane; tl < pair.z; tl += 32) far = max(far, p.positions[pair.y + tl]);
+  far = __reduce_max_sync(0xffffffffu, far);
+  const int last = far < 0 ? -1 : min(p.width - 1, far / p.page_size);
+  for (int w0 = 0; w0 <= last; w0 += window) {
+    const int pages = min(window, last + 1 - w0);
+    for (int i = threadIdx.x; i < pages * bits; i += LIST_NT) s_bits[i] = 0;
+    __syncthreads();
+    for (int i = threadIdx.x; i < pair.z * p.top; i += LIST_NT) {
+      const int tl = i / p.top, t = pair.y + tl, j = p.chosen[((int64_t)t * p.Hkv + g) * p.top + i - tl * p.top];
+      if (j >= w0 && j < w0 + pages && (int64_t)j * p.page_size <= p.positions[t]) {
+        const int w = tl / p.tile_tokens, bit = tl - w * p.tile_tokens;
+        const unsigned mine = 1u << (bit & 31);
+        if (atomicOr(&s_bits[(j - w0) * bits + w * p.words + (bit >> 5)], mine) & mine) twice = 1;
+      }
+    }
+    __syncthreads();
+    for (int j0 = 0; j0 < pages; j0 += LIST_NT) {
+      const int j = j0 + threadIdx.x;
+      bool in = false;
+      int page = -1;
+      if (j < pages) {
+        for (int w = 0; w < bits; ++w) in |= s_bits[j * bits + w] != 0;
+        if (in) page = table[w0 + j];
+        in = in && page >= 0 && page < p.num_pages;
+      }
+      const unsigned ball = __ballot_sync(0xffffffffu, in);
+      if (lane == 0) s_warp[warp] = __popc(ball);
+      __syncthreads();
+      int below = 0, all = 0;
+#pragma unroll
+      for (int w = 0; w < LIST_NT / 32; ++w) {
+        below += w < warp ? s_warp[w] : 0;
+        all += s_warp[w];
+      }
+      if (in) {
+        const int e0 = n + (below + __popc(ball & ((1u << lane) - 1))) * per_page;
+        for (int x = 0; x < per_page; ++x) {
+          entries[e0 + x] = make_int2(page * 2 * p.Hkv * p.page_size + x * p.unit, (w0 + j) * p.page_size + x * p.unit);
+          for (int w = 0; w < bits; ++w) masks[(int64_t)(e0 + x) * bits + w] = s_bits[j * bits + w];
+        }
+      }
+      n += all * per_page;
+      __syncthreads();
+    }
+  }
+  const int full = (n + p.per_tile - 1) / p.per_tile * p.per_tile;
+  for (int e = n + threadIdx.x; e < full; e += LIST_NT) {       // the last key tile is filled up with entries that nobody sees
+    entries[e] = make_int2(-1, 0);
+    for (int w = 0; w < bits; ++w) masks[(int64_t)e * bits + w] = 0;
+  }
+  twice = __syncthreads_or(twice);
+  if (threadIdx.x == 0) p.counts[at] = full | (twice ? TWICE : 0);
+}
+
+// The rows of a block once more, a warp per row and key by key, from nothing but what the row's token sees.
+template <int D>
+__device__ __noinline__ void rows_again(const Params& p, int request, int first, int tokens, int g) {
+  const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+  const int* table = p.table + (int64_t)request * p.width;
+  const int64_t plane = (int64_t)p.Hkv * p.page_size * D;
+  for (int row = warp; row < tokens * p.group; row += NTHREADS / 32) {
+    const int t = first + row / p.group, h = g * p.group + row % p.group, pos = p.positions[t];
+    float qv[D / 32], acc[D / 32];
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) {
+      qv[c] = __bfloat162float(p.q[(int64_t)t * p.ldq + (int64_t)h * D + lane + 32 * c]) * p.scale;
+      acc[c] = 0.f;
+    }
+    float m = -INFINITY, l = 0.f;
+    for (int i = 0; i < p.top; ++i) {
+      const int j = p.chosen[((int64_t)t * p.Hkv + g) * p.top + i];
+      if (j < 0 || j >= p.width || (int64_t)j * p.page_size > pos) continue;
+      const int page = table[j];
+      if (page < 0 || page >= p.num_pages) continue;
+      const __nv_bfloat16* kp = p.cache + (int64_t)page * 2 * plane + (int64_t)g * p.page_size * D;
+      const int keys = min(p.page_size, pos - j * p.page_size + 1);
+      for (int o = 0; o < keys; ++o) {
+        float s = 0.f;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) s = fmaf(qv[c], __bfloat162float(kp[o * D + lane + 32 * c]), s);
+        s = warp_sum(s);
+        const float n = fmaxf(m, s), base = n == -INFINITY ? 0.f : n, alpha = expf(m - base), w = expf(s - base);
+        m = n;
+        l = fmaf(l, alpha, w);
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(acc[c], alpha, w * __bfloat162float(kp[plane + o * D + lane + 32 * c]));
+      }
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+#pragma unroll
+    for (int c = 0; c < D / 32; ++c) p.out[(int64_t)t * p.ldo + (int64_t)h * D + lane + 32 * c] = __float2bfloat16_rn(acc[c] * inv);
+  }
+}
+
+template <int D> constexpr size_t smem_bytes() {
+  return (size_t)(2 * BM * D * 2 + 2 * STAGES * BN * D * 2 + 2 * BM * BN * 2) + 1024;
+}
+
+template <int D>
+__global__ void __launch_bounds__(NTHREADS, 1)
+attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Params p) {
+  constexpr int NH = D / 64;                          // 64-wide halves of the head
+  constexpr uint32_t Q_HALF = BM * 128, KV_HALF = BN * 128;
+  constexpr uint32_t Q_BYTES = NH * Q_HALF, KV_BYTES = NH * KV_HALF, P_BYTES = BM * BN * 2;
+  constexpr int TMEM_COLS = 512, O_COL = 256;         // S of (row tile w, buffer b) at (2w + b) * 64; O of A 256, of B 384
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES],
+      s_full[2][2], p_full[2], pv_done[2], o_full[2];
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_abort, s_odd;
+  __shared__ int s_first[LIST_SLOTS];                  // the list's beginning: first positions and bits
+  __shared__ unsigned s_bits[LIST_SLOTS * 2];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int hk = blockIdx.x;
+  pdl_enter();
+  const int3 pair = pair_of(p, blockIdx.y);
+  if (pair.x < 0) return;                              // beyond the batch's pairs
+  const int64_t at = (int64_t)blockIdx.y * p.Hkv + hk;
+  const int count = p.counts[at], n_tiles = (count & ~TWICE) / p.per_tile;
+  const int2* entries = p.entries + at * p.cap;
+  const unsigned* masks = p.masks + at * p.cap * 2 * p.words;
+  const bool b_on = pair.z > p.tile_tokens;            // the second row tile exists
+
+  const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  const uint32_t sQ = base, sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES, sP = sV + STAGES * KV_BYTES;
+  {
+    // zeroed K/V stages: an entry that is no page leaves its slot as it was, and it must hold finite numbers
+    uint4* z = reinterpret_cast<uint4*>(smem_dyn + (sK - smem_u32(smem_dyn)));
+    for (int i = threadIdx.x; i < (int)(2 * STAGES * KV_BYTES / 16); i += NTHREADS) z[i] = make_uint4(0, 0, 0, 0);
+  }
+  const int held = min(n_tiles * p.per_tile, LIST_SLOTS / p.words);
+  for (int i = threadIdx.x; i < held; i += NTHREADS) s_first[i] = entries[i].y;
+  for (int i = threadIdx.x; i < held * 2 * p.words; i += NTHREADS) s_bits[i] = masks[i];
+  if (threadIdx.x == 0) {
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
+    asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
+    mbar_init(smem_u32(&q_full), 1);
+    for (int s = 0; s < STAGES; ++s) {
+      mbar_init(smem_u32(&k_full[s]), 1); mbar_init(smem_u32(&k_empty[s]), 2);       // empty: both MMA issuers
+      mbar_init(smem_u32(&v_full[s]), 1); mbar_init(smem_u32(&v_empty[s]), 2);
+    }
+    for (int w = 0; w < 2; ++w) {
+      mbar_init(smem_u32(&s_full[w][0]), 1);
+      mbar_init(smem_u32(&s_full[w][1]), 1);
+      mbar_init(smem_u32(&p_full[w]), 128);
+      mbar_init(smem_u32(&pv_done[w]), 1);
+      mbar_init(smem_u32(&o_full[w]), 1);
+    }
+    s_abort = 0;
+    s_odd = count & TWICE ? 1 : 0;
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 1) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(TMEM_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the zero fill above, before TMA writes the same bytes
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem_base;
+
+  if (warp == 0 || warp == V_WARP) {
+    // ---- TMA producers: warp 0 Q (once, lane 0) and the K tiles, another warp the V tiles; per tile one copy per entry and 64-wide
+    // half, spread over the lanes.  The next tile's entries are asked for while the ring's stage is waited for.
+    const int kv = warp == 0 ? 0 : 1;
+    if (kv == 0 && lane == 0) {
+      const uint32_t qb = smem_u32(&q_full);
+      // (a box has tile_tokens x group rows, at most 128)
+      const uint32_t rows = (uint32_t)(p.tile_tokens * p.group) * 128;
+      mbar_expect_tx(qb, (b_on ? 2 : 1) * NH * rows);
+      for (int w = 0; w < (b_on ? 2 : 1); ++w)
+        for (int h = 0; h < NH; ++h)
+          tma_load_3d(sQ + w * Q_BYTES + h * Q_HALF, &map_q, h * 64, hk * p.group, pair.y + w * p.tile_tokens, qb);
+    }
+    const int n_ops = p.per_tile * NH, x = lane / NH, h = lane % NH;       // copies of a tile, <= 8
+    const bool mine = lane < n_ops;
+    int row = mine && n_tiles > 0 ? entries[x].x : -1;
+    for (int j = 0; j < n_tiles; ++j) {
+      const int s = j % STAGES;
+      const bool valid = row >= 0;
+      const uint32_t bytes = __reduce_add_sync(0xffffffffu, valid ? (uint32_t)(p.unit * 128) : 0u);
+      const int row_k = row + (kv * p.Hkv + hk) * p.page_size;
+      const int next = mine && j + 1 < n_tiles ? entries[(j + 1) * p.per_tile + x].x : -1;
+      bool ok = true;
+      if (lane == 0) ok = mbar_wait(smem_u32(kv == 0 ? &k_empty[s] : &v_empty[s]), ((j / STAGES) & 1) ^ 1);
+      ok = __shfl_sync(0xffffffffu, ok, 0);
+      if (!ok) { if (lane == 0) { s_abort = 1; atomicExch(p.status, 61); } break; }
+      const uint32_t bar = smem_u32(kv == 0 ? &k_full[s] : &v_full[s]);
+      if (lane == 0) {
+        if (bytes == 0) mbar_arrive(bar); else mbar_expect_tx(bar, bytes);
+      }
+      __syncwarp();
+      if (valid) tma_load_2d((kv == 0 ? sK : sV) + s * KV_BYTES + h * KV_HALF + x * p.unit * 128, &map_kv, h * 64, row_k, bar);
+      row = next;
+    }
+  } else if (warp == 1 || warp == MMA_WARP_B) {
+    if (lane == 0) {
+      // ---- MMA issue: one thread per row tile.  Each runs its tile's chain on its own, so neither waits for the other's softmax; the
+      // K and V stages go back to the producers when both have committed (or, without a second row tile, plainly arrived on) their
+      // empty barriers.
+      const int w = warp == 1 ? 0 : 1;
+      const bool on = w == 0 || b_on;
+      constexpr uint32_t idesc_qk = idesc_bf16(BM, BN, 0), idesc_pv = idesc_bf16(BM, D, 1);
+      const uint64_t dq = desc_k_major(sQ + w * Q_BYTES), dk = desc_k_major(sK);
+      const uint64_t dp = desc_k_major(sP + w * P_BYTES), dv = desc_mn_major(sV, KV_HALF);
+      const uint32_t o_tmem = tmem + O_COL + w * 128;
+      auto issue_qk = [&](int t) {                                  // S_w[t % 2] = Q_w K(t)^T
+        const uint64_t dks = dk + (uint64_t)((t % STAGES) * (KV_BYTES >> 4));
+        const uint32_t s_tmem = tmem + (2 * w + (t & 1)) * BN;
+#pragma unroll
+        for (int k = 0; k < D / 16; ++k)
+          tc_mma(s_tmem, dq + (uint64_t)(((k / 4) * Q_HALF + (k % 4) * 32) >> 4),
+                 dks + (uint64_t)(((k / 4) * KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
+        tc_commit(smem_u32(&s_full[w][t & 1]));
+      };
+      auto issue_pv = [&](int s, int j) {
+        const uint64_t dvs = dv + (uint64_t)(s * (KV_BYTES >> 4));
+#pragma unroll
+        for (int k = 0; k < BN / 16; ++k)
+          tc_mma(o_tmem, dp + (uint64_t)(k * 2), dvs + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+      };
+      bool ok = true;
+      if (on && !mbar_wait(smem_u32(&q_full), 0)) { s_abort = 1; atomicExch(p.status, 62); ok = false; }
+      auto take_k = [&](int t) {                                    // S of key tile t, or the stage handed back once it is full
+        if (!mbar_wait(smem_u32(&k_full[t % STAGES]), (t / STAGES) & 1)) { s_abort = 1; atomicExch(p.status, 63); ok = false; return; }
+        if (on) {
+          tc_fence_after();
+          issue_qk(t);
+          tc_commit(smem_u32(&k_empty[t % STAGES]));
+        } else {
+          mbar_arrive(smem_u32(&k_empty[t % STAGES]));
+        }
+      };
+      for (int t = 0; t < 2 && t < n_tiles && ok; ++t) take_k(t);
+      for (int j = 0; j < n_tiles && ok; ++j) {
+        const int s = j % STAGES;
+        if (on && !mbar_wait(smem_u32(&p_full[w]), j & 1)) { s_abort = 1; atomicExch(p.status, 64); ok = false; break; }
+        if (!mbar_wait(smem_u32(&v_full[s]), (j / STAGES) & 1)) { s_abort = 1; atomicExch(p.status, 63); ok = false; break; }
+        if (on) {
+          tc_fence_after();
+          issue_pv(s, j);
+          tc_commit(smem_u32(&pv_done[w]));                         // P_w is free again, O_w is quiet until the next P V
+          if (j + 1 == n_tiles) tc_commit(smem_u32(&o_full[w]));     // this row tile's last P V
+          tc_commit(smem_u32(&v_empty[s]));
+        } else {
+          mbar_arrive(smem_u32(&v_empty[s]));
+        }
+        if (j + 2 < n_tiles) take_k(j + 2);                          // into the buffer of S that tile j just left
+      }
+    }
+  } else {                                                          // ---- softmax and output: one thread per row
+    const int w = (warp - 2) >> 2;                                  // row tile A (warps 2..5) or B (warps 6..9)
+    const int quarter = warp & 3;
+    const int r = quarter * 32 + lane;
+    const int token = r / p.group;                                  // of the row tile
+    const bool row_ok = token < p.tile_tokens && w * p.tile_tokens + token < pair.z;
+    const int t = pair.y + w * p.tile_tokens + token;
+    const int pos = row_ok ? p.positions[t] : -1;
+    const int n_w = w == 0 || b_on ? n_tiles : 0;
+    const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
+    const uint32_t s_addr = lane_addr + 2 * w * BN, o_addr = lane_addr + O_COL + w * 128;
+    unsigned char* prow = smem_dyn + (sP - smem_u32(smem_dyn)) + w * P_BYTES + r * 128;
+    float m_run = -INFINITY, l_run = 0.f;                           // reference maximum (scaled, log2 units), running sum
+    bool ok = true;
+    // the keys of each entry of a tile that this row sees, a byte each (a tile has up to four entries): its bit, and what is not behind it
+    const int my_word = w * p.words + (row_ok ? token >> 5 : 0);
+    // (asked for a tile ahead and looked at only when the tile's turn comes)
+    unsigned word[4];
+    int first[4];
+    auto ask = [&](int j) {
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (x < p.per_tile) {
+          const int e = j * p.per_tile + x;
+          if (e < held) {
+            word[x] = s_bits[e * 2 * p.words + my_word];
+            first[x] = s_first[e];
+          } else {
+            word[x] = masks[(int64_t)e * 2 * p.words + my_word];
+            first[x] = entries[e].y;
+          }
+        }
+    };
+    const unsigned all_seen = p.per_tile == 1 ? 64u : p.per_tile == 2 ? 0x2020u : 0x10101010u;
+    if (n_w > 0) ask(0);
+    for (int j = 0; j < n_w; ++j) {
+      unsigned seen = 0;
+#pragma unroll
+      for (int x = 0; x < 4; ++x)
+        if (x < p.per_tile && row_ok && (word[x] >> (token & 31) & 1))
+          seen |= (unsigned)max(0, min(p.unit, pos - first[x] + 1)) << (8 * x);
+      if (j + 1 < n_w) ask(j + 1);
+      if (!mbar_wait(smem_u32(&s_full[w][j & 1]), (j >> 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
+      tc_fence_after();
+      if (!__any_sync(0xffffffffu, seen)) {                         // nothing here for the warp's rows: weights of zero
+        if (j > 0 && !mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
+#pragma unroll
+        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + (c << 4)) = make_uint4(0, 0, 0, 0);
+        tc_fence_before();
+        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+        mbar_arrive(smem_u32(&p_full[w]));
+        continue;
+      }
+      float s0[32], s1[32];
+      tmem_ld32(s_addr + (j & 1) * BN, s0);
+      tmem_ld32(s_addr + (j & 1) * BN + 32, s1);
+      tmem_ld_wait();
+      if (__any_sync(0xffffffffu, seen != all_seen)) {
+        if (p.per_tile == 1) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i >= (int)seen) s0[i] = -INFINITY;
+            if (i + 32 >= (int)seen) s1[i] = -INFINITY;
+          }
+        } else if (p.per_tile == 2) {
+          const int a = seen & 255, b = seen >> 8;
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (i >= a) s0[i] = -INFINITY;
+            if (i >= b) s1[i] = -INFINITY;
+          }
+        } else {
+          const int a = seen & 255, b = seen >> 8 & 255, c = seen >> 16 & 255, d = seen >> 24;
+#pragma unroll
+          for (int i = 0; i < 16; ++i) {
+            if (i >= a) s0[i] = -INFINITY;
+            if (i >= b) s0[16 + i] = -INFINITY;
+            if (i >= c) s1[i] = -INFINITY;
+            if (i >= d) s1[16 + i] = -INFINITY;
+          }
+        }
+      }
+      // maximum of the raw scores (the scale is positive), as eight short chains instead of one long one
+      float mq[8];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) mq[i] = fmaxf(s0[i], s1[i]);
+#pragma unroll
+      for (int i = 8; i < 32; ++i) mq[i & 7] = fmaxf(mq[i & 7], fmaxf(s0[i], s1[i]));
+      float mx = fmaxf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), fmaxf(fmaxf(mq[4], mq[5]), fmaxf(mq[6], mq[7])));
+      mx *= p.scale_log2;
+      // raise the reference maximum only when it grows by more than 8 (in log2 units)
+      const bool raise = mx > m_run + 8.f;
+      bool pv_seen = j == 0;                                        // P V of tile j-1 known to be complete
+      if (j > 0 && __any_sync(0xffffffffu, raise)) {
+        // O_w must be quiet: P V of tile j-1 complete (P V of tile j waits for our P)
+        if (!mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
+        tc_fence_after();
+        pv_seen = true;
+        const float alpha = raise ? fast_exp2(m_run - mx) : 1.f;     // m_run = -inf gives 0
+        l_run *= alpha;
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_ld_wait();
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] *= alpha;
+          tmem_st32(o_addr + c * 32, o);
+        }
+        tmem_st_wait();
+      }
+      if (raise) m_run = mx;
+      const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+      float sq[8];                                                  // eight partial sums: short dependency chains
+#pragma unroll
+      for (int i = 0; i < 8; ++i) sq[i] = 0.f;
+#pragma unroll
+      for (int i = 0; i < 32; ++i) {
+        s0[i] = fast_exp2(fmaf(s0[i], p.scale_log2, neg_m));         // masked: -inf stays -inf, 2^-inf = 0
+        s1[i] = fast_exp2(fmaf(s1[i], p.scale_log2, neg_m));
+        sq[i & 7] += s0[i] + s1[i];
+      }
+      l_run += ((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7]));
+      // the P V of tile j-1 must have read P before it is overwritten
+      if (!pv_seen) {
+        if (!mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
+      }
+      // P row r: 64 keys = 8 chunks of 16 bytes, swizzled like a K-major tile with 128-byte rows (rounded to bfloat16: 2^-9 of each
+      // weight; their sum is taken before)
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        const float* src = c < 4 ? s0 + c * 8 : s1 + (c - 4) * 8;
+        uint4 v;
+        v.x = pack_bf16(src[0], src[1]); v.y = pack_bf16(src[2], src[3]);
+        v.z = pack_bf16(src[4], src[5]); v.w = pack_bf16(src[6], src[7]);
+        *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = v;
+      }
+      tc_fence_before();
+      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+      mbar_arrive(smem_u32(&p_full[w]));
+    }
+    if (ok && n_w > 0) {
+      if (!mbar_wait(smem_u32(&o_full[w]), 0)) { s_abort = 1; atomicExch(p.status, 66); ok = false; }
+      tc_fence_after();
+    }
+    if (ok && (w == 0 || b_on)) {
+      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+      bool odd = false;
+      __nv_bfloat16* dst = row_ok ? p.out + (int64_t)t * p.ldo + (int64_t)(hk * p.group + r % p.group) * D : nullptr;
+#pragma unroll
+      for (int c = 0; c < D / 32; ++c) {
+        float o[32];
+        if (n_w > 0) {
+          tmem_ld32(o_addr + c * 32, o);
+          tmem_ld_wait();
+        }
+        if (l_run == 0.f)                                           // a row that sees nothing
+#pragma unroll
+          for (int i = 0; i < 32; ++i) o[i] = 0.f;
+        if (row_ok) {
+#pragma unroll
+          for (int i = 0; i < 32; ++i) odd |= !isfinite(o[i]);
+#pragma unroll
+          for (int q4 = 0; q4 < 4; ++q4) {
+            uint4 v;
+            v.x = pack_bf16(o[q4 * 8] * inv, o[q4 * 8 + 1] * inv); v.y = pack_bf16(o[q4 * 8 + 2] * inv, o[q4 * 8 + 3] * inv);
+            v.z = pack_bf16(o[q4 * 8 + 4] * inv, o[q4 * 8 + 5] * inv); v.w = pack_bf16(o[q4 * 8 + 6] * inv, o[q4 * 8 + 7] * inv);
+            reinterpret_cast<uint4*>(dst + c * 32)[q4] = v;
+          }
+        }
+      }
+      if (odd) s_odd = 1;
+    }
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  if (warp == 1) {
+    if (s_abort) {                                                  // copies and products in flight come to their end first
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+    }
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
+  }
+  if (s_odd) rows_again<D>(p, pair.x, pair.y, pair.z, hk);
+}
+
+typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
+                                  const cuuint32_t*, const cuuint32_t*, CUtensorMapInterleave, CUtensorMapSwizzle,
+                                  CUtensorMapL2promotion, CUtensorMapFloatOOBfill);
+EncodeTiledFn encode_fn() {
+  static EncodeTiledFn fn = [] {
+    void* f = nullptr;
+    cudaDriverEntryPointQueryResult q;
+    const bool ok = cudaGetDriverEntryPoint("cuTensorMapEncodeTiled", &f, cudaEnableDefault, &q) == cudaSuccess && q == cudaDriverEntryPointSuccess;
+    return reinterpret_cast<EncodeTiledFn>(ok ? f : nullptr);
+  }();
+  return fn;
+}
+
+template <int D>
+int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const Params& p, cudaStream_t stream) {
+  auto k = attention_pages_umma_kernel<D>;
+  constexpr size_t sm = smem_bytes<D>();
+  static thread_local int set_for = -1;                    // the attribute belongs to the device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (set_for != dev) {
+    if (cudaFuncSetAttribute(k, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)sm) != cudaSuccess)
+      return cuda_status("attention_pages_umma: shared memory");
+    set_for = dev;
+  }
+  launch_pdl(page_lists_kernel, dim3(p.Hkv, p.pairs), dim3(LIST_NT), 0, stream, p);
+  launch_pdl(k, dim3(p.Hkv, p.pairs), dim3(NTHREADS), sm, stream, mq, mkv, p);
+  return cuda_status("attention_pages_umma");
+}
+
+int64_t room(Params& p, unsigned char* at) {
+  p.tile_tokens = BM / p.group;
+  p.words = (p.tile_tokens + 31) / 32;
+  p.unit = p.page_size < BN ? p.page_size : BN;
+  p.per_tile = BN / p.unit;
+  const int64_t pairs = (int64_t)p.T / (2 * p.tile_tokens) + (p.B < p.T ? p.B : p.T);     // of every way the tokens may be dealt out
+  p.pairs = (int)(pairs > INT32_MAX ? INT32_MAX : pairs);
+  const int64_t most = (int64_t)2 * p.tile_tokens * p.top, pages = most < p.width ? most : p.width;
+  p.cap = (int)((pages * (p.page_size / p.unit) + p.per_tile - 1) / p.per_tile * p.per_tile);
+  unsigned char* start = at;
+  auto take = [&](int64_t bytes) { unsigned char* x = at; at += (bytes + 255) / 256 * 256; return x; };
+  const int64_t lists = pairs * p.Hkv;
+  p.counts = (int*)take(lists * 4);
+  p.entries = (int2*)take(lists * p.cap * 8);
+  p.masks = (unsigned*)take(lists * p.cap * 2 * p.words * 4);
+  return at - start;
+}
+
+constexpr int64_t MAX_ROOM = 1ll << 30;
+
+}  // namespace
+
+DINFER_DEFINE_LAST_ERROR()
+
+// Bytes of workspace that the call wants, 0 where it does not take the sizes.
+DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size) {
+  if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > BM || top <= 0 || width <= 0 || num_reqs <= 0 || (D != 64 && D != 128)) return 0;
+  if (page_size < 16 || page_size > 128 || (page_size & (page_size - 1)) || (int64_t)width * page_size > INT32_MAX) return 0;
+  Params p{};
+  p.width = width; p.B = num_reqs; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.page_size = page_size;
+  const int64_t bytes = room(p, nullptr);
+  return p.pairs > 65535 || bytes > MAX_ROOM ? 0 : bytes;
+}
+
+// As dinfer_attention_pages, for rows and bases on 16-byte boundaries and a positive scale.
+DINFER_API int dinfer_attention_pages_umma(const void* q, int64_t ldq, void* out, int64_t ldo, const void* cache, int num_pages,
+                                           const int* table, int width, const int* cu_seqlens, int num_reqs, const int* positions,
+                                           const int* chosen, int top, int T, int H, int Hkv, int D, int page_size, float scale,
+                                           void* workspace, int64_t workspace_bytes, int* status, cudaStream_t stream) {
+  const int64_t need = dinfer_attention_pages_umma_workspace(num_reqs, width, top, T, H, Hkv, D, page_size);
+  if (need == 0) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d width=%d", T, H, Hkv, D, page_size, top, width);
+  if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255) || !status)
+    return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: a workspace of %lld bytes and a status word are required", (long long)need);
+  if (!(scale > 0.f)) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: the score scale must be positive, got %g", (double)scale);
+  if ((ldq % 8) || (ldo % 8) || (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15))
+    return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: rows and bases must be 16-byte aligned");
+  const int64_t cache_rows = (int64_t)num_pages * 2 * Hkv * page_size;
+  if (num_pages <= 0 || cache_rows > INT32_MAX) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: %d pages are too many rows for a tensor map's coordinate", num_pages);
+  EncodeTiledFn fn = encode_fn();
+  if (!fn) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: cuTensorMapEncodeTiled is not available from this driver");
+  Params p{};
+  p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.out = (__nv_bfloat16*)out; p.ldo = ldo; p.cache = (const __nv_bfloat16*)cache;
+  p.num_pages = num_pages; p.table = table; p.width = width; p.cu = cu_seqlens; p.B = num_reqs; p.positions = positions;
+  p.chosen = chosen; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.page_size = page_size; p.scale = scale;
+  p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
+  room(p, (unsigned char*)workspace);
+  CUtensorMap mq, mkv;
+  {
+    cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};
+    cuuint64_t strides[2] = {(cuuint64_t)D * 2, (cuuint64_t)ldq * 2};
+    cuuint32_t box[3] = {64, (cuuint32_t)p.group, (cuuint32_t)p.tile_tokens};
+    cuuint32_t estr[3] = {1, 1, 1};
+    CUresult r = fn(&mq, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(q), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: tensor map of q failed with %d", (int)r);
+  }
+  {
+    cuuint64_t dims[2] = {(cuuint64_t)D, (cuuint64_t)cache_rows};
+    cuuint64_t strides[1] = {(cuuint64_t)D * 2};
+    cuuint32_t box[2] = {64, (cuuint32_t)p.unit};
+    cuuint32_t estr[2] = {1, 1};
+    CUresult r = fn(&mkv, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 2, const_cast<void*>(cache), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+                    CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+    if (r != CUDA_SUCCESS) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: tensor map of the cache failed with %d", (int)r);
+  }
+  return D == 64 ? launch<64>(mq, mkv, p, stream) : launch<128>(mq, mkv, p, stream);
+}

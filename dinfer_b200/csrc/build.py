@@ -56,6 +56,7 @@ LIBRARIES: Dict[str, tuple] = {
     "page_append": ("page_append.cu", []),
     "page_choice": ("page_choice.cu", []),
     "attention_pages": ("attention_pages.cu", []),
+    "attention_pages_umma": ("attention_pages_umma.cu", []),
     # host-side bookkeeping (page pools, cache manager, decode plans): plain C++, no CUDA
     "host_core": ("host_core.cpp", []),
 }

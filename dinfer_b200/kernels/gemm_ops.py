@@ -66,6 +66,12 @@ STATUS_MEANING = {
     47: "routed products: a warp waited for the experts' weights",
     51: "state-space chunks: the sums waited for their operands or their MMAs",
     52: "state-space chunks: the outputs waited for their operands or their MMAs",
+    61: "attention over chosen pages: a TMA producer waited for a free K or V stage",
+    62: "attention over chosen pages: an MMA thread waited for the Q tiles",
+    63: "attention over chosen pages: an MMA thread waited for a K or V tile",
+    64: "attention over chosen pages: an MMA thread waited for the softmax warps' P tile",
+    65: "attention over chosen pages: the softmax warps waited for a score tile or for P V to finish",
+    66: "attention over chosen pages: the softmax warps waited for the last P V before writing the output",
     53: "state-space chunks: the step has more portions than its launch was made for",
 }
 

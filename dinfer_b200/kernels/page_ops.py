@@ -17,19 +17,27 @@ from typing import Optional
 
 import torch
 
+from . import gemm_ops
 from .lib import DTYPE_CODE, KernelError, check, dtype_code, library, num_sms, ptr, require_cuda, stream_handle
 from .ops import _fn
 
 
-# Steps of at least so many tokens turn the attention round: pages meet the tokens that chose them, through a workspace.
+# Steps of at least so many tokens, and so many a request, walk the pages that neighbouring tokens chose together
 PORTION_TOKENS = 64
+PORTION_TOKENS_A_REQUEST = 4
 
 
-def _workspace(num_reqs: int, width: int, top: int, T: int, num_heads: int, num_kv_heads: int, head_dim: int) -> int:
-    """Bytes that the portions' form needs (0: it does not take these sizes)."""
-    f = library("attention_pages").dinfer_attention_pages_workspace
-    f.argtypes, f.restype = [c_int] * 7, c_int64
-    return f(num_reqs, width, top, T, num_heads, num_kv_heads, head_dim)
+def _portions(q, out, cache, block_table, top: int, scale: float) -> int:
+    """Bytes of workspace of the kernel for portions where it takes this call, else 0: bfloat16 rows that TMA can address, a positive
+    scale, enough tokens."""
+    T, B = q.shape[0], block_table.shape[0]
+    if T < PORTION_TOKENS or T < PORTION_TOKENS_A_REQUEST * B or q.dtype != torch.bfloat16 or not scale > 0:
+        return 0
+    if q.stride(0) % 8 or out.stride(0) % 8 or (q.data_ptr() | out.data_ptr() | cache.data_ptr()) % 16 or cache.numel() // cache.shape[-1] > 0x7fffffff:
+        return 0
+    f = library("attention_pages_umma").dinfer_attention_pages_umma_workspace
+    f.argtypes, f.restype = [c_int] * 8, c_int64
+    return f(B, block_table.shape[1], top, T, q.shape[1] // cache.shape[4], cache.shape[2], cache.shape[4], cache.shape[3])
 
 
 def _here(what: str, *tensors) -> None:
@@ -196,15 +204,16 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     if chosen.dim() != 3 or tuple(chosen.shape[:2]) != (T, Hkv) or chosen.shape[2] == 0:
         raise KernelError(f"{what}: chosen int32 [T, Hkv, top] with top > 0")
     top = chosen.shape[2]
-    size, work = 0, None
-    if T >= PORTION_TOKENS and q.dtype == torch.bfloat16:
-        size = _workspace(block_table.shape[0], block_table.shape[1], top, T, num_heads, Hkv, D)
-        if size > 0:
-            work = torch.empty(size, dtype=torch.uint8, device=q.device)
-    lib, f = _fn("attention_pages", "dinfer_attention_pages",
-                 [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-                  c_int, c_int, c_int, c_int, c_int, c_int, c_float, c_void_p, c_int64, c_int, c_int, c_void_p])
-    check(lib, f(ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(cache), num_pages, ptr(block_table), block_table.shape[1],
-                 ptr(cu_seqlens), block_table.shape[0], ptr(positions), ptr(chosen), top, T, num_heads, Hkv, D, page_size,
-                 scale, ptr(work), size, num_sms(), DTYPE_CODE[q.dtype], stream_handle()), what)
+    head = (ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(cache), num_pages, ptr(block_table), block_table.shape[1],
+            ptr(cu_seqlens), block_table.shape[0], ptr(positions), ptr(chosen), top, T, num_heads, Hkv, D, page_size, scale)
+    types = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
+             c_int, c_int, c_int, c_int, c_int, c_int, c_float]
+    size = _portions(q, out, cache, block_table, top, scale)
+    if size:
+        work = torch.empty(size, dtype=torch.uint8, device=q.device)
+        lib, f = _fn("attention_pages_umma", "dinfer_attention_pages_umma", types + [c_void_p, c_int64, c_void_p, c_void_p])
+        check(lib, f(*head, ptr(work), size, ptr(gemm_ops._state(q.device)["status"]), stream_handle()), "attention_pages_umma")
+        return out
+    lib, f = _fn("attention_pages", "dinfer_attention_pages", types + [c_int, c_int, c_void_p])
+    check(lib, f(*head, num_sms(), DTYPE_CODE[q.dtype], stream_handle()), what)
     return out

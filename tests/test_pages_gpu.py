@@ -209,7 +209,9 @@ def choices(b, G, top, g, kind):
 
 
 ATTENTION = SIZES + [([(2000, 200), (0, 300)], 16, 8, 2, 128), ([(777, 300)], 64, 16, 1, 64), ([(640, 150)], 32, 12, 4, 128),
-                     ([(256, 130), (31, 1), (100, 1), (2, 2)], 64, 8, 8, 128), ([(400, 90)], 128, 4, 2, 64), ([(50, 40)] * 5, 16, 10, 2, 128)]
+                     ([(256, 130), (31, 1), (100, 1), (2, 2)], 64, 8, 8, 128), ([(400, 90)], 128, 4, 2, 64), ([(50, 40)] * 5, 16, 10, 2, 128),
+                     ([(3000, 500), (20, 90), (500, 1)], 64, 8, 2, 128), ([(70, 300)], 32, 6, 2, 64), ([(0, 129), (4000, 64)], 16, 32, 2, 64),
+                     ([(1, 200)], 16, 3, 3, 128)]
 
 
 @pytest.mark.parametrize("kind", ["usual", "far", "odd"])
@@ -247,7 +249,9 @@ def test_attention(size, dtype, kind):
 @pytest.mark.parametrize("what", ["value", "key"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 def test_no_token_sees_a_later_one(dtype, what, new):
-    """A NaN in a token's own key or value reaches the tokens from it on that read its page, and nothing before or beside."""
+    """A NaN in a token's own key or value reaches the tokens from it on that read its page, and nothing before or beside: those are
+    what they are without it, up to the bound that every result keeps (the kernel for portions makes the rows beside such a value
+    again, one by one, with sums in another order)."""
     from dinfer_b200.kernels import page_ops
     if dtype == F32 and new > 100:
         new = 100
@@ -258,7 +262,7 @@ def test_no_token_sees_a_later_one(dtype, what, new):
     cache = torch.randn(b.num_pages, 2, G, P, D, generator=g).to(dtype)
     chosen = choices(b, G, 3, g, "usual")
     args = (c(b.table), c(b.cu), c(b.positions), c(chosen), H, 0.1)
-    clean = page_ops.attention_pages(c(q), torch.empty_like(c(q)), c(cache), *args).cpu()
+    clean, size, qk = plain_attention(q, cache, b, chosen, H, 0.1)
     at = 100 + new // 2
     cache[int(b.table[0, at // P]), 0 if what == "key" else 1, 1, at % P, 7] = math.nan
     got = page_ops.attention_pages(c(q), torch.empty_like(c(q)), c(cache), *args).cpu()
@@ -266,7 +270,7 @@ def test_no_token_sees_a_later_one(dtype, what, new):
     heads = torch.arange(H * D) // D >= H // G
     hit = reaches[:, None] & heads[None] & (torch.ones(H * D, dtype=torch.bool) if what == "key" else torch.arange(H * D) % D == 7)
     assert torch.equal(torch.isnan(got), hit)
-    assert torch.equal(got[~hit], clean[~hit])
+    assert bool(((got.double() - clean).abs() <= attention_bound(dtype, D, clean, size, qk))[~hit].all())
 
 
 @pytest.mark.parametrize("new", [1, 200])
