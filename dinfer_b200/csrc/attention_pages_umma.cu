@@ -199,7 +199,8 @@ template <int D> constexpr size_t smem_bytes() {
   return (size_t)(2 * BM * D * 2 + 2 * STAGES * BN * D * 2 + 2 * BM * BN * 2) + 1024;
 }
 
-template <int D>
+// NP: entries of a key tile
+template <int D, int NP>
 __global__ void __launch_bounds__(NTHREADS, 1)
 attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Params p) {
   constexpr int NH = D / 64;                          // 64-wide halves of the head
@@ -338,7 +339,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       for (int t = 0; t < 2 && t < n_tiles && ok; ++t) take_k(t);
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int s = j % STAGES;
-        if (on && !mbar_wait(smem_u32(&p_full[w]), j & 1)) { s_abort = 1; atomicExch(p.status, 64); ok = false; break; }
+        if (on && !mbar_spin(smem_u32(&p_full[w]), j & 1)) { s_abort = 1; atomicExch(p.status, 64); ok = false; break; }
         if (!mbar_wait(smem_u32(&v_full[s]), (j / STAGES) & 1)) { s_abort = 1; atomicExch(p.status, 63); ok = false; break; }
         if (on) {
           tc_fence_after();
@@ -366,81 +367,65 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     unsigned char* prow = smem_dyn + (sP - smem_u32(smem_dyn)) + w * P_BYTES + r * 128;
     float m_run = -INFINITY, l_run = 0.f;                           // reference maximum (scaled, log2 units), running sum
     bool ok = true;
-    // the keys of each entry of a tile that this row sees, a byte each (a tile has up to four entries): its bit, and what is not behind it
-    const int my_word = w * p.words + (row_ok ? token >> 5 : 0);
-    // (asked for a tile ahead and looked at only when the tile's turn comes)
-    unsigned word[4];
-    int first[4];
-    auto ask = [&](int j) {
+    const int my_word = w * p.words + (row_ok ? token >> 5 : 0), my_bit = token & 31, bits = 2 * p.words;
+    constexpr int UNIT = BN / NP;
+    // the keys of each entry of a tile that this row sees, by its bit and by what is not behind it; made for the next tile
+    // when a tile's weights have been handed over
+    int seen[NP];
+    auto look = [&](int j) {
 #pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (x < p.per_tile) {
-          const int e = j * p.per_tile + x;
-          if (e < held) {
-            word[x] = s_bits[e * 2 * p.words + my_word];
-            first[x] = s_first[e];
-          } else {
-            word[x] = masks[(int64_t)e * 2 * p.words + my_word];
-            first[x] = entries[e].y;
-          }
-        }
+      for (int x = 0; x < NP; ++x) {
+        const int e = j * NP + x;
+        const unsigned word = e < held ? s_bits[e * bits + my_word] : masks[(int64_t)e * bits + my_word];
+        const int first = e < held ? s_first[e] : entries[e].y;
+        seen[x] = row_ok && (word >> my_bit & 1) ? max(0, min(UNIT, pos - first + 1)) : 0;
+      }
     };
-    const unsigned all_seen = p.per_tile == 1 ? 64u : p.per_tile == 2 ? 0x2020u : 0x10101010u;
-    if (n_w > 0) ask(0);
+    if (n_w > 0) look(0);
     for (int j = 0; j < n_w; ++j) {
-      unsigned seen = 0;
-#pragma unroll
-      for (int x = 0; x < 4; ++x)
-        if (x < p.per_tile && row_ok && (word[x] >> (token & 31) & 1))
-          seen |= (unsigned)max(0, min(p.unit, pos - first[x] + 1)) << (8 * x);
-      if (j + 1 < n_w) ask(j + 1);
       if (!mbar_wait(smem_u32(&s_full[w][j & 1]), (j >> 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
       tc_fence_after();
-      if (!__any_sync(0xffffffffu, seen)) {                         // nothing here for the warp's rows: weights of zero
+      bool some = false, part = false;
+#pragma unroll
+      for (int x = 0; x < NP; ++x) {
+        some |= seen[x] > 0;
+        part |= seen[x] > 0 && seen[x] < UNIT;
+      }
+      if (!__any_sync(0xffffffffu, some)) {                         // nothing here for the warp's rows: weights of zero
         if (j > 0 && !mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
 #pragma unroll
         for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + (c << 4)) = make_uint4(0, 0, 0, 0);
         tc_fence_before();
         asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
         mbar_arrive(smem_u32(&p_full[w]));
+        if (j + 1 < n_w) look(j + 1);
         continue;
       }
-      float s0[32], s1[32];
-      tmem_ld32(s_addr + (j & 1) * BN, s0);
-      tmem_ld32(s_addr + (j & 1) * BN + 32, s1);
+      float s0[64];
+      tmem_ld32(s_addr + (j & 1) * BN, *reinterpret_cast<float(*)[32]>(s0));
+      tmem_ld32(s_addr + (j & 1) * BN + 32, *reinterpret_cast<float(*)[32]>(s0 + 32));
       tmem_ld_wait();
-      if (__any_sync(0xffffffffu, seen != all_seen)) {
-        if (p.per_tile == 1) {
+      if (__any_sync(0xffffffffu, part)) {                          // (the token's own page)
 #pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i >= (int)seen) s0[i] = -INFINITY;
-            if (i + 32 >= (int)seen) s1[i] = -INFINITY;
-          }
-        } else if (p.per_tile == 2) {
-          const int a = seen & 255, b = seen >> 8;
-#pragma unroll
-          for (int i = 0; i < 32; ++i) {
-            if (i >= a) s0[i] = -INFINITY;
-            if (i >= b) s1[i] = -INFINITY;
-          }
-        } else {
-          const int a = seen & 255, b = seen >> 8 & 255, c = seen >> 16 & 255, d = seen >> 24;
-#pragma unroll
-          for (int i = 0; i < 16; ++i) {
-            if (i >= a) s0[i] = -INFINITY;
-            if (i >= b) s0[16 + i] = -INFINITY;
-            if (i >= c) s1[i] = -INFINITY;
-            if (i >= d) s1[16 + i] = -INFINITY;
-          }
-        }
+        for (int i = 0; i < BN; ++i)
+          if (i % UNIT >= seen[i / UNIT]) s0[i] = -INFINITY;
       }
-      // maximum of the raw scores (the scale is positive), as eight short chains instead of one long one
-      float mq[8];
+      // maximum of the raw scores of the entries that the row sees (the scale is positive), as short chains
+      float mx = -INFINITY;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) mq[i] = fmaxf(s0[i], s1[i]);
+      for (int x = 0; x < NP; ++x) {
+        constexpr int CH = UNIT < 32 ? 4 : 8;
+        float mq[CH];
 #pragma unroll
-      for (int i = 8; i < 32; ++i) mq[i & 7] = fmaxf(mq[i & 7], fmaxf(s0[i], s1[i]));
-      float mx = fmaxf(fmaxf(fmaxf(mq[0], mq[1]), fmaxf(mq[2], mq[3])), fmaxf(fmaxf(mq[4], mq[5]), fmaxf(mq[6], mq[7])));
+        for (int i = 0; i < CH; ++i) mq[i] = s0[x * UNIT + i];
+#pragma unroll
+        for (int i = CH; i < UNIT; ++i) mq[i % CH] = fmaxf(mq[i % CH], s0[x * UNIT + i]);
+#pragma unroll
+        for (int i = CH / 2; i > 0; i >>= 1)
+#pragma unroll
+          for (int k = 0; k < i; ++k) mq[k] = fmaxf(mq[k], mq[k + i]);
+        if (seen[x] > 0) mx = fmaxf(mx, mq[0]);
+      }
       mx *= p.scale_log2;
       // raise the reference maximum only when it grows by more than 8 (in log2 units)
       const bool raise = mx > m_run + 8.f;
@@ -465,14 +450,19 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       }
       if (raise) m_run = mx;
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
+      // 2^(s * scale - m); of an entry that the row does not see 2^-inf = 0 (a score there that is not a finite number makes the row's
+      // sums one that is not, and the block's rows are made again)
       float sq[8];                                                  // eight partial sums: short dependency chains
 #pragma unroll
       for (int i = 0; i < 8; ++i) sq[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) {
-        s0[i] = fast_exp2(fmaf(s0[i], p.scale_log2, neg_m));         // masked: -inf stays -inf, 2^-inf = 0
-        s1[i] = fast_exp2(fmaf(s1[i], p.scale_log2, neg_m));
-        sq[i & 7] += s0[i] + s1[i];
+      for (int x = 0; x < NP; ++x) {
+        const float neg = seen[x] > 0 ? neg_m : -INFINITY;
+#pragma unroll
+        for (int i = x * UNIT; i < (x + 1) * UNIT; ++i) {
+          s0[i] = fast_exp2(fmaf(s0[i], p.scale_log2, neg));
+          sq[i & 7] += s0[i];
+        }
       }
       l_run += ((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7]));
       // the P V of tile j-1 must have read P before it is overwritten
@@ -483,7 +473,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       // weight; their sum is taken before)
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
-        const float* src = c < 4 ? s0 + c * 8 : s1 + (c - 4) * 8;
+        const float* src = s0 + c * 8;
         uint4 v;
         v.x = pack_bf16(src[0], src[1]); v.y = pack_bf16(src[2], src[3]);
         v.z = pack_bf16(src[4], src[5]); v.w = pack_bf16(src[6], src[7]);
@@ -492,6 +482,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       tc_fence_before();
       asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
       mbar_arrive(smem_u32(&p_full[w]));
+      if (j + 1 < n_w) look(j + 1);
     }
     if (ok && n_w > 0) {
       if (!mbar_wait(smem_u32(&o_full[w]), 0)) { s_abort = 1; atomicExch(p.status, 66); ok = false; }
@@ -499,7 +490,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     }
     if (ok && (w == 0 || b_on)) {
       const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-      bool odd = false;
+      bool odd = row_ok && !(l_run == l_run);
       __nv_bfloat16* dst = row_ok ? p.out + (int64_t)t * p.ldo + (int64_t)(hk * p.group + r % p.group) * D : nullptr;
 #pragma unroll
       for (int c = 0; c < D / 32; ++c) {
@@ -552,9 +543,9 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
-template <int D>
+template <int D, int NP>
 int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const Params& p, cudaStream_t stream) {
-  auto k = attention_pages_umma_kernel<D>;
+  auto k = attention_pages_umma_kernel<D, NP>;
   constexpr size_t sm = smem_bytes<D>();
   static thread_local int set_for = -1;                    // the attribute belongs to the device
   int dev = 0;
@@ -644,5 +635,9 @@ DINFER_API int dinfer_attention_pages_umma(const void* q, int64_t ldq, void* out
                     CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
     if (r != CUDA_SUCCESS) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: tensor map of the cache failed with %d", (int)r);
   }
-  return D == 64 ? launch<64>(mq, mkv, p, stream) : launch<128>(mq, mkv, p, stream);
+  switch (p.per_tile) {
+    case 1: return D == 64 ? launch<64, 1>(mq, mkv, p, stream) : launch<128, 1>(mq, mkv, p, stream);
+    case 2: return D == 64 ? launch<64, 2>(mq, mkv, p, stream) : launch<128, 2>(mq, mkv, p, stream);
+    default: return D == 64 ? launch<64, 4>(mq, mkv, p, stream) : launch<128, 4>(mq, mkv, p, stream);
+  }
 }
