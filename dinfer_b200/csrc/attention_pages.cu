@@ -390,11 +390,39 @@ bool tensor_cores(const void* q, const void* out, const void* cache, const Pages
 }
 }  // namespace
 
-// chosen int32 [T, Hkv, top]; cache [num_pages, 2, Hkv, page_size, D].
-DINFER_API int dinfer_attention_pages(const void* q, int64_t ldq, void* out, int64_t ldo, const void* cache, int num_pages,
-                                      const int* table, int width, const int* cu_seqlens, int num_reqs, const int* positions,
-                                      const int* chosen, int top, int T, int H, int Hkv, int D, int page_size, float scale,
-                                      int sms, int dtype, cudaStream_t stream) {
+// What the call takes, 8 bytes a field (a caller packs them and hands over one address).  chosen int32 [T, Hkv,
+// top]; cache [num_pages, 2, Hkv, page_size, D]; sms: the device's multiprocessors.
+struct AttentionPagesArgs {
+  const void* q;
+  int64_t ldq;
+  void* out;
+  int64_t ldo;
+  const void* cache;
+  int64_t num_pages;
+  const int* table;
+  int64_t width;
+  const int* cu_seqlens;
+  int64_t num_reqs;
+  const int *positions, *chosen;
+  int64_t top, T, H, Hkv, D, page_size;
+  double scale;
+  int64_t sms, dtype;
+  cudaStream_t stream;
+};
+
+DINFER_API int dinfer_attention_pages(const AttentionPagesArgs* a) {
+  const int64_t most = 0x7fffffff;
+  if (a->num_pages > most || a->width > most || a->num_reqs >= most || a->top > most || a->T > most / 8 || a->H > most || a->Hkv > most || a->D > most || a->page_size > most)
+    return refuse(DINFER_BAD_ARGUMENT, "attention_pages: a size beyond 32 bits");
+  const void *q = a->q, *cache = a->cache;
+  void* out = a->out;
+  const int64_t ldq = a->ldq, ldo = a->ldo;
+  const int *table = a->table, *cu_seqlens = a->cu_seqlens, *positions = a->positions, *chosen = a->chosen;
+  const int num_pages = (int)a->num_pages, width = (int)a->width, num_reqs = (int)a->num_reqs, top = (int)a->top, T = (int)a->T, H = (int)a->H,
+            Hkv = (int)a->Hkv, D = (int)a->D, page_size = (int)a->page_size;
+  const float scale = (float)a->scale;
+  cudaStream_t stream = a->stream;
+  const int sms = (int)a->sms, dtype = (int)a->dtype;
   if (T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 512 || page_size <= 0 || num_reqs <= 0 || top <= 0 || width < 0)
     return refuse(DINFER_BAD_ARGUMENT, "attention_pages: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d", T, H, Hkv, D, page_size, top);
   if ((H + WARPS - 1) / WARPS > 65535) return refuse(DINFER_BAD_ARGUMENT, "attention_pages: %d heads", H);

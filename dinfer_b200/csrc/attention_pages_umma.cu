@@ -594,11 +594,43 @@ DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width
   return p.pairs > 65535 || bytes > MAX_ROOM ? 0 : bytes;
 }
 
-// As dinfer_attention_pages, for rows and bases on 16-byte boundaries and a positive scale.
-DINFER_API int dinfer_attention_pages_umma(const void* q, int64_t ldq, void* out, int64_t ldo, const void* cache, int num_pages,
-                                           const int* table, int width, const int* cu_seqlens, int num_reqs, const int* positions,
-                                           const int* chosen, int top, int T, int H, int Hkv, int D, int page_size, float scale,
-                                           void* workspace, int64_t workspace_bytes, int* status, cudaStream_t stream) {
+// What the call takes, 8 bytes a field (a caller packs them and hands over one address).  As
+// dinfer_attention_pages, for rows and bases on 16-byte boundaries and a positive scale.
+struct AttentionPagesArgs {
+  const void* q;
+  int64_t ldq;
+  void* out;
+  int64_t ldo;
+  const void* cache;
+  int64_t num_pages;
+  const int* table;
+  int64_t width;
+  const int* cu_seqlens;
+  int64_t num_reqs;
+  const int *positions, *chosen;
+  int64_t top, T, H, Hkv, D, page_size;
+  double scale;
+  void* workspace;
+  int64_t workspace_bytes;
+  int* status;
+  cudaStream_t stream;
+};
+
+DINFER_API int dinfer_attention_pages_umma(const AttentionPagesArgs* a) {
+  const int64_t most = 0x7fffffff;
+  if (a->num_pages > most || a->width > most || a->num_reqs >= most || a->top > most || a->T > most / 8 || a->H > most || a->Hkv > most || a->D > most || a->page_size > most)
+    return refuse(DINFER_BAD_ARGUMENT, "attention_pages: a size beyond 32 bits");
+  const void *q = a->q, *cache = a->cache;
+  void* out = a->out;
+  const int64_t ldq = a->ldq, ldo = a->ldo;
+  const int *table = a->table, *cu_seqlens = a->cu_seqlens, *positions = a->positions, *chosen = a->chosen;
+  const int num_pages = (int)a->num_pages, width = (int)a->width, num_reqs = (int)a->num_reqs, top = (int)a->top, T = (int)a->T, H = (int)a->H,
+            Hkv = (int)a->Hkv, D = (int)a->D, page_size = (int)a->page_size;
+  const float scale = (float)a->scale;
+  cudaStream_t stream = a->stream;
+  void* workspace = a->workspace;
+  const int64_t workspace_bytes = a->workspace_bytes;
+  int* status = a->status;
   const int64_t need = dinfer_attention_pages_umma_workspace(num_reqs, width, top, T, H, Hkv, D, page_size);
   if (need == 0) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d width=%d", T, H, Hkv, D, page_size, top, width);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255) || !status)

@@ -360,21 +360,41 @@ int run(const void* qkv, void* q_out, const void* qw, const void* kw, void* cach
 
 }  // namespace
 
-// w_dtype: element type of the norm weights (both given or neither).  cos_sin: f32 [table_rows, rot], rot 0: no rotation.
-DINFER_API int dinfer_page_append(const void* qkv, int64_t ld, const int* positions, const void* q_weight,
-                                  const void* k_weight, float eps, const float* cos_sin, int table_rows, int rot,
-                                  int interleaved, void* q_out, int64_t ldq, void* cache, void* means, const int* slots,
-                                  int num_pages, int page_size, int T, int H, int Hkv, int D, int dtype, int w_dtype,
-                                  cudaStream_t stream) {
-  if (T < 0 || H <= 0 || Hkv <= 0 || D <= 0 || page_size <= 0 || num_pages < 0)
-    return refuse(DINFER_BAD_ARGUMENT, "page_append: sizes T=%d H=%d Hkv=%d D=%d page=%d", T, H, Hkv, D, page_size);
-  if (D > MAX_D) return refuse(DINFER_BAD_ARGUMENT, "page_append: head size %d is above %d", D, MAX_D);
-  if (rot < 0 || rot > D || rot % 2 || (rot > 0 && (!cos_sin || table_rows <= 0)))
-    return refuse(DINFER_BAD_ARGUMENT, "page_append: %d turned elements of %d, %d angle rows", rot, D, table_rows);
-  if (T == 0) return DINFER_OK;
-  const Append p{ld, ldq, positions, eps, cos_sin, table_rows, rot, interleaved, slots, num_pages, page_size, H, Hkv, D};
-  DINFER_DISPATCH_DTYPE(dtype, TA, {
-    DINFER_DISPATCH_DTYPE(w_dtype, TW, { return (run<TA, TW>(qkv, q_out, q_weight, k_weight, cache, means, p, T, stream)); });
+// What the call takes, 8 bytes a field (a caller packs them and hands over one address).  w_dtype: element type of the norm weights (both
+// given or neither); cos_sin: f32 [table_rows, rot], rot 0: no rotation.
+struct PageAppendArgs {
+  const void* qkv;
+  int64_t ld;
+  const int* positions;
+  const void *q_weight, *k_weight;
+  double eps;
+  const float* cos_sin;
+  int64_t table_rows, rot, interleaved;
+  void* q_out;
+  int64_t ldq;
+  void *cache, *means;
+  const int* slots;
+  int64_t num_pages, page_size, T, H, Hkv, D, dtype, w_dtype;
+  cudaStream_t stream;
+};
+
+DINFER_API int dinfer_page_append(const PageAppendArgs* args) {
+  const PageAppendArgs& a = *args;
+  const int64_t most = 0x7fffffff;
+  if (a.T < 0 || a.H <= 0 || a.Hkv <= 0 || a.D <= 0 || a.page_size <= 0 || a.num_pages < 0 || a.T > most / 16 || a.H > 65535 || a.Hkv > 65535 ||
+      a.page_size > most || a.num_pages * a.page_size > most || a.table_rows > most)
+    return refuse(DINFER_BAD_ARGUMENT, "page_append: sizes T=%lld H=%lld Hkv=%lld D=%lld, %lld pages of %lld", (long long)a.T, (long long)a.H,
+                  (long long)a.Hkv, (long long)a.D, (long long)a.num_pages, (long long)a.page_size);
+  if (a.D > MAX_D) return refuse(DINFER_BAD_ARGUMENT, "page_append: head size %lld is above %d", (long long)a.D, MAX_D);
+  if (a.rot < 0 || a.rot > a.D || a.rot % 2 || (a.rot > 0 && (!a.cos_sin || a.table_rows <= 0)))
+    return refuse(DINFER_BAD_ARGUMENT, "page_append: %lld turned elements of %lld, %lld angle rows", (long long)a.rot, (long long)a.D, (long long)a.table_rows);
+  if (a.T == 0) return DINFER_OK;
+  const Append p{a.ld, a.ldq, a.positions, (float)a.eps, a.cos_sin, (int)a.table_rows, (int)a.rot, (int)a.interleaved, a.slots,
+                 (int)a.num_pages, (int)a.page_size, (int)a.H, (int)a.Hkv, (int)a.D};
+  DINFER_DISPATCH_DTYPE(a.dtype, TA, {
+    DINFER_DISPATCH_DTYPE(a.w_dtype, TW, {
+      return (run<TA, TW>(a.qkv, a.q_out, a.q_weight, a.k_weight, a.cache, a.means, p, (int)a.T, a.stream));
+    });
   });
 }
 

@@ -428,9 +428,32 @@ choose_block_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
 }  // namespace
 
 // out[t * ldt + g * ldg + j] for j < pages; rows behind the last request's tokens are left as they are.
-DINFER_API int dinfer_page_scores(const void* q, int64_t ldq, const void* means, int num_pages, const int* table, int width,
-                                  const int* cu_seqlens, int num_reqs, const int* positions, float* out, int64_t ldt, int64_t ldg,
-                                  int T, int H, int Hkv, int D, int page_size, int pages, int dtype, cudaStream_t stream) {
+// (The arguments of the calls lie in one struct, 8 bytes a field: a caller packs them and hands over one address.)
+struct PageScoresArgs {
+  const void* q;
+  int64_t ldq;
+  const void* means;
+  int64_t num_pages;
+  const int* table;
+  int64_t width;
+  const int* cu_seqlens;
+  int64_t num_reqs;
+  const int* positions;
+  float* out;
+  int64_t ldt, ldg, T, H, Hkv, D, page_size, pages, dtype;
+  cudaStream_t stream;
+};
+
+DINFER_API int dinfer_page_scores(const PageScoresArgs* a) {
+  const void *q = a->q, *means = a->means;
+  const int64_t ldq = a->ldq, ldt = a->ldt, ldg = a->ldg, most = 0x7fffffff;
+  const int *table = a->table, *cu_seqlens = a->cu_seqlens, *positions = a->positions;
+  float* out = a->out;
+  cudaStream_t stream = a->stream;
+  if (a->T > most || a->num_pages > most || a->width > most || a->num_reqs >= most || a->H > most || a->Hkv > most || a->D > most || a->page_size > most || a->pages > most)
+    return refuse(DINFER_BAD_ARGUMENT, "page_scores: a size beyond 32 bits");
+  const int num_pages = (int)a->num_pages, width = (int)a->width, num_reqs = (int)a->num_reqs, T = (int)a->T, H = (int)a->H, Hkv = (int)a->Hkv,
+            D = (int)a->D, page_size = (int)a->page_size, pages = (int)a->pages, dtype = (int)a->dtype;
   if (T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || page_size <= 0 || num_reqs <= 0 || pages < 0 || pages > width)
     return refuse(DINFER_BAD_ARGUMENT, "page_scores: sizes T=%d H=%d Hkv=%d D=%d page=%d pages=%d of %d", T, H, Hkv, D,
                   page_size, pages, width);
@@ -462,8 +485,26 @@ DINFER_API int dinfer_page_scores(const void* q, int64_t ldq, const void* means,
 }
 
 // scores [t * ldt + g * ldg + j], j < pages; out int32 [T, Hkv, top].  recent >= 1 (a token's own page is always read).
-DINFER_API int dinfer_choose_pages(const float* scores, int64_t ldt, int64_t ldg, const int* positions, int page_size, int first,
-                                   int recent, int top, int pages, int* out, int T, int Hkv, cudaStream_t stream) {
+struct ChoosePagesArgs {
+  const float* scores;
+  int64_t ldt, ldg;
+  const int* positions;
+  int64_t page_size, first, recent, top, pages;
+  int* out;
+  int64_t T, Hkv;
+  cudaStream_t stream;
+};
+
+DINFER_API int dinfer_choose_pages(const ChoosePagesArgs* a) {
+  const float* scores = a->scores;
+  const int64_t ldt = a->ldt, ldg = a->ldg, most = 0x3fffffff;
+  const int* positions = a->positions;
+  int* out = a->out;
+  cudaStream_t stream = a->stream;
+  if (a->page_size > most || a->first > most || a->recent > most || a->top > most || a->pages > most || a->T > most || a->Hkv > most)
+    return refuse(DINFER_BAD_ARGUMENT, "choose_pages: a size beyond 30 bits");
+  const int page_size = (int)a->page_size, first = (int)a->first, recent = (int)a->recent, top = (int)a->top, pages = (int)a->pages,
+            T = (int)a->T, Hkv = (int)a->Hkv;
   if (T < 0 || Hkv <= 0 || page_size <= 0 || pages <= 0 || first < 0 || recent < 1 || top < first + recent)
     return refuse(DINFER_BAD_ARGUMENT, "choose_pages: sizes T=%d Hkv=%d page=%d pages=%d, %d first and %d recent of %d", T, Hkv,
                   page_size, pages, first, recent, top);

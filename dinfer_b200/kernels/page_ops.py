@@ -12,14 +12,50 @@ up to 512, any number of heads per key/value head, any page size.  Bfloat16 with
 """
 from __future__ import annotations
 
-from ctypes import c_float, c_int, c_int64, c_void_p
+import struct
+from ctypes import c_char_p, c_int, c_int64
 from typing import Optional
 
 import torch
 
 from . import gemm_ops
-from .lib import DTYPE_CODE, KernelError, check, dtype_code, library, num_sms, ptr, require_cuda, stream_handle
+from .lib import DTYPE_CODE, KernelError, check, library, num_sms, require_cuda
 from .ops import _fn
+
+_I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
+
+# A decode step of few tokens is as long as its calls take the host.  So the arguments of a call go as one packed struct (24 of them one
+# by one cost ctypes 2.8 us, packed 0.5), the stream last, and the checks ask each tensor once for each thing.
+_PACK = {
+    "dinfer_page_append": struct.Struct("5qd18q").pack,
+    "dinfer_page_scores": struct.Struct("20q").pack,
+    "dinfer_choose_pages": struct.Struct("13q").pack,
+    "dinfer_attention_pages": struct.Struct("18qd3q").pack,
+    "dinfer_attention_pages_umma": struct.Struct("18qd4q").pack,
+}
+_BOUND = {}
+_SMS = {}                               # multiprocessors by device
+
+
+def _call(libname: str, fname: str, what: str, *args) -> None:
+    """The library's function on the current stream."""
+    bound = _BOUND.get(fname)
+    if bound is None:
+        bound = _BOUND[fname] = _fn(libname, fname, [c_char_p]) + (_PACK[fname],)
+    lib, f, pack = bound
+    check(lib, f(pack(*args, _stream())), what)
+
+
+_raw_device = getattr(torch._C, "_cuda_getDevice", None)
+_raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+
+
+def _device() -> int:
+    return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
+def _stream() -> int:
+    return _raw_stream(_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
 # Steps of at least so many tokens, and so many a request, walk the pages that neighbouring tokens chose together
@@ -27,46 +63,69 @@ PORTION_TOKENS = 64
 PORTION_TOKENS_A_REQUEST = 4
 
 
-def _portions(q, out, cache, block_table, top: int, scale: float) -> int:
-    """Bytes of workspace of the kernel for portions where it takes this call, else 0: bfloat16 rows that TMA can address, a positive
-    scale, enough tokens."""
-    T, B = q.shape[0], block_table.shape[0]
-    if T < PORTION_TOKENS or T < PORTION_TOKENS_A_REQUEST * B or q.dtype != torch.bfloat16 or not scale > 0:
-        return 0
-    if q.stride(0) % 8 or out.stride(0) % 8 or (q.data_ptr() | out.data_ptr() | cache.data_ptr()) % 16 or cache.numel() // cache.shape[-1] > 0x7fffffff:
+def _portions(head) -> int:
+    """Bytes of workspace of the kernel for portions where it takes this call, else 0: rows that TMA can address, a positive scale."""
+    q, ldq, out, ldo, cache, num_pages, _, width, _, B, _, _, top, T, H, Hkv, D, page_size, scale = head
+    if not scale > 0 or ldq % 8 or ldo % 8 or (q | out | cache) % 16 or num_pages * 2 * Hkv * page_size > 0x7fffffff:
         return 0
     f = library("attention_pages_umma").dinfer_attention_pages_umma_workspace
     f.argtypes, f.restype = [c_int] * 8, c_int64
-    return f(B, block_table.shape[1], top, T, q.shape[1] // cache.shape[4], cache.shape[2], cache.shape[4], cache.shape[3])
+    return f(B, width, top, T, H, Hkv, D, page_size)
 
 
 def _here(what: str, *tensors) -> None:
     """On CUDA, all on the current device (the kernels run there, whatever the tensors say)."""
-    require_cuda(*tensors)
-    here = torch.cuda.current_device()
+    at = tensors[0].get_device()
     for t in tensors:
-        if t is not None and t.get_device() != here:
-            raise KernelError(f"{what}: a tensor on device {t.get_device()}, the current device is {here}")
+        if t is not None and t.get_device() != at:
+            require_cuda(*tensors)
+            raise KernelError(f"{what}: tensors on devices {at} and {t.get_device()}")
+    if at < 0 or at != _device():
+        require_cuda(*tensors)
+        raise KernelError(f"{what}: tensors on device {at}, the current device is {_device()}")
 
 
-def _ints(what: str, **tensors) -> None:
-    for name, t in tensors.items():
-        if t.dtype != torch.int32 or not t.is_contiguous():
-            raise KernelError(f"{what}: {name} must be contiguous int32")
+def _ints(what: str, names: str, *tensors) -> None:
+    for t in tensors:
+        if t.dtype != _I32 or not t.is_contiguous():
+            raise KernelError(f"{what}: {names} must be contiguous int32")
 
 
-def _batch(what: str, T: int, block_table, cu_seqlens, positions) -> None:
-    _ints(what, block_table=block_table, cu_seqlens=cu_seqlens, positions=positions)
-    if block_table.dim() != 2 or cu_seqlens.dim() != 1 or cu_seqlens.numel() != block_table.shape[0] + 1 or positions.numel() != T \
-            or block_table.shape[0] == 0:
+def _batch(what: str, T: int, block_table, cu_seqlens, positions):
+    """(requests, table width)"""
+    _ints(what, "block_table, cu_seqlens and positions", block_table, cu_seqlens, positions)
+    shape = block_table.shape
+    if len(shape) != 2 or cu_seqlens.dim() != 1 or cu_seqlens.numel() != shape[0] + 1 or positions.numel() != T or shape[0] == 0:
         raise KernelError(f"{what}: block_table [B, width] with B > 0, cu_seqlens [B + 1], positions [T]")
+    return shape
 
 
-def _heads(what: str, q, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
-    if q.dim() != 2 or q.stride(1) != 1 or q.shape[1] != num_heads * head_dim:
-        raise KernelError(f"{what}: rows [T, {num_heads} * {head_dim}] with a contiguous last axis, not {tuple(q.shape)}")
-    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or head_dim > 512:
+def _rows(what: str, name: str, t, width: int):
+    """(rows, row stride) of rows [T, width] with a contiguous last axis"""
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 2 or stride[1] != 1 or shape[1] != width:
+        raise KernelError(f"{what}: {name} rows [T, {width}] with a contiguous last axis, not {tuple(shape)}")
+    return shape[0], stride[0]
+
+
+def _heads(what: str, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
+    if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or not 0 < head_dim <= 512:
         raise KernelError(f"{what}: {num_heads} heads of {head_dim} over {num_kv_heads} key/value heads")
+
+
+def _paged(what: str, cache):
+    """(pages, 2, key/value heads, page size, head size) of a paged cache"""
+    shape = cache.shape
+    if len(shape) != 5 or shape[1] != 2 or shape[3] == 0 or not cache.is_contiguous():
+        raise KernelError(f"{what}: cache shape {tuple(shape)} is not [pages, 2, Hkv, page, D], contiguous")
+    return shape
+
+
+def _code(what: str, dtype) -> int:
+    code = DTYPE_CODE.get(dtype)
+    if code is None:
+        raise KernelError(f"{what}: dtype {dtype} is not one the kernels take (float32, bfloat16)")
+    return code
 
 
 def append(qkv: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_heads: int, head_dim: int, eps: float,
@@ -80,42 +139,38 @@ def append(qkv: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_he
     ``x / sqrt(mean(x^2) + eps) * w``, or None for both; ``cos_sin`` f32 [positions, rot]: the angle table (``cos | sin``) of the
     first ``rot`` elements, pairs (i, i + rot/2) or with ``interleaved`` (2i, 2i + 1), which reaches every position; None: no
     rotation.  A slot is written by one token of the step at most.  Returns ``q_out``."""
-    what = "page append"
+    what = "page_append"
     _here(what, qkv, positions, q_weight, k_weight, cos_sin, q_out, cache, slots, means)
+    _heads(what, num_heads, num_kv_heads, head_dim)
+    T, ld = _rows(what, "qkv", qkv, (num_heads + 2 * num_kv_heads) * head_dim)
+    rows, ldq = _rows(what, "q_out", q_out, num_heads * head_dim)
+    num_pages, _, Hkv, page_size, D = _paged(what, cache)
     dt = qkv.dtype
-    if qkv.dim() != 2 or qkv.stride(1) != 1 or qkv.shape[1] != (num_heads + 2 * num_kv_heads) * head_dim:
-        raise KernelError(f"{what}: qkv rows [T, ({num_heads} + 2 * {num_kv_heads}) * {head_dim}] with a contiguous last axis")
-    T = qkv.shape[0]
-    _heads(what, q_out, num_heads, num_kv_heads, head_dim)
-    if q_out.shape[0] != T or q_out.dtype != dt or cache.dtype != dt or means.dtype != dt:
-        raise KernelError(f"{what}: q_out, cache and means of the rows' dtype, q_out [T, H * D]")
-    if cache.dim() != 5 or tuple(cache.shape[1:3]) != (2, num_kv_heads) or cache.shape[4] != head_dim or cache.shape[3] == 0 \
-            or not cache.is_contiguous():
-        raise KernelError(f"{what}: cache shape {tuple(cache.shape)} is not [pages, 2, {num_kv_heads}, page, {head_dim}], contiguous")
-    if tuple(means.shape) != (cache.shape[0], num_kv_heads, head_dim) or not means.is_contiguous():
+    if rows != T or q_out.dtype != dt or cache.dtype != dt or means.dtype != dt or Hkv != num_kv_heads or D != head_dim:
+        raise KernelError(f"{what}: q_out [T, H * D], cache [pages, 2, {num_kv_heads}, page, {head_dim}] and means of the rows' dtype")
+    if means.shape != (num_pages, Hkv, D) or not means.is_contiguous():
         raise KernelError(f"{what}: means [pages, Hkv, D], contiguous, not {tuple(means.shape)}")
-    _ints(what, positions=positions, slots=slots)
+    _ints(what, "positions and slots", positions, slots)
     if positions.numel() != T or slots.numel() != T:
         raise KernelError(f"{what}: positions and slots int32 [T]")
-    if (q_weight is None) != (k_weight is None):
-        raise KernelError(f"{what}: q and k norm weights come together")
-    w_dt = dt
-    if q_weight is not None:
+    w_dt, qw, kw = dt, 0, 0
+    if q_weight is not None and k_weight is not None:
         w_dt = q_weight.dtype
-        if q_weight.numel() != head_dim or k_weight.numel() != head_dim or k_weight.dtype != w_dt \
-                or not q_weight.is_contiguous() or not k_weight.is_contiguous():
+        if q_weight.numel() != D or k_weight.numel() != D or k_weight.dtype != w_dt or not q_weight.is_contiguous() \
+                or not k_weight.is_contiguous():
             raise KernelError(f"{what}: norm weights [head_dim], contiguous, of one dtype")
-    rot = rows = 0
+        qw, kw = q_weight.data_ptr(), k_weight.data_ptr()
+    elif q_weight is not None or k_weight is not None:
+        raise KernelError(f"{what}: q and k norm weights come together")
+    rot = table_rows = angles = 0
     if cos_sin is not None:
-        if cos_sin.dtype != torch.float32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
+        if cos_sin.dtype != _F32 or cos_sin.dim() != 2 or not cos_sin.is_contiguous():
             raise KernelError(f"{what}: angle table must be contiguous float32 [positions, rot]")
-        rows, rot = cos_sin.shape
-    lib, f = _fn("page_append", "dinfer_page_append",
-                 [c_void_p, c_int64, c_void_p, c_void_p, c_void_p, c_float, c_void_p, c_int, c_int, c_int, c_void_p, c_int64,
-                  c_void_p, c_void_p, c_void_p, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p])
-    check(lib, f(ptr(qkv), qkv.stride(0), ptr(positions), ptr(q_weight), ptr(k_weight), eps, ptr(cos_sin), rows, rot,
-                 int(bool(interleaved)), ptr(q_out), q_out.stride(0), ptr(cache), ptr(means), ptr(slots), cache.shape[0],
-                 cache.shape[3], T, num_heads, num_kv_heads, head_dim, dtype_code(dt), dtype_code(w_dt), stream_handle()), what)
+        table_rows, rot = cos_sin.shape
+        angles = cos_sin.data_ptr()
+    _call("page_append", "dinfer_page_append", what, qkv.data_ptr(), ld, positions.data_ptr(), qw, kw, eps, angles, table_rows, rot,
+          1 if interleaved else 0, q_out.data_ptr(), ldq, cache.data_ptr(), means.data_ptr(), slots.data_ptr(), num_pages, page_size,
+          T, num_heads, Hkv, D, _code(what, dt), _code(what, w_dt))
     return q_out
 
 
@@ -128,26 +183,26 @@ def page_scores(q: torch.Tensor, means: torch.Tensor, block_table: torch.Tensor,
     is not a number makes the page's score one that is not.  Rows behind the last request's tokens are left as they are."""
     what = "page_scores"
     _here(what, q, means, block_table, cu_seqlens, positions, out)
-    if means.dim() != 3 or not means.is_contiguous() or means.dtype != q.dtype:
+    shape = means.shape
+    if len(shape) != 3 or not means.is_contiguous() or means.dtype != q.dtype:
         raise KernelError(f"{what}: means [pages, Hkv, D], contiguous, of q's dtype")
-    num_pages, Hkv, D = means.shape
-    _heads(what, q, num_heads, Hkv, D)
-    T = q.shape[0]
-    _batch(what, T, block_table, cu_seqlens, positions)
-    width = block_table.shape[1]
+    num_pages, Hkv, D = shape
+    _heads(what, num_heads, Hkv, D)
+    T, ldq = _rows(what, "q", q, num_heads * D)
+    B, width = _batch(what, T, block_table, cu_seqlens, positions)
     pages = width if pages is None else pages
     if not 0 <= pages <= width or page_size <= 0:
         raise KernelError(f"{what}: {pages} pages of {page_size} tokens, the table holds {width}")
     if out is None:
-        out = torch.empty((T, Hkv, pages), dtype=torch.float32, device=q.device)
-    elif out.dtype != torch.float32 or tuple(out.shape) != (T, Hkv, pages) or (pages > 1 and out.stride(2) != 1):
-        raise KernelError(f"{what}: out float32 [T, Hkv, pages] with a contiguous last axis")
-    lib, f = _fn("page_choice", "dinfer_page_scores",
-                 [c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p, c_int64, c_int64,
-                  c_int, c_int, c_int, c_int, c_int, c_int, c_int, c_void_p])
-    check(lib, f(ptr(q), q.stride(0), ptr(means), num_pages, ptr(block_table), width, ptr(cu_seqlens), block_table.shape[0],
-                 ptr(positions), ptr(out), out.stride(0), out.stride(1), T, num_heads, Hkv, D, page_size, pages,
-                 dtype_code(q.dtype), stream_handle()), what)
+        out = torch.empty((T, Hkv, pages), dtype=_F32, device=q.device)
+        ldt, ldg = Hkv * pages, pages
+    else:
+        if out.dtype != _F32 or out.shape != (T, Hkv, pages) or (pages > 1 and out.stride(2) != 1):
+            raise KernelError(f"{what}: out float32 [T, Hkv, pages] with a contiguous last axis")
+        ldt, ldg, _ = out.stride()
+    _call("page_choice", "dinfer_page_scores", what, q.data_ptr(), ldq, means.data_ptr(), num_pages, block_table.data_ptr(), width,
+          cu_seqlens.data_ptr(), B, positions.data_ptr(), out.data_ptr(), ldt, ldg, T, num_heads, Hkv, D, page_size, pages,
+          _code(what, q.dtype))
     return out
 
 
@@ -160,22 +215,21 @@ def choose_pages(scores: torch.Tensor, positions: torch.Tensor, page_size: int, 
     every number.  A negative position chooses no page."""
     what = "choose_pages"
     _here(what, scores, positions, out)
-    if scores.dim() != 3 or scores.dtype != torch.float32 or (scores.shape[2] > 1 and scores.stride(2) != 1) or scores.shape[2] == 0:
+    shape, stride = scores.shape, scores.stride()
+    if len(shape) != 3 or scores.dtype != _F32 or (shape[2] > 1 and stride[2] != 1) or shape[2] == 0:
         raise KernelError(f"{what}: scores float32 [T, Hkv, pages] with a contiguous last axis and at least one page")
-    T, Hkv, pages = scores.shape
-    _ints(what, positions=positions)
+    T, Hkv, pages = shape
+    _ints(what, "positions", positions)
     if positions.numel() != T:
         raise KernelError(f"{what}: positions int32 [T]")
     if page_size <= 0 or first < 0 or recent < 1 or top < first + recent:
         raise KernelError(f"{what}: {first} first and {recent} recent pages of {top}, pages of {page_size} tokens")
     if out is None:
-        out = torch.empty((T, Hkv, top), dtype=torch.int32, device=scores.device)
-    elif out.dtype != torch.int32 or tuple(out.shape) != (T, Hkv, top) or not out.is_contiguous():
+        out = torch.empty((T, Hkv, top), dtype=_I32, device=scores.device)
+    elif out.dtype != _I32 or out.shape != (T, Hkv, top) or not out.is_contiguous():
         raise KernelError(f"{what}: out int32 [T, Hkv, top], contiguous")
-    lib, f = _fn("page_choice", "dinfer_choose_pages",
-                 [c_void_p, c_int64, c_int64, c_void_p, c_int, c_int, c_int, c_int, c_int, c_void_p, c_int, c_int, c_void_p])
-    check(lib, f(ptr(scores), scores.stride(0), scores.stride(1), ptr(positions), page_size, first, recent, top, pages, ptr(out),
-                 T, Hkv, stream_handle()), what)
+    _call("page_choice", "dinfer_choose_pages", what, scores.data_ptr(), stride[0], stride[1], positions.data_ptr(), page_size, first,
+          recent, top, pages, out.data_ptr(), T, Hkv)
     return out
 
 
@@ -189,31 +243,34 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     the last request's tokens are left as they are.  Returns ``out``."""
     what = "attention_pages"
     _here(what, q, out, cache, block_table, cu_seqlens, positions, chosen)
-    if q.dtype not in DTYPE_CODE or out.dtype != q.dtype or cache.dtype != q.dtype:
-        raise KernelError(f"{what}: q, out and cache of one dtype, float32 or bfloat16")
-    if cache.dim() != 5 or cache.shape[1] != 2 or cache.shape[3] == 0 or not cache.is_contiguous():
-        raise KernelError(f"{what}: cache shape {tuple(cache.shape)} is not [pages, 2, Hkv, page, D], contiguous")
-    num_pages, _, Hkv, page_size, D = cache.shape
-    _heads(what, q, num_heads, Hkv, D)
-    _heads(what, out, num_heads, Hkv, D)
-    T = q.shape[0]
-    if out.shape[0] != T:
+    dt = q.dtype
+    if out.dtype != dt or cache.dtype != dt:
+        raise KernelError(f"{what}: q, out and cache of one dtype")
+    code = _code(what, dt)
+    num_pages, _, Hkv, page_size, D = _paged(what, cache)
+    _heads(what, num_heads, Hkv, D)
+    T, ldq = _rows(what, "q", q, num_heads * D)
+    rows, ldo = _rows(what, "out", out, num_heads * D)
+    if rows != T:
         raise KernelError(f"{what}: out [T, H * D] of q's shape")
-    _batch(what, T, block_table, cu_seqlens, positions)
-    _ints(what, chosen=chosen)
-    if chosen.dim() != 3 or tuple(chosen.shape[:2]) != (T, Hkv) or chosen.shape[2] == 0:
+    B, width = _batch(what, T, block_table, cu_seqlens, positions)
+    _ints(what, "chosen", chosen)
+    shape = chosen.shape
+    if len(shape) != 3 or shape[0] != T or shape[1] != Hkv or shape[2] == 0:
         raise KernelError(f"{what}: chosen int32 [T, Hkv, top] with top > 0")
-    top = chosen.shape[2]
-    head = (ptr(q), q.stride(0), ptr(out), out.stride(0), ptr(cache), num_pages, ptr(block_table), block_table.shape[1],
-            ptr(cu_seqlens), block_table.shape[0], ptr(positions), ptr(chosen), top, T, num_heads, Hkv, D, page_size, scale)
-    types = [c_void_p, c_int64, c_void_p, c_int64, c_void_p, c_int, c_void_p, c_int, c_void_p, c_int, c_void_p, c_void_p,
-             c_int, c_int, c_int, c_int, c_int, c_int, c_float]
-    size = _portions(q, out, cache, block_table, top, scale)
-    if size:
-        work = torch.empty(size, dtype=torch.uint8, device=q.device)
-        lib, f = _fn("attention_pages_umma", "dinfer_attention_pages_umma", types + [c_void_p, c_int64, c_void_p, c_void_p])
-        check(lib, f(*head, ptr(work), size, ptr(gemm_ops._state(q.device)["status"]), stream_handle()), "attention_pages_umma")
-        return out
-    lib, f = _fn("attention_pages", "dinfer_attention_pages", types + [c_int, c_int, c_void_p])
-    check(lib, f(*head, num_sms(), DTYPE_CODE[q.dtype], stream_handle()), what)
+    top = shape[2]
+    head = (q.data_ptr(), ldq, out.data_ptr(), ldo, cache.data_ptr(), num_pages, block_table.data_ptr(), width, cu_seqlens.data_ptr(), B,
+            positions.data_ptr(), chosen.data_ptr(), top, T, num_heads, Hkv, D, page_size, scale)
+    if T >= PORTION_TOKENS and T >= PORTION_TOKENS_A_REQUEST * B and dt == _BF16:
+        size = _portions(head)
+        if size:
+            work = torch.empty(size, dtype=torch.uint8, device=q.device)
+            _call("attention_pages_umma", "dinfer_attention_pages_umma", "attention_pages_umma", *head, work.data_ptr(), size,
+                  gemm_ops._state(q.device)["status"].data_ptr())
+            return out
+    at = _device()
+    sms = _SMS.get(at)
+    if sms is None:
+        sms = _SMS[at] = num_sms()
+    _call("attention_pages", "dinfer_attention_pages", what, *head, sms, code)
     return out

@@ -16,7 +16,8 @@ def no_device(monkeypatch):
 
     def library(*args):
         raise Launched
-    monkeypatch.setattr(page_ops, "_fn", library)
+    monkeypatch.setattr(page_ops, "_call", library)
+    monkeypatch.setattr(page_ops, "_device", lambda: 0)
 
 
 class Launched(Exception):

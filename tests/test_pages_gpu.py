@@ -378,18 +378,14 @@ def test_replayed_from_a_graph_on_another_stream(new):
             assert torch.equal(out, wanted)
 
 
-def test_another_device_is_refused():
+def test_another_device_is_refused(monkeypatch):
     """Tensors off the current device are refused by name, not read."""
     from dinfer_b200.kernels import page_ops
     from dinfer_b200.kernels.lib import KernelError
     x = torch.zeros(1, 1, 4, device="cuda")
-    real = torch.cuda.current_device
-    try:
-        torch.cuda.current_device = lambda: 1
-        with pytest.raises(KernelError, match="current device is 1"):
-            page_ops.choose_pages(x, torch.zeros(1, dtype=torch.int32, device="cuda"), 16, 4)
-    finally:
-        torch.cuda.current_device = real
+    monkeypatch.setattr(page_ops, "_device", lambda: 1)
+    with pytest.raises(KernelError, match="current device is 1"):
+        page_ops.choose_pages(x, torch.zeros(1, dtype=torch.int32, device="cuda"), 16, 4)
 
 
 def test_no_tokens():
