@@ -7,9 +7,13 @@
 // the best-scored, `top` in all; of equal scores the lower page, what is not a number behind every number.  Ascending, -1 behind
 // the last.
 #include "mma_tiles.cuh"
+#include "umma_attention.cuh"
 
 using namespace dinfer;
-using namespace dinfer_mma;
+using dinfer_mma::cp_async16;
+using dinfer_mma::cp_async_commit;
+using dinfer_mma::cp_async_wait;
+using dinfer_mma::mma_bf16;
 
 namespace {
 
@@ -174,6 +178,142 @@ page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const _
       }
     }
   }
+}
+
+// Bfloat16, head sizes 64 and 128, many tokens: 128 pages of a (request, key head) are the rows of a tcgen05.mma, up to 256 (token, head)
+// pairs its columns (the group filled up to a power of two, GP, with its last head), D its depth; S comes out in tensor memory with a page
+// to a lane, so that a thread takes the maximum over a token's heads among its own registers and a warp writes 32 pages of a
+// token side by side.  A block keeps its pages and walks runs of tokens; two blocks share an SM, so that one loads while
+// the other multiplies or writes.  The wait for the products is bounded.
+// Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2.  @SCORES@
+constexpr int U_ROWS = 128, U_COLS = 256, U_NT = 256;
+// from so many tokens on, and so many a request
+constexpr int MANY_TOKENS = 64, MANY_TOKENS_A_REQUEST = 16;
+
+template <int D, int GP>
+__global__ void __launch_bounds__(U_NT, 2)
+page_scores_umma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const __nv_bfloat16* __restrict__ means, int num_pages,
+                        const int* __restrict__ table, int width, const int* __restrict__ cu, int num_reqs,
+                        const int* __restrict__ positions, float* __restrict__ out, int64_t ldt, int64_t ldg, int group, int Hkv,
+                        int page_size, int pages, int tiles, int per_block, int* status) {
+  using namespace dinfer_umma;
+  constexpr int TOKENS = U_COLS / GP, NH = D / 64, C = D / 8;
+  constexpr uint32_t A_HALF = U_ROWS * 128, B_HALF = U_COLS * 128;
+  extern __shared__ unsigned char smem_dyn[];
+  __shared__ __align__(8) uint64_t s_done;
+  __shared__ uint32_t s_tmem_base;
+  __shared__ int s_full[TOKENS];
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y, j0 = blockIdx.z * U_ROWS;
+  const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  unsigned char* sA = smem_dyn + (base - smem_u32(smem_dyn));      // [NH][128 pages][128 B], TMA's 128-byte swizzle
+  unsigned char* sB = sA + NH * A_HALF;                            // [NH][256 columns][128 B]
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&s_done), 1);
+    asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+  }
+  if (warp == 0) {
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(U_COLS) : "memory");
+    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = s_tmem_base;
+  // this thread's page: lane quarter warp % 4 of tensor memory, half of the columns warp / 4
+  const int j = j0 + (warp & 3) * 32 + lane;
+  bool held = false;
+  int request = -1, turn = 0;
+  for (int y = blockIdx.x * per_block; y < min(tiles, (int)(blockIdx.x + 1) * per_block); ++y) {
+    const int3 tile = token_tile(cu, num_reqs, TOKENS, y);
+    if (tile.x < 0) break;                                         // (the whole block alike)
+    if (tile.x != request) {                                       // the pages of another request
+      request = tile.x;
+      const int* row_table = table + (int64_t)request * width;
+      for (int i = threadIdx.x; i < U_ROWS * C; i += U_NT) {
+        const int row = i / C, c = i % C;
+        const int page = j0 + row < pages ? row_table[j0 + row] : -1;
+        const bool ok = page >= 0 && page < num_pages;
+        cp_async16(sA + (c >> 3) * A_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4), means + ((int64_t)(ok ? page : 0) * Hkv + g) * D + c * 8, ok);
+      }
+      const int page = j < pages ? row_table[j] : -1;
+      held = page >= 0 && page < num_pages;
+    }
+    for (int i = threadIdx.x; i < U_COLS * C; i += U_NT) {
+      const int col = i / C, c = i % C, at = col / GP, h = min(col % GP, group - 1);
+      const bool ok = at < tile.z;
+      cp_async16(sB + (c >> 3) * B_HALF + col * 128 + (((c & 7) ^ (col & 7)) << 4),
+                 q + (ok ? (int64_t)(tile.y + at) * ldq + (int64_t)(g * group + h) * D + c * 8 : 0), ok);
+    }
+    cp_async_commit();
+    for (int i = threadIdx.x; i < TOKENS; i += U_NT) s_full[i] = i < tile.z ? positions[tile.y + i] / page_size : 0;
+    cp_async_wait<0>();
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+      tc_fence_after();
+      constexpr uint32_t idesc = idesc_bf16(U_ROWS, U_COLS, 0);
+      const uint64_t da = desc_k_major(smem_u32(sA)), db = desc_k_major(smem_u32(sB));
+#pragma unroll
+      for (int k = 0; k < D / 16; ++k)
+        tc_mma(tmem, da + (uint64_t)(((k / 4) * A_HALF + (k % 4) * 32) >> 4), db + (uint64_t)(((k / 4) * B_HALF + (k % 4) * 32) >> 4),
+               idesc, k > 0 ? 1u : 0u);
+      tc_commit(smem_u32(&s_done));
+    }
+    const bool ok = mbar_wait(smem_u32(&s_done), turn & 1);
+    ++turn;
+    if (__syncthreads_or(!ok)) {                                   // nobody reads what has not come
+      if (threadIdx.x == 0) atomicExch(status, 67);
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
+      break;
+    }
+    tc_fence_after();
+    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
+    float* row = out + (int64_t)tile.y * ldt + (int64_t)g * ldg + j;
+#pragma unroll 1
+    for (int c0 = (warp >> 2) * (U_COLS / 2); c0 < ((warp >> 2) + 1) * (U_COLS / 2); c0 += 32) {
+      if (c0 / GP >= tile.z) break;                                // (a warp alike)
+      float v[32];
+      tmem_ld32(lane_addr + c0, v);
+      tmem_ld_wait();
+#pragma unroll
+      for (int i = 0; i < 32 / GP; ++i) {
+        float x = v[i * GP];
+#pragma unroll
+        for (int h = 1; h < GP; ++h) x = max_nan(x, v[i * GP + h]);
+        const int at = c0 / GP + i;
+        if (at < tile.z && j < pages) row[(int64_t)at * ldt] = held && j < s_full[at] ? x : -INFINITY;
+      }
+    }
+    tc_fence_before();
+    __syncthreads();                                               // tensor and shared memory are free again
+  }
+  if (warp == 0) {
+    tc_fence_after();
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(U_COLS) : "memory");
+  }
+}
+
+template <int D, int GP>
+int run_scores_umma(const __nv_bfloat16* q, int64_t ldq, const __nv_bfloat16* means, int num_pages, const int* table, int width, const int* cu,
+                    int num_reqs, const int* positions, float* out, int64_t ldt, int64_t ldg, int T, int group, int Hkv, int page_size,
+                    int pages, int sms, int* status, cudaStream_t stream) {
+  auto kernel = page_scores_umma_kernel<D, GP>;
+  constexpr int smem = (D / 64) * (U_ROWS + U_COLS) * 128 + 1024, tokens = U_COLS / GP;
+  static thread_local int set_for = -1;                            // the attribute belongs to the device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (set_for != dev) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, smem) != cudaSuccess)
+      return cuda_status("page_scores: shared memory");
+    set_for = dev;
+  }
+  const int tiles = T / tokens + (num_reqs < T ? num_reqs : T), z = (pages + U_ROWS - 1) / U_ROWS;
+  // a block's pages are loaded once for all its runs of tokens: as few blocks as fill the SMs twice over
+  const int blocks = 2 * sms / (Hkv * z) < 1 ? 1 : 2 * sms / (Hkv * z), per_block = (tiles + blocks - 1) / blocks;
+  launch_pdl(kernel, dim3((tiles + per_block - 1) / per_block, Hkv, z), dim3(U_NT), smem, stream, q, ldq, means, num_pages, table, width, cu,
+             num_reqs, positions, out, ldt, ldg, group, Hkv, page_size, pages, tiles, per_block, status);
+  return cuda_status("page_scores (many tokens)");
 }
 
 // Scores as whole numbers of the same order; 0 for what is not a number, 1 for -inf.
@@ -440,7 +580,8 @@ struct PageScoresArgs {
   int64_t num_reqs;
   const int* positions;
   float* out;
-  int64_t ldt, ldg, T, H, Hkv, D, page_size, pages, dtype;
+  int64_t ldt, ldg, T, H, Hkv, D, page_size, pages, dtype, sms;
+  int* status;                   // of the kernels with bounded waits
   cudaStream_t stream;
 };
 
@@ -462,6 +603,22 @@ DINFER_API int dinfer_page_scores(const PageScoresArgs* a) {
   const int group = H / Hkv;
   const int64_t z = (pages + WARPS * 32 - 1) / (WARPS * 32);
   if (dtype == DINFER_BF16 && (D == 64 || D == 128) && group <= 16 && ldq % 8 == 0 && ((uintptr_t)q | (uintptr_t)means) % 16 == 0 && z <= 65535) {
+    // (measured: see MANY_TOKENS)
+    if (a->status && T >= MANY_TOKENS && T >= MANY_TOKENS_A_REQUEST * (int64_t)num_reqs) {
+      const __nv_bfloat16 *qb = (const __nv_bfloat16*)q, *mb = (const __nv_bfloat16*)means;
+      const int sms = (int)a->sms;
+#define DINFER_SCORES(GP)                                                                                                              \
+  return D == 64 ? run_scores_umma<64, GP>(qb, ldq, mb, num_pages, table, width, cu_seqlens, num_reqs, positions, out, ldt, ldg, T, group, \
+                                           Hkv, page_size, pages, sms, a->status, stream)                                              \
+                 : run_scores_umma<128, GP>(qb, ldq, mb, num_pages, table, width, cu_seqlens, num_reqs, positions, out, ldt, ldg, T, group, \
+                                            Hkv, page_size, pages, sms, a->status, stream)
+      if (group == 1) DINFER_SCORES(1);
+      if (group == 2) DINFER_SCORES(2);
+      if (group <= 4) DINFER_SCORES(4);
+      if (group <= 8) DINFER_SCORES(8);
+      DINFER_SCORES(16);
+#undef DINFER_SCORES
+    }
     const int64_t tiles = (int64_t)T / TILE_TOKENS + (num_reqs < T ? num_reqs : T);     // of every way the tokens may be dealt out
     const dim3 grid((unsigned)tiles, Hkv, (unsigned)z);
 #define DINFER_SCORES(GP)                                                                                                       \

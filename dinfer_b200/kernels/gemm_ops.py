@@ -72,6 +72,7 @@ STATUS_MEANING = {
     64: "attention over chosen pages: an MMA thread waited for the softmax warps' P tile",
     65: "attention over chosen pages: the softmax warps waited for a score tile or for P V to finish",
     66: "attention over chosen pages: the softmax warps waited for the last P V before writing the output",
+    67: "page scores: the threads waited for the products",
     53: "state-space chunks: the step has more portions than its launch was made for",
 }
 

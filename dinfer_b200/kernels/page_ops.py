@@ -28,7 +28,7 @@ _I32, _F32, _BF16 = torch.int32, torch.float32, torch.bfloat16
 # by one cost ctypes 2.8 us, packed 0.5), the stream last, and the checks ask each tensor once for each thing.
 _PACK = {
     "dinfer_page_append": struct.Struct("5qd18q").pack,
-    "dinfer_page_scores": struct.Struct("20q").pack,
+    "dinfer_page_scores": struct.Struct("22q").pack,
     "dinfer_choose_pages": struct.Struct("13q").pack,
     "dinfer_attention_pages": struct.Struct("18qd3q").pack,
     "dinfer_attention_pages_umma": struct.Struct("18qd4q").pack,
@@ -52,6 +52,14 @@ _raw_stream = getattr(torch._C, "_cuda_getCurrentRawStream", None)
 
 def _device() -> int:
     return _raw_device() if _raw_device is not None else torch.cuda.current_device()
+
+
+def _multiprocessors() -> int:
+    at = _device()
+    n = _SMS.get(at)
+    if n is None:
+        n = _SMS[at] = num_sms()
+    return n
 
 
 def _stream() -> int:
@@ -202,7 +210,7 @@ def page_scores(q: torch.Tensor, means: torch.Tensor, block_table: torch.Tensor,
         ldt, ldg, _ = out.stride()
     _call("page_choice", "dinfer_page_scores", what, q.data_ptr(), ldq, means.data_ptr(), num_pages, block_table.data_ptr(), width,
           cu_seqlens.data_ptr(), B, positions.data_ptr(), out.data_ptr(), ldt, ldg, T, num_heads, Hkv, D, page_size, pages,
-          _code(what, q.dtype))
+          _code(what, q.dtype), _multiprocessors(), gemm_ops._state(q.device)["status"].data_ptr())
     return out
 
 
@@ -268,9 +276,5 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
             _call("attention_pages_umma", "dinfer_attention_pages_umma", "attention_pages_umma", *head, work.data_ptr(), size,
                   gemm_ops._state(q.device)["status"].data_ptr())
             return out
-    at = _device()
-    sms = _SMS.get(at)
-    if sms is None:
-        sms = _SMS[at] = num_sms()
-    _call("attention_pages", "dinfer_attention_pages", what, *head, sms, code)
+    _call("attention_pages", "dinfer_attention_pages", what, *head, _multiprocessors(), code)
     return out

@@ -18,6 +18,7 @@ def no_device(monkeypatch):
         raise Launched
     monkeypatch.setattr(page_ops, "_call", library)
     monkeypatch.setattr(page_ops, "_device", lambda: 0)
+    monkeypatch.setattr(page_ops.gemm_ops, "_state", lambda device: {"status": torch.zeros(1, dtype=I32)})
 
 
 class Launched(Exception):

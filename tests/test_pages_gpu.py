@@ -122,7 +122,9 @@ def test_means_do_not_depend_on_the_portions(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("size", SIZES + [([(1700, 40), (33, 1), (0, 90), (640, 3)], 16, 8, 2, 128), ([(900, 1)] * 9, 16, 4, 2, 64)], ids=str)
+@pytest.mark.parametrize("size", SIZES + [([(1700, 40), (33, 1), (0, 90), (640, 3)], 16, 8, 2, 128), ([(900, 1)] * 9, 16, 4, 2, 64),
+                                          ([(2500, 150), (0, 40), (4100, 300)], 16, 8, 2, 128), ([(300, 90)], 16, 5, 5, 64), ([(700, 200)], 32, 10, 2, 64),
+                                          ([(600, 70)], 16, 12, 4, 128), ([(520, 66)], 16, 32, 2, 64), ([(0, 64), (64, 64)], 64, 16, 2, 64)], ids=str)
 def test_scores(size, dtype):
     from dinfer_b200.kernels import page_ops
     requests, P, H, G, D = size
@@ -146,7 +148,7 @@ def test_scores(size, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-@pytest.mark.parametrize("new", [1, 40])
+@pytest.mark.parametrize("new", [1, 40, 100])
 def test_scores_of_what_is_no_number(new, dtype):
     """A NaN or infinity in one query or one mean stays with its own scores; in a page not scored it changes nothing."""
     from dinfer_b200.kernels import page_ops
@@ -157,7 +159,7 @@ def test_scores_of_what_is_no_number(new, dtype):
     clean = page_ops.page_scores(c(q), c(means), c(b.table), c(b.cu), c(b.positions), H, P).cpu()
     q[b.T - 1, 3] = math.nan                                 # a head of key head 0
     means[int(b.table[0, 7]), 1, 9] = math.inf
-    means[int(b.table[0, 41 if new > 16 else 40]), 0, 0] = math.nan
+    means[int(b.table[0, (40 * P + new - 1) // P]), 0, 0] = math.nan
     got = page_ops.page_scores(c(q), c(means), c(b.table), c(b.cu), c(b.positions), H, P).cpu()
     want = plain_scores(q, means, b, H, b.width)[0]
     assert torch.equal(torch.isnan(got), torch.isnan(want))
