@@ -180,13 +180,13 @@ page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const _
   }
 }
 
-// Bfloat16, head sizes 64 and 128, many tokens: 128 pages of a (request, key head) are the rows of a tcgen05.mma, up to 256 (token, head)
+// Bfloat16, head sizes 64 and 128, many tokens: 128 pages of a (request, key head) are the rows of a tcgen05.mma, up to 128 (token, head)
 // pairs its columns (the group filled up to a power of two, GP, with its last head), D its depth; S comes out in tensor memory with a page
 // to a lane, so that a thread takes the maximum over a token's heads among its own registers and a warp writes 32 pages of a
-// token side by side.  A block keeps its pages and walks runs of tokens; two blocks share an SM, so that one loads while
-// the other multiplies or writes.  The wait for the products is bounded.
-// Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2.  @SCORES@
-constexpr int U_ROWS = 128, U_COLS = 256, U_NT = 256;
+// token side by side.  A block keeps its pages and walks runs of tokens: while the products of a run are made, the next run's rows
+// of q are on their way and the results of the run before are written.  Two blocks share an SM.  The waits for the products are
+// bounded.  Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2.  @SCORES@
+constexpr int U_ROWS = 128, U_COLS = 128, U_NT = 256;
 // from so many tokens on, and so many a request
 constexpr int MANY_TOKENS = 64, MANY_TOKENS_A_REQUEST = 16;
 
@@ -200,20 +200,27 @@ page_scores_umma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const 
   constexpr int TOKENS = U_COLS / GP, NH = D / 64, C = D / 8;
   constexpr uint32_t A_HALF = U_ROWS * 128, B_HALF = U_COLS * 128;
   extern __shared__ unsigned char smem_dyn[];
-  __shared__ __align__(8) uint64_t s_done;
+  __shared__ __align__(8) uint64_t s_done[2];
   __shared__ uint32_t s_tmem_base;
-  __shared__ int s_full[TOKENS];
+  __shared__ int s_full[3][TOKENS];                                // of the run before, this one and the next
+  __shared__ volatile int s_abort;
   pdl_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y, j0 = blockIdx.z * U_ROWS;
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   unsigned char* sA = smem_dyn + (base - smem_u32(smem_dyn));      // [NH][128 pages][128 B], TMA's 128-byte swizzle
-  unsigned char* sB = sA + NH * A_HALF;                            // [NH][256 columns][128 B]
+  unsigned char* sB = sA + NH * A_HALF;                            // [2][NH][128 columns][128 B]
+  int y = blockIdx.x * per_block;
+  const int end = min(tiles, y + per_block);
+  int3 tile = y < end ? token_tile(cu, num_reqs, TOKENS, y) : make_int3(-1, 0, 0);
+  if (tile.x < 0) return;                                          // (the whole block alike)
   if (threadIdx.x == 0) {
-    mbar_init(smem_u32(&s_done), 1);
+    mbar_init(smem_u32(&s_done[0]), 1);
+    mbar_init(smem_u32(&s_done[1]), 1);
+    s_abort = 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
   }
   if (warp == 0) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(U_COLS) : "memory");
+    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(2 * U_COLS) : "memory");
     asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
   }
   tc_fence_before();
@@ -223,74 +230,111 @@ page_scores_umma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const 
   // this thread's page: lane quarter warp % 4 of tensor memory, half of the columns warp / 4
   const int j = j0 + (warp & 3) * 32 + lane;
   bool held = false;
-  int request = -1, turn = 0;
-  for (int y = blockIdx.x * per_block; y < min(tiles, (int)(blockIdx.x + 1) * per_block); ++y) {
-    const int3 tile = token_tile(cu, num_reqs, TOKENS, y);
-    if (tile.x < 0) break;                                         // (the whole block alike)
-    if (tile.x != request) {                                       // the pages of another request
-      request = tile.x;
-      const int* row_table = table + (int64_t)request * width;
-      for (int i = threadIdx.x; i < U_ROWS * C; i += U_NT) {
-        const int row = i / C, c = i % C;
-        const int page = j0 + row < pages ? row_table[j0 + row] : -1;
-        const bool ok = page >= 0 && page < num_pages;
-        cp_async16(sA + (c >> 3) * A_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4), means + ((int64_t)(ok ? page : 0) * Hkv + g) * D + c * 8, ok);
-      }
-      const int page = j < pages ? row_table[j] : -1;
-      held = page >= 0 && page < num_pages;
+  auto load_pages = [&](int request) {
+    const int* row_table = table + (int64_t)request * width;
+    for (int i = threadIdx.x; i < U_ROWS * C; i += U_NT) {
+      const int row = i / C, c = i % C;
+      const int page = j0 + row < pages ? row_table[j0 + row] : -1;
+      const bool ok = page >= 0 && page < num_pages;
+      cp_async16(sA + (c >> 3) * A_HALF + row * 128 + (((c & 7) ^ (row & 7)) << 4), means + ((int64_t)(ok ? page : 0) * Hkv + g) * D + c * 8, ok);
     }
-    for (int i = threadIdx.x; i < U_COLS * C; i += U_NT) {
-      const int col = i / C, c = i % C, at = col / GP, h = min(col % GP, group - 1);
-      const bool ok = at < tile.z;
-      cp_async16(sB + (c >> 3) * B_HALF + col * 128 + (((c & 7) ^ (col & 7)) << 4),
-                 q + (ok ? (int64_t)(tile.y + at) * ldq + (int64_t)(g * group + h) * D + c * 8 : 0), ok);
+    const int page = j < pages ? row_table[j] : -1;
+    held = page >= 0 && page < num_pages;
+  };
+  // this thread's copies of a run: the same 16 bytes of the same head of every STEP-th token (so many columns further on the swizzle is the same)
+  constexpr int COLS = U_NT / C, STEP = COLS / GP;
+  static_assert(COLS % 8 == 0 && COLS % GP == 0, "a thread's columns have one head and one swizzle");
+  const int col0 = threadIdx.x / C, c0 = threadIdx.x % C;
+  const uint32_t dst0 = (c0 >> 3) * B_HALF + col0 * 128 + (((c0 & 7) ^ (col0 & 7)) << 4);
+  const __nv_bfloat16* src0 = q + (int64_t)(g * group + min(col0 % GP, group - 1)) * D + c0 * 8;
+  auto load_tokens = [&](const int3& run, int b, int i0) {           // run number i0
+    unsigned char* dst = sB + b * NH * B_HALF + dst0;
+    const __nv_bfloat16* src = src0 + (int64_t)(run.y + col0 / GP) * ldq;
+#pragma unroll
+    for (int k = 0; k < U_COLS / COLS; ++k) {
+      const bool ok = col0 / GP + k * STEP < run.z;
+      cp_async16(dst + k * COLS * 128, ok ? src : q, ok);
+      src += (int64_t)STEP * ldq;
     }
     cp_async_commit();
-    for (int i = threadIdx.x; i < TOKENS; i += U_NT) s_full[i] = i < tile.z ? positions[tile.y + i] / page_size : 0;
+    if (threadIdx.x < TOKENS) s_full[i0 % 3][threadIdx.x] = threadIdx.x < run.z ? positions[run.y + threadIdx.x] / page_size : 0;
+  };
+  auto write = [&](const int3& run, int i) {                        // the results of products i
+    const int b = i & 1;
+    if (!mbar_wait(smem_u32(&s_done[b]), (i >> 1) & 1)) { s_abort = 1; atomicExch(status, 67); return; }
+    tc_fence_after();
+    const uint32_t addr = tmem + ((uint32_t)((warp & 3) * 32) << 16) + b * U_COLS;
+    constexpr int PER = 32 / GP;                                    // tokens of 32 columns
+    const int* full = s_full[i % 3];
+    const int mine = held ? j : 0x7fffffff;
+#pragma unroll
+    for (int u = 0; u < U_COLS / 64; ++u) {
+      const int col = (warp >> 2) * (U_COLS / 2) + u * 32, first = col / GP;
+      if (first >= run.z) break;                                    // (a warp alike)
+      float v[32];
+      tmem_ld32(addr + col, v);
+      tmem_ld_wait();
+      float* row = out + (int64_t)(run.y + first) * ldt + (int64_t)g * ldg + j;
+      const int n = j < pages ? run.z - first : 0;
+#pragma unroll
+      for (int k = 0; k < PER; ++k) {
+        float x = v[k * GP];
+#pragma unroll
+        for (int h = 1; h < GP; ++h) x = max_nan(x, v[k * GP + h]);
+        if (k < n) *row = mine < full[first + k] ? x : -INFINITY;
+        row += ldt;
+      }
+    }
+  };
+  int ends = cu[tile.x + 1];                                       // of the request
+  load_pages(tile.x);
+  load_tokens(tile, 0, 0);
+  int3 before = make_int3(-1, 0, 0);                                // the run whose results are to be written
+  for (int i = 0;; ++i) {
+    const int b = i & 1;
     cp_async_wait<0>();
     asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-    __syncthreads();
+    tc_fence_before();
+    __syncthreads();                                               // the run is here; tensor memory b has been read
+    if (s_abort) break;
     if (threadIdx.x == 0) {
       tc_fence_after();
       constexpr uint32_t idesc = idesc_bf16(U_ROWS, U_COLS, 0);
-      const uint64_t da = desc_k_major(smem_u32(sA)), db = desc_k_major(smem_u32(sB));
+      const uint64_t da = desc_k_major(smem_u32(sA)), db = desc_k_major(smem_u32(sB) + b * NH * B_HALF);
 #pragma unroll
       for (int k = 0; k < D / 16; ++k)
-        tc_mma(tmem, da + (uint64_t)(((k / 4) * A_HALF + (k % 4) * 32) >> 4), db + (uint64_t)(((k / 4) * B_HALF + (k % 4) * 32) >> 4),
-               idesc, k > 0 ? 1u : 0u);
-      tc_commit(smem_u32(&s_done));
+        tc_mma(tmem + b * U_COLS, da + (uint64_t)(((k / 4) * A_HALF + (k % 4) * 32) >> 4),
+               db + (uint64_t)(((k / 4) * B_HALF + (k % 4) * 32) >> 4), idesc, k > 0 ? 1u : 0u);
+      tc_commit(smem_u32(&s_done[b]));
     }
-    const bool ok = mbar_wait(smem_u32(&s_done), turn & 1);
-    ++turn;
-    if (__syncthreads_or(!ok)) {                                   // nobody reads what has not come
-      if (threadIdx.x == 0) atomicExch(status, 67);
-      for (int i = 0; i < 64; ++i) __nanosleep(1000);
-      break;
+    ++y;
+    const bool same = y < end && tile.y + TOKENS < ends;
+    int3 next = make_int3(tile.x, tile.y + TOKENS, min(TOKENS, ends - tile.y - TOKENS));
+    if (!same) next = y < end ? token_tile(cu, num_reqs, TOKENS, y) : make_int3(-1, 0, 0);
+    // the other buffer is free once the products before have been made
+    if (before.x >= 0 && !mbar_wait(smem_u32(&s_done[b ^ 1]), ((i - 1) >> 1) & 1)) { s_abort = 1; atomicExch(status, 67); }
+    if (same) load_tokens(next, b ^ 1, i + 1);
+    if (before.x >= 0) write(before, i - 1);
+    if (!same) {
+      write(tile, i);
+      if (next.x < 0) break;
+      __syncthreads();                                             // (everyone has written: the lists of full pages are free)
+      load_pages(next.x);
+      load_tokens(next, b ^ 1, i + 1);
+      ends = cu[next.x + 1];
+      before.x = -1;
+    } else {
+      before = tile;
     }
-    tc_fence_after();
-    const uint32_t lane_addr = tmem + ((uint32_t)((warp & 3) * 32) << 16);
-    float* row = out + (int64_t)tile.y * ldt + (int64_t)g * ldg + j;
-#pragma unroll 1
-    for (int c0 = (warp >> 2) * (U_COLS / 2); c0 < ((warp >> 2) + 1) * (U_COLS / 2); c0 += 32) {
-      if (c0 / GP >= tile.z) break;                                // (a warp alike)
-      float v[32];
-      tmem_ld32(lane_addr + c0, v);
-      tmem_ld_wait();
-#pragma unroll
-      for (int i = 0; i < 32 / GP; ++i) {
-        float x = v[i * GP];
-#pragma unroll
-        for (int h = 1; h < GP; ++h) x = max_nan(x, v[i * GP + h]);
-        const int at = c0 / GP + i;
-        if (at < tile.z && j < pages) row[(int64_t)at * ldt] = held && j < s_full[at] ? x : -INFINITY;
-      }
-    }
-    tc_fence_before();
-    __syncthreads();                                               // tensor and shared memory are free again
+    tile = next;
   }
+  tc_fence_before();
+  __syncthreads();
   if (warp == 0) {
+    if (s_abort)
+      for (int i = 0; i < 64; ++i) __nanosleep(1000);
     tc_fence_after();
-    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(U_COLS) : "memory");
+    asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(2 * U_COLS) : "memory");
   }
 }
 
@@ -299,7 +343,7 @@ int run_scores_umma(const __nv_bfloat16* q, int64_t ldq, const __nv_bfloat16* me
                     int num_reqs, const int* positions, float* out, int64_t ldt, int64_t ldg, int T, int group, int Hkv, int page_size,
                     int pages, int sms, int* status, cudaStream_t stream) {
   auto kernel = page_scores_umma_kernel<D, GP>;
-  constexpr int smem = (D / 64) * (U_ROWS + U_COLS) * 128 + 1024, tokens = U_COLS / GP;
+  constexpr int smem = (D / 64) * (U_ROWS + 2 * U_COLS) * 128 + 1024, tokens = U_COLS / GP;
   static thread_local int set_for = -1;                            // the attribute belongs to the device
   int dev = 0;
   cudaGetDevice(&dev);
