@@ -9,22 +9,12 @@
 #include <cooperative_groups.h>
 
 #include "mma_tiles.cuh"
+#include "page_batch.cuh"
 
 using namespace dinfer;
 using namespace dinfer_mma;
 
 namespace {
-
-// The request of token t: the first whose tokens end behind it (every lane of a full warp asks; requests without tokens are passed
-// over), -1 where there is none.
-__device__ __forceinline__ int request_of(const int* cu, int num_reqs, int t) {
-  int ended = 0;
-  for (int i0 = 0; i0 < num_reqs; i0 += 32) {
-    const int i = i0 + (threadIdx.x & 31);
-    ended += __popc(__ballot_sync(0xffffffffu, i < num_reqs && cu[i + 1] <= t));
-  }
-  return ended < num_reqs && t >= cu[0] ? ended : -1;
-}
 
 struct Pages {
   int64_t ldq, ldo;
@@ -121,6 +111,203 @@ int run(const void* q, void* out, const void* cache, const Pages& p, cudaStream_
   return cuda_status("attention_pages");
 }
 
+
+// ------------------------------------------------------------------------------------------------
+// 32-bit, head sizes 64 and 128, groups of up to 8 heads: several tokens a request.  Eight neighbouring tokens share a block and walk
+// the pages that any of them chose in ascending order (their choices, sorted in shared memory), each page read once for all; a warp owns a
+// token and passes over the pages it did not choose.  Tiles of up to 32 keys ride two cp.async stages.  A score is a lane's own sum over
+// its key's row; for O the lanes split the elements and the keys that the token sees come one by one.  All of it multiply-adds in 32
+// bits.  Bound by shared memory's reads (a key's row once for the group's scores, a value's once for its sums).
+// @FLOAT@
+constexpr int F_TOKENS = 8, F_NT = F_TOKENS * 32, F_KEYS = 32, F_PICKS = 1024;
+
+template <int D, int G>              // G: at least the group
+__global__ void __launch_bounds__(F_NT)
+pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const float* __restrict__ cache, const Pages p) {
+  extern __shared__ __align__(16) unsigned char smem_raw[];
+  float* sK = reinterpret_cast<float*>(smem_raw);          // [2][F_KEYS][D], 16-byte pieces exchanged by key & 7: eight rows' in different banks
+  float* sV = sK + 2 * F_KEYS * D;                         // [2][F_KEYS][D]
+  float* sQ = sV + 2 * F_KEYS * D;                         // [F_TOKENS][group][D]
+  // (page, token), sorted; all ones: none
+  unsigned long long* s_pick = reinterpret_cast<unsigned long long*>(sQ + F_TOKENS * (p.H / p.Hkv) * D);
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y;
+  const int3 tile = token_tile(p.cu, p.num_reqs, F_TOKENS, blockIdx.x);
+  if (tile.x < 0) return;
+  const int* table = p.table + (int64_t)tile.x * p.width;
+  const int group = p.H / p.Hkv, P = p.page_size, picks = F_TOKENS * p.top;
+  int n2 = 1;                                              // what is sorted: a power of two
+  while (n2 < picks) n2 <<= 1;
+  for (int i = threadIdx.x; i < n2; i += F_NT) {
+    const int tl = i / p.top, t = tile.y + tl;
+    unsigned long long key = ~0ull;
+    if (i < picks && tl < tile.z) {
+      const int j = p.chosen[((int64_t)t * p.Hkv + g) * p.top + i - tl * p.top];
+      if (j >= 0 && j < p.width && (int64_t)j * P <= p.positions[t]) key = (unsigned long long)j << 8 | tl;
+    }
+    s_pick[i] = key;
+  }
+  for (int i = threadIdx.x; i < tile.z * group * (D / 4); i += F_NT) {
+    const int row = i / (D / 4), e = i % (D / 4) * 4;      // (token, head)
+    *reinterpret_cast<float4*>(sQ + row * D + e) =
+        *reinterpret_cast<const float4*>(q + (int64_t)(tile.y + row / group) * p.ldq + (int64_t)(g * group + row % group) * D + e);
+  }
+  __syncthreads();
+  for (int k = 2; k <= n2; k <<= 1)                        // a bitonic sort
+    for (int m = k >> 1; m > 0; m >>= 1) {
+      for (int i = threadIdx.x; i < n2; i += F_NT) {
+        const int o = i ^ m;
+        if (o > i) {
+          const unsigned long long a = s_pick[i], b = s_pick[o];
+          if ((a > b) == !(i & k)) { s_pick[i] = b; s_pick[o] = a; }
+        }
+      }
+      __syncthreads();
+    }
+  // A visit is a page with the tokens that chose it (a token that names a page twice gets a second visit).  `at` runs over the picks.
+  const int KT = P < F_KEYS ? P : F_KEYS, per_page = P / KT;
+  const int64_t plane = (int64_t)p.Hkv * P * D;
+  auto visit = [&](int& at, unsigned& tokens) {            // the next one's page in the table, or -1
+    while (at < n2 && s_pick[at] != ~0ull) {
+      const int j = (int)(s_pick[at] >> 8);
+      tokens = 0;
+      int last = -1;
+      for (; at < n2 && (int64_t)(s_pick[at] >> 8) == j; ++at) {
+        const int tl = (int)(s_pick[at] & 255);
+        if (tl == last) break;
+        tokens |= 1u << tl;
+        last = tl;
+      }
+      const int page = table[j];
+      if (page >= 0 && page < p.num_pages) return make_int2(j, page);
+    }
+    return make_int2(-1, -1);
+  };
+  auto load = [&](const int2& v, int part, int stage) {
+    const float* k = cache + (int64_t)v.y * 2 * plane + ((int64_t)g * P + part * KT) * D;
+    for (int i = threadIdx.x; i < KT * (D / 4); i += F_NT) {
+      const int row = i / (D / 4), e = i % (D / 4) * 4;
+      cp_async16(sK + (stage * F_KEYS + row) * D + (e ^ ((row & 7) << 2)), k + row * D + e, true);
+      cp_async16(sV + (stage * F_KEYS + row) * D + e, k + plane + row * D + e, true);
+    }
+  };
+  const int t = tile.y + warp;
+  const bool live = warp < tile.z;
+  const int pos = live ? p.positions[t] : -1;
+  const float* mine = sQ + warp * group * D;
+  constexpr int E = D / 32;                                // elements a lane
+  struct alignas(E * 4) Vec { float v[E]; };
+  float acc[G][E], m[G], l[G];
+#pragma unroll
+  for (int h = 0; h < G; ++h) {
+    m[h] = -INFINITY;
+    l[h] = 0.f;
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[h][e] = 0.f;
+  }
+  int at = 0, part = 0, stage = 0;
+  unsigned tokens = 0, tokens_next = 0;
+  int2 now = visit(at, tokens), next = now;
+  int part_next = 0;
+  if (now.x >= 0) load(now, 0, 0);
+  cp_async_commit();
+  while (now.x >= 0) {
+    tokens_next = tokens;
+    part_next = part + 1;
+    next = now;
+    if (part_next == per_page) { part_next = 0; next = visit(at, tokens_next); }
+    cp_async_wait<0>();
+    __syncthreads();                                       // the tile is here, and everyone is done with the one before
+    if (next.x >= 0) load(next, part_next, stage ^ 1);
+    cp_async_commit();
+    const int n = min(KT, pos - now.x * P - part * KT + 1);        // keys that the token sees
+    if (live && (tokens >> warp & 1) && n > 0) {
+      const int swap = (lane & 7) << 2;
+      const float *k = sK + (stage * F_KEYS + min(lane, KT - 1)) * D, *v = sV + stage * F_KEYS * D + lane * E;
+      float s[G];
+#pragma unroll
+      for (int h = 0; h < G; ++h) s[h] = 0.f;
+#pragma unroll 8
+      for (int e = 0; e < D; e += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(k + (e ^ swap));
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+          if (h < group) {
+            const float4 y = *reinterpret_cast<const float4*>(mine + h * D + e);
+            s[h] = fmaf(x.x, y.x, s[h]); s[h] = fmaf(x.y, y.y, s[h]); s[h] = fmaf(x.z, y.z, s[h]); s[h] = fmaf(x.w, y.w, s[h]);
+          }
+      }
+#pragma unroll
+      for (int h = 0; h < G; ++h)
+        if (h < group) {
+          s[h] = lane < n ? s[h] * p.scale : -INFINITY;
+          const float top = fmaxf(m[h], warp_max(s[h])), base = top == -INFINITY ? 0.f : top, alpha = expf(m[h] - base);
+          m[h] = top;
+          s[h] = lane < n ? expf(s[h] - base) : 0.f;
+          l[h] = fmaf(l[h], alpha, s[h]);                  // (a lane's own keys; the lanes come together at the end)
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[h][e] *= alpha;
+        }
+      auto add = [&](int i) {
+        const Vec x = *reinterpret_cast<const Vec*>(v + i * D);
+#pragma unroll
+        for (int h = 0; h < G; ++h)
+          if (h < group) {
+            const float w = __shfl_sync(0xffffffffu, s[h], i);
+#pragma unroll
+            for (int e = 0; e < E; ++e) acc[h][e] = fmaf(w, x.v[e], acc[h][e]);
+          }
+      };
+      int i = 0;
+      for (; i + 8 <= n; i += 8)
+#pragma unroll
+        for (int u = 0; u < 8; ++u) add(i + u);
+      for (; i < n; ++i) add(i);
+    }
+    now = next;
+    part = part_next;
+    tokens = tokens_next;
+    stage ^= 1;
+  }
+  cp_async_wait<0>();
+  if (!live) return;
+#pragma unroll
+  for (int h = 0; h < G; ++h)
+    if (h < group) {
+      const float sum = warp_sum(l[h]), inv = sum == 0.f ? 0.f : 1.f / sum;
+      Vec x;
+#pragma unroll
+      for (int e = 0; e < E; ++e) x.v[e] = acc[h][e] * inv;
+      *reinterpret_cast<Vec*>(out + (int64_t)t * p.ldo + (int64_t)(g * group + h) * D + lane * E) = x;
+    }
+}
+
+template <int D, int G>
+int run_float(const void* q, void* out, const void* cache, const Pages& p, cudaStream_t stream) {
+  const int group = p.H / p.Hkv;
+  int n2 = 1;
+  while (n2 < F_TOKENS * p.top) n2 <<= 1;
+  const size_t smem = (size_t)(4 * F_KEYS * D + F_TOKENS * group * D) * 4 + (size_t)n2 * 8;
+  auto kernel = pages_float_kernel<D, G>;
+  static thread_local int set_for = -1;                    // the attribute belongs to the device
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (set_for != dev) {
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * F_KEYS * D + F_TOKENS * G * D) * 4 + F_PICKS * 8) != cudaSuccess)
+      return cuda_status("attention_pages: shared memory");
+    set_for = dev;
+  }
+  const int tiles = p.T / F_TOKENS + (p.num_reqs < p.T ? p.num_reqs : p.T);
+  launch_pdl(kernel, dim3(tiles, p.Hkv), dim3(F_NT), smem, stream, (const float*)q, (float*)out, (const float*)cache, p);
+  return cuda_status("attention_pages (32-bit)");
+}
+
+// Whether the 32-bit kernel for several tokens a request takes the call.
+bool float_tiles(const void* q, const void* out, const void* cache, const Pages& p) {
+  return (p.D == 64 || p.D == 128) && p.page_size >= 16 && !(p.page_size & (p.page_size - 1)) && p.H / p.Hkv <= 8 && p.top * F_TOKENS <= F_PICKS &&
+         p.ldq % 4 == 0 && p.ldo % 4 == 0 && (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15) == 0 && p.Hkv <= 65535 &&
+         p.T >= 2 * (int64_t)p.num_reqs;
+}
 
 // ------------------------------------------------------------------------------------------------
 // Bfloat16, head sizes 64 and 128, pages of 16 to 128 tokens, groups of up to 16 heads: few tokens (decode steps).
@@ -434,6 +621,15 @@ DINFER_API int dinfer_attention_pages(const AttentionPagesArgs* a) {
     while (splits < 8 && (int64_t)T * Hkv * splits * 2 <= 2 * sms && splits * 2 * BN <= (int64_t)top * page_size) splits *= 2;
     if (D == 128) return H / Hkv <= 8 ? run_token<128, 1>(q, out, cache, p, splits, stream) : run_token<128, 2>(q, out, cache, p, splits, stream);
     return H / Hkv <= 8 ? run_token<64, 1>(q, out, cache, p, splits, stream) : run_token<64, 2>(q, out, cache, p, splits, stream);
+  }
+  if (dtype == DINFER_F32 && float_tiles(q, out, cache, p)) {
+    const int group = H / Hkv;
+#define DINFER_FLOAT(G) return D == 64 ? run_float<64, G>(q, out, cache, p, stream) : run_float<128, G>(q, out, cache, p, stream)
+    if (group == 1) DINFER_FLOAT(1);
+    if (group == 2) DINFER_FLOAT(2);
+    if (group <= 4) DINFER_FLOAT(4);
+    DINFER_FLOAT(8);
+#undef DINFER_FLOAT
   }
   DINFER_DISPATCH_DTYPE(dtype, E, { return run<E>(q, out, cache, p, stream); });
 }
