@@ -113,23 +113,24 @@ int run(const void* q, void* out, const void* cache, const Pages& p, cudaStream_
 
 
 // ------------------------------------------------------------------------------------------------
-// 32-bit, head sizes 64 and 128, groups of up to 8 heads: several tokens a request.  Eight neighbouring tokens share a block and walk
-// the pages that any of them chose in ascending order (their choices, sorted in shared memory), each page read once for all; a warp owns a
-// token and passes over the pages it did not choose.  Tiles of up to 32 keys ride two cp.async stages.  A score is a lane's own sum over
-// its key's row; for O the lanes split the elements and the keys that the token sees come one by one.  All of it multiply-adds in 32
+// 32-bit, head sizes 64 and 128, groups of up to 8 heads: several tokens a request.  Four neighbouring tokens share a block and walk
+// the pages that any of them chose in ascending order (their choices, sorted in shared memory), each page read once for all; two warps own a
+// token, half of a tile's keys each, and pass over the pages it did not choose.  Tiles of up to 32 keys ride a ring of cp.async stages.  A score is the sum of the
+// lanes that share a key's row; for O the lanes split the elements and the keys that the token sees come one by one.  All of it multiply-adds in 32
 // bits.  Bound by shared memory's reads (a key's row once for the group's scores, a value's once for its sums).
 // @FLOAT@
-constexpr int F_TOKENS = 8, F_NT = F_TOKENS * 32, F_KEYS = 32, F_PICKS = 1024;
+constexpr int F_TOKENS = 4, F_NT = F_TOKENS * 64, F_KEYS = 32, F_PICKS = 1024, F_STAGES = 2;
 
 template <int D, int G>              // G: at least the group
-__global__ void __launch_bounds__(F_NT)
+__global__ void __launch_bounds__(F_NT, G > 4 ? 2 : 3)
 pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const float* __restrict__ cache, const Pages p) {
   extern __shared__ __align__(16) unsigned char smem_raw[];
-  float* sK = reinterpret_cast<float*>(smem_raw);          // [2][F_KEYS][D], 16-byte pieces exchanged by key & 7: eight rows' in different banks
-  float* sV = sK + 2 * F_KEYS * D;                         // [2][F_KEYS][D]
-  float* sQ = sV + 2 * F_KEYS * D;                         // [F_TOKENS][group][D]
+  float* sK = reinterpret_cast<float*>(smem_raw);          // [F_STAGES][F_KEYS][D], 16-byte pieces exchanged by key & 7: eight rows' in different banks
+  float* sV = sK + F_STAGES * F_KEYS * D;                  // [F_STAGES][F_KEYS][D]
+  float* sQ = sV + F_STAGES * F_KEYS * D;                       // [F_TOKENS][group][D]
   // (page, token), sorted; all ones: none
   unsigned long long* s_pick = reinterpret_cast<unsigned long long*>(sQ + F_TOKENS * (p.H / p.Hkv) * D);
+  __shared__ int s_warp[F_NT / 32];
   pdl_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y;
   const int3 tile = token_tile(p.cu, p.num_reqs, F_TOKENS, blockIdx.x);
@@ -138,6 +139,8 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
   const int group = p.H / p.Hkv, P = p.page_size, picks = F_TOKENS * p.top;
   int n2 = 1;                                              // what is sorted: a power of two
   while (n2 < picks) n2 <<= 1;
+  int2* s_visit = reinterpret_cast<int2*>(s_pick + n2);    // (number in the request, page)
+  unsigned char* s_tokens = reinterpret_cast<unsigned char*>(s_visit + n2);
   for (int i = threadIdx.x; i < n2; i += F_NT) {
     const int tl = i / p.top, t = tile.y + tl;
     unsigned long long key = ~0ull;
@@ -164,25 +167,43 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
       }
       __syncthreads();
     }
-  // A visit is a page with the tokens that chose it (a token that names a page twice gets a second visit).  `at` runs over the picks.
+  // Visits: a page with the tokens that chose it (a token that names a page twice begins another visit), in order.
   const int KT = P < F_KEYS ? P : F_KEYS, per_page = P / KT;
   const int64_t plane = (int64_t)p.Hkv * P * D;
-  auto visit = [&](int& at, unsigned& tokens) {            // the next one's page in the table, or -1
-    while (at < n2 && s_pick[at] != ~0ull) {
-      const int j = (int)(s_pick[at] >> 8);
-      tokens = 0;
+  int visits = 0;
+  for (int i0 = 0; i0 < n2; i0 += F_NT) {
+    const int i = i0 + threadIdx.x;
+    const unsigned long long key = i < n2 ? s_pick[i] : ~0ull;
+    const bool begins = key != ~0ull && (i == 0 || s_pick[i - 1] >> 8 != key >> 8 || s_pick[i - 1] == key);
+    int3 v = make_int3((int)(key >> 8), -1, 0);
+    if (begins) {
       int last = -1;
-      for (; at < n2 && (int64_t)(s_pick[at] >> 8) == j; ++at) {
-        const int tl = (int)(s_pick[at] & 255);
+      for (int k = i; k < n2 && s_pick[k] >> 8 == key >> 8; ++k) {
+        const int tl = (int)(s_pick[k] & 255);
         if (tl == last) break;
-        tokens |= 1u << tl;
+        v.z |= 1 << tl;
         last = tl;
       }
-      const int page = table[j];
-      if (page >= 0 && page < p.num_pages) return make_int2(j, page);
+      v.y = table[v.x];
     }
-    return make_int2(-1, -1);
-  };
+    const bool in = begins && v.y >= 0 && v.y < p.num_pages;
+    const unsigned ball = __ballot_sync(0xffffffffu, in);
+    if (lane == 0) s_warp[warp] = __popc(ball);
+    __syncthreads();
+    int below = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < F_NT / 32; ++w) {
+      below += w < warp ? s_warp[w] : 0;
+      all += s_warp[w];
+    }
+    if (in) {
+      const int at = visits + below + __popc(ball & ((1u << lane) - 1));
+      s_visit[at] = make_int2(v.x, v.y);
+      s_tokens[at] = (unsigned char)v.z;
+    }
+    visits += all;
+    __syncthreads();
+  }
   auto load = [&](const int2& v, int part, int stage) {
     const float* k = cache + (int64_t)v.y * 2 * plane + ((int64_t)g * P + part * KT) * D;
     for (int i = threadIdx.x; i < KT * (D / 4); i += F_NT) {
@@ -191,10 +212,12 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
       cp_async16(sV + (stage * F_KEYS + row) * D + e, k + plane + row * D + e, true);
     }
   };
-  const int t = tile.y + warp;
-  const bool live = warp < tile.z;
+  const int tl = warp >> 1, half = warp & 1, t = tile.y + tl;
+  const bool live = tl < tile.z;
   const int pos = live ? p.positions[t] : -1;
-  const float* mine = sQ + warp * group * D;
+  // a warp's keys: half of the tile's, with as many lanes to a key as that leaves
+  const int keys = KT >> 1, sharing = 32 / keys, key = lane & (keys - 1), share = lane / keys, depth = D / sharing;
+  const float* mine = sQ + tl * group * D + share * depth;
   constexpr int E = D / 32;                                // elements a lane
   struct alignas(E * 4) Vec { float v[E]; };
   float acc[G][E], m[G], l[G];
@@ -205,31 +228,30 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
 #pragma unroll
     for (int e = 0; e < E; ++e) acc[h][e] = 0.f;
   }
-  int at = 0, part = 0, stage = 0;
-  unsigned tokens = 0, tokens_next = 0;
-  int2 now = visit(at, tokens), next = now;
-  int part_next = 0;
-  if (now.x >= 0) load(now, 0, 0);
-  cp_async_commit();
-  while (now.x >= 0) {
-    tokens_next = tokens;
-    part_next = part + 1;
-    next = now;
-    if (part_next == per_page) { part_next = 0; next = visit(at, tokens_next); }
-    cp_async_wait<0>();
-    __syncthreads();                                       // the tile is here, and everyone is done with the one before
-    if (next.x >= 0) load(next, part_next, stage ^ 1);
+  const int tiles = visits * per_page;
+#pragma unroll
+  for (int i = 0; i < F_STAGES - 1; ++i) {
+    if (i < tiles) load(s_visit[i / per_page], i % per_page, i);
     cp_async_commit();
-    const int n = min(KT, pos - now.x * P - part * KT + 1);        // keys that the token sees
-    if (live && (tokens >> warp & 1) && n > 0) {
-      const int swap = (lane & 7) << 2;
-      const float *k = sK + (stage * F_KEYS + min(lane, KT - 1)) * D, *v = sV + stage * F_KEYS * D + lane * E;
+  }
+  for (int i0 = 0; i0 < tiles; ++i0) {
+    const int stage = i0 % F_STAGES, ahead = i0 + F_STAGES - 1, part = i0 % per_page;
+    const int2 now = s_visit[i0 / per_page];
+    const unsigned tokens = s_tokens[i0 / per_page];
+    cp_async_wait<F_STAGES - 2>();
+    __syncthreads();                                       // the tile is here, and everyone is done with the one before
+    if (ahead < tiles) load(s_visit[ahead / per_page], ahead % per_page, ahead % F_STAGES);
+    cp_async_commit();
+    const int n = min(keys, pos - now.x * P - part * KT - half * keys + 1);        // of the warp's keys, those that the token sees
+    if (live && (tokens >> tl & 1) && n > 0) {
+      const int row = half * keys + key, swap = (row & 7) << 2;
+      const float *k = sK + (stage * F_KEYS + row) * D, *v = sV + (stage * F_KEYS + half * keys) * D + lane * E;
       float s[G];
 #pragma unroll
       for (int h = 0; h < G; ++h) s[h] = 0.f;
 #pragma unroll 8
-      for (int e = 0; e < D; e += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(k + (e ^ swap));
+      for (int e = 0; e < depth; e += 4) {
+        const float4 x = *reinterpret_cast<const float4*>(k + ((share * depth + e) ^ swap));
 #pragma unroll
         for (int h = 0; h < G; ++h)
           if (h < group) {
@@ -237,14 +259,17 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
             s[h] = fmaf(x.x, y.x, s[h]); s[h] = fmaf(x.y, y.y, s[h]); s[h] = fmaf(x.z, y.z, s[h]); s[h] = fmaf(x.w, y.w, s[h]);
           }
       }
+      for (int o = keys; o < 32; o <<= 1)
+#pragma unroll
+        for (int h = 0; h < G; ++h) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
 #pragma unroll
       for (int h = 0; h < G; ++h)
         if (h < group) {
-          s[h] = lane < n ? s[h] * p.scale : -INFINITY;
+          s[h] = key < n ? s[h] * p.scale : -INFINITY;
           const float top = fmaxf(m[h], warp_max(s[h])), base = top == -INFINITY ? 0.f : top, alpha = expf(m[h] - base);
           m[h] = top;
-          s[h] = lane < n ? expf(s[h] - base) : 0.f;
-          l[h] = fmaf(l[h], alpha, s[h]);                  // (a lane's own keys; the lanes come together at the end)
+          s[h] = key < n ? expf(s[h] - base) : 0.f;
+          l[h] = fmaf(l[h], alpha, share == 0 ? s[h] : 0.f);       // (a lane's own keys; the lanes come together at the end)
 #pragma unroll
           for (int e = 0; e < E; ++e) acc[h][e] *= alpha;
         }
@@ -264,20 +289,31 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
         for (int u = 0; u < 8; ++u) add(i + u);
       for (; i < n; ++i) add(i);
     }
-    now = next;
-    part = part_next;
-    tokens = tokens_next;
-    stage ^= 1;
   }
   cp_async_wait<0>();
-  if (!live) return;
+  __syncthreads();
+  // the two warps of a token come together in the tiles' memory
+  float* s_acc = sK + tl * G * (D + 2);
+#pragma unroll
+  for (int h = 0; h < G; ++h) l[h] = warp_sum(l[h]);
+  if (half == 1)
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+#pragma unroll
+      for (int e = 0; e < E; ++e) s_acc[h * (D + 2) + lane * E + e] = acc[h][e];
+      if (lane == 0) { s_acc[h * (D + 2) + D] = m[h]; s_acc[h * (D + 2) + D + 1] = l[h]; }
+    }
+  __syncthreads();
+  if (!live || half == 1) return;
 #pragma unroll
   for (int h = 0; h < G; ++h)
     if (h < group) {
-      const float sum = warp_sum(l[h]), inv = sum == 0.f ? 0.f : 1.f / sum;
+      const float* o = s_acc + h * (D + 2);
+      const float top = fmaxf(m[h], o[D]), base = top == -INFINITY ? 0.f : top, a = expf(m[h] - base), b = expf(o[D] - base);
+      const float sum = l[h] * a + o[D + 1] * b, inv = sum == 0.f ? 0.f : 1.f / sum;
       Vec x;
 #pragma unroll
-      for (int e = 0; e < E; ++e) x.v[e] = acc[h][e] * inv;
+      for (int e = 0; e < E; ++e) x.v[e] = (acc[h][e] * a + o[lane * E + e] * b) * inv;
       *reinterpret_cast<Vec*>(out + (int64_t)t * p.ldo + (int64_t)(g * group + h) * D + lane * E) = x;
     }
 }
@@ -287,13 +323,13 @@ int run_float(const void* q, void* out, const void* cache, const Pages& p, cudaS
   const int group = p.H / p.Hkv;
   int n2 = 1;
   while (n2 < F_TOKENS * p.top) n2 <<= 1;
-  const size_t smem = (size_t)(4 * F_KEYS * D + F_TOKENS * group * D) * 4 + (size_t)n2 * 8;
+  const size_t smem = (size_t)(2 * F_STAGES * F_KEYS * D + F_TOKENS * group * D) * 4 + (size_t)n2 * 17;
   auto kernel = pages_float_kernel<D, G>;
   static thread_local int set_for = -1;                    // the attribute belongs to the device
   int dev = 0;
   cudaGetDevice(&dev);
   if (set_for != dev) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (4 * F_KEYS * D + F_TOKENS * G * D) * 4 + F_PICKS * 8) != cudaSuccess)
+    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * F_STAGES * F_KEYS * D + F_TOKENS * G * D) * 4 + F_PICKS * 17) != cudaSuccess)
       return cuda_status("attention_pages: shared memory");
     set_for = dev;
   }
