@@ -43,6 +43,18 @@ def _take(d: Dict[str, Any], key: str, kind, default=_MISSING):
     return v
 
 
+def _page_attention(v) -> Optional[Dict[str, int]]:
+    if v is None:
+        return None
+    if not isinstance(v, dict) or set(v) - {"page", "top", "first", "recent"} or "top" not in v:
+        raise ConfigError("config.json: 'page_attention' must be an object with 'top' and, optionally, 'page', 'first' and 'recent'")
+    got = {"page": _take(v, "page", int, 64), "top": _take(v, "top", int), "first": _take(v, "first", int, 1),
+           "recent": _take(v, "recent", int, 1)}
+    if got["page"] <= 0 or got["first"] < 0 or got["recent"] < 1 or got["top"] < got["first"] + got["recent"]:
+        raise ConfigError(f"config.json: 'page_attention' needs positive pages and room for the first and recent ones among 'top', got {v!r}")
+    return got
+
+
 @dataclass(frozen=True)
 class Qwen3Config:
     """``config.json`` of ``Qwen3ForCausalLM``.
@@ -70,6 +82,9 @@ class Qwen3Config:
     hidden_act: str = "silu"
     eos_token_ids: Tuple[int, ...] = ()
     architecture: str = "Qwen3ForCausalLM"
+    # attention over chosen pages of the context instead of all of it: ``top`` pages a token at most, of ``page`` tokens (64), among them
+    # always the ``first`` (1) and the last ``recent`` ones (1, the token's own included)
+    page_attention: Optional[Dict[str, int]] = None
 
     @classmethod
     def from_dict(cls, d: Dict[str, Any]) -> "Qwen3Config":
@@ -106,6 +121,7 @@ class Qwen3Config:
             hidden_act=_take(d, "hidden_act", str, "silu"),
             eos_token_ids=eos_ids,
             architecture=str(archs[0]),
+            page_attention=_page_attention(d.get("page_attention")),
         )
         cfg.check()
         return cfg
@@ -150,7 +166,7 @@ class Qwen3Config:
         """The ``config.json`` dictionary that reads back as this configuration."""
         d: Dict[str, Any] = {"architectures": [self.architecture], "model_type": "qwen3"}
         for f in fields(self):
-            if f.name in ("eos_token_ids", "architecture"):
+            if f.name in ("eos_token_ids", "architecture") or (f.name == "page_attention" and not self.page_attention):
                 continue
             d[f.name] = getattr(self, f.name)
         if self.eos_token_ids:

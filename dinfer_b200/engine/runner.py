@@ -196,7 +196,8 @@ class ModelRunner:
         # one table width for all groups: what the group with the smallest pages needs
         self.max_blocks_per_seq = max([(e.max_model_len + b - 1) // b for b in sizes] or [(e.max_model_len + bs - 1) // bs])
         elt = 4 if self.act_dtype == torch.float32 else 2
-        bytes_per_token = sum(n.planes * n.num_kv_heads * n.head_dim * elt for n in needs if isinstance(n, KvCacheNeed))
+        bytes_per_token = sum(n.planes * n.num_kv_heads * n.head_dim * elt + (-(-n.num_kv_heads * n.head_dim * elt // (n.block_size or bs)) if n.key_means else 0)
+                              for n in needs if isinstance(n, KvCacheNeed))
         # every group gets pages for the same number of tokens: ``num_blocks`` pages of the engine's page size
         longest = (e.max_model_len + bs - 1) // bs
         if e.num_blocks is not None:
@@ -227,7 +228,7 @@ class ModelRunner:
         for i, (entry, n, sn) in enumerate(zip(self.spec.schedule, needs, states)):
             if entry.cache_from is not None:
                 src = self.bindings[entry.cache_from]
-                self.bindings.append(CacheBinding(kv=src.kv, group=src.group, write=False, state=src.state))
+                self.bindings.append(CacheBinding(kv=src.kv, group=src.group, write=False, state=src.state, means=src.means))
                 continue
             binding = CacheBinding()
             if isinstance(n, KvCacheNeed):
@@ -235,6 +236,8 @@ class ModelRunner:
                 binding.kv = torch.zeros((group_blocks[g], n.planes, n.num_kv_heads, sizes[g], n.head_dim),
                                          dtype=self.act_dtype, device=self.device)
                 binding.group = g
+                if n.key_means:
+                    binding.means = torch.zeros((group_blocks[g], n.num_kv_heads, n.head_dim), dtype=self.act_dtype, device=self.device)
             if isinstance(sn, StateNeed):
                 # one slot more than requests: the rows that pad a captured batch point at it
                 binding.state = torch.zeros((e.max_num_seqs + 1,) + tuple(sn.shape), dtype=sn.dtype, device=self.device)

@@ -1,7 +1,8 @@
 """Qwen3 dense (``Qwen3ForCausalLM``) as a list of parts.
 
 Every layer: RMSNorm -> GQA attention with per-head RMSNorm of q and k and neox RoPE over the whole
-head at ``rope_theta`` -> RMSNorm -> SwiGLU MLP; final RMSNorm; tied or untied head
+head at ``rope_theta`` -> RMSNorm -> SwiGLU MLP; final RMSNorm; tied or untied head.  With ``page_attention`` in the
+configuration a token's attention reads a few chosen pages of its context instead of all of it
 (models/qwen3/src/model.rs:129-315,427-496; tensor names listed at model.rs:5-6).
 """
 from __future__ import annotations
@@ -19,7 +20,8 @@ def qwen3_spec(cfg: Qwen3Config) -> ModelSpec:
         layers.append(LayerSpec(
             prefix=f"model.layers.{l}.",
             block="prenorm_residual",
-            mixer=PartSpec("gqa_attention", {
+            mixer=PartSpec("page_attention" if cfg.page_attention else "gqa_attention", {
+                **(cfg.page_attention or {}),
                 "num_heads": cfg.num_attention_heads, "num_kv_heads": cfg.num_key_value_heads,
                 "head_dim": cfg.head_dim, "qk_norm": True, "eps": cfg.rms_norm_eps, "position": position,
                 "q_proj": "self_attn.q_proj.weight", "k_proj": "self_attn.k_proj.weight",

@@ -29,7 +29,8 @@ class KvCacheNeed:
     ``block_size`` tokens (None: the engine's page size).  ``planes``: 2 = keys and values apart
     (``[pages, 2, Hkv, page, D]``); 1 = one row per token that serves as both (a latent cache:
     ``[pages, 1, Hkv, page, D]``).  ``chunked``: the window is a chunk of so many positions, counted from the
-    sequence's first: a token sees the tokens of its own chunk, and a chunk's pages go back when the next one begins."""
+    sequence's first: a token sees the tokens of its own chunk, and a chunk's pages go back when the next one begins.
+    ``key_means``: beside the pages the mean of each full page's keys (``CacheBinding.means``), which the mixer keeps up."""
     num_kv_heads: int
     head_dim: int
     window: Optional[int] = None
@@ -37,6 +38,7 @@ class KvCacheNeed:
     planes: int = 2
     keep_first: int = 0        # with a window: the first so many tokens of a request stay (their pages are not given back)
     chunked: bool = False
+    key_means: bool = False
 
     def group_key(self):
         # layers whose pages live and die together: same span of tokens, same page size
@@ -100,6 +102,7 @@ class CacheBinding:
     group: int = -1                        # index into StepContext.groups
     write: bool = True                     # False when the entry reads another entry's cache
     state: Optional[torch.Tensor] = None   # [num_slots, *shape] of this entry
+    means: Optional[torch.Tensor] = None   # [num_blocks, Hkv, D] of this entry, where the need asks for ``key_means``
 
 
 @dataclass

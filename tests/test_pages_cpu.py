@@ -113,3 +113,40 @@ def test_tensors_off_the_device_are_refused(monkeypatch):
     for call in ("append", "page_scores", "choose_pages", "attention_pages"):
         with pytest.raises(KernelError, match="CUDA tensors only"):
             getattr(page_ops, call)(**{k: v for k, v in args(call).items()})
+
+
+# ---------------------------------------------------------------- the model's configuration and the part
+
+def test_configuration_and_spec():
+    import helpers as H
+    from dinfer_b200.config.model_config import Qwen3Config
+    from dinfer_b200.models.qwen3 import qwen3_spec
+    plain = Qwen3Config.from_dict(H.TINY_D)
+    assert plain.page_attention is None and "page_attention" not in plain.to_dict()
+    assert all(l.mixer.kind == "gqa_attention" for l in qwen3_spec(plain).layers)
+    c = Qwen3Config.from_dict({**H.TINY_D, "page_attention": {"top": 8}})
+    assert c.page_attention == {"page": 64, "top": 8, "first": 1, "recent": 1} and Qwen3Config.from_dict(c.to_dict()) == c
+    mixers = [l.mixer for l in qwen3_spec(c).layers]
+    assert all(m.kind == "page_attention" and m.params["top"] == 8 and m.params["num_heads"] == 8 for m in mixers)
+
+
+@pytest.mark.parametrize("value", [{}, {"page": 16}, {"top": 4, "size": 16}, {"top": 1, "first": 1, "recent": 1}, {"top": 4, "recent": 0},
+                                   {"top": 4, "first": -1}, {"top": 4, "page": 0}, {"top": "4"}, [4], {"top": 4.0}])
+def test_configuration_refusals(value):
+    import helpers as H
+    from dinfer_b200.config.model_config import ConfigError, Qwen3Config
+    with pytest.raises(ConfigError):
+        Qwen3Config.from_dict({**H.TINY_D, "page_attention": value})
+
+
+@pytest.mark.parametrize("change", [dict(top=1), dict(recent=0), dict(first=-1), dict(page=0), dict(num_kv_heads=3), dict(head_dim=513)])
+def test_part_refusals(change):
+    from dinfer_b200.parts.base import BuildEnv, MIXERS
+    from dinfer_b200.parts import page_attention  # noqa: F401
+    env = BuildEnv(torch.device("cpu"), BF16, 64, 128)
+    params = dict(num_heads=4, num_kv_heads=2, head_dim=16, top=6, page=16)
+    mixer = MIXERS.get("page_attention")(params, env)
+    need = mixer.cache_need()
+    assert need.key_means and need.block_size == 16 and [d.shape for d in mixer.declare()] == [(64, 64), (32, 64), (32, 64), (64, 64)]
+    with pytest.raises(ValueError):
+        MIXERS.get("page_attention")({**params, **change}, env)
