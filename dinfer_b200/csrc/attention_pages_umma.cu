@@ -11,8 +11,9 @@
 //                                  (or that lie behind it) to -inf, exp2, P -> shared memory (bfloat16)
 //     O[128, D]  += P V            tcgen05.mma accumulating in tensor memory; O is rescaled in place only when a row's maximum grows
 //                                  by more than 2^8
-// A page is read once for the 256 rows, not once for each token that chose it, and no partial results leave the SM.  A warp none
-// of whose rows sees a tile passes it with zeros.
+// A page is read once for the 256 rows, not once for each token that chose it.  A warp none of whose rows sees a tile passes it with zeros.
+// Few tokens fill few SMs: then the blocks of a cluster share a pair's list, a run of its key tiles each, and fold their results
+// through distributed shared memory behind two cluster barriers, each block writing out a share of the 256 rows.
 //
 // Warp roles (384 threads): warp 0 brings Q (once) and K, warp 11 V, page by page through a map over the cache, each on a ring of its own;
 // warps 1 and 10 issue the products of the two row tiles; warps 2..9 are softmax and output, four per row tile.  Every mbarrier wait
@@ -52,6 +53,7 @@ struct Params {
   int unit, per_tile;                  // keys of a list entry (a page, or 64 of its keys), entries of a key tile
   int cap;                             // entries that a list has room for (a multiple of per_tile)
   int pairs;                           // pairs of row tiles that the grid counts
+  int ksplit;                          // blocks of a cluster that share a pair's list (1, 2, 4 or 8)
   int* counts;                         // [pairs][Hkv]: entries, to a multiple of per_tile
   int2* entries;                       // [pairs][Hkv][cap]: first row of the entry's keys in key head 0's share of the cache (-1: none), first position
   unsigned* masks;                     // [pairs][Hkv][cap][2][words]
@@ -157,12 +159,14 @@ __global__ void __launch_bounds__(LIST_NT) page_lists_kernel(const Params p) {
 
 // The rows of a block once more, a warp per row and key by key, from nothing but what the row's token sees.
 template <int D>
-__device__ __noinline__ void rows_again(const Params& p, int request, int first, int tokens, int g) {
+__device__ __noinline__ void rows_again(const Params& p, int request, int first, int tokens, int g, int row0, int row1) {
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int* table = p.table + (int64_t)request * p.width;
   const int64_t plane = (int64_t)p.Hkv * p.page_size * D;
-  for (int row = warp; row < tokens * p.group; row += NTHREADS / 32) {
-    const int t = first + row / p.group, h = g * p.group + row % p.group, pos = p.positions[t];
+  for (int row = row0 + warp; row < row1; row += NTHREADS / 32) {  // of the pair's 256
+    const int w = row / BM, r = row % BM, token = r / p.group;
+    if (token >= p.tile_tokens || w * p.tile_tokens + token >= tokens) continue;
+    const int t = first + w * p.tile_tokens + token, h = g * p.group + r % p.group, pos = p.positions[t];
     float qv[D / 32], acc[D / 32];
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) {
@@ -214,15 +218,18 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   __shared__ int s_abort, s_odd;
   __shared__ int s_first[LIST_SLOTS];                  // the list's beginning: first positions and bits
   __shared__ unsigned s_bits[LIST_SLOTS * 2];
+  __shared__ float x_max[2 * BM], x_sum[2 * BM];       // what the other blocks of a cluster found for the rows that this one writes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int hk = blockIdx.x;
+  const int rank = p.ksplit > 1 ? (int)cluster_ctarank() : 0, hk = blockIdx.x / p.ksplit;
   pdl_enter();
   const int3 pair = pair_of(p, blockIdx.y);
   if (pair.x < 0) return;                              // beyond the batch's pairs
   const int64_t at = (int64_t)blockIdx.y * p.Hkv + hk;
-  const int count = p.counts[at], n_tiles = (count & ~TWICE) / p.per_tile;
-  const int2* entries = p.entries + at * p.cap;
-  const unsigned* masks = p.masks + at * p.cap * 2 * p.words;
+  // this block's run of the list's key tiles
+  const int count = p.counts[at], all_tiles = (count & ~TWICE) / p.per_tile, per = (all_tiles + p.ksplit - 1) / p.ksplit;
+  const int tile0 = min(rank * per, all_tiles), n_tiles = min(per, all_tiles - tile0);
+  const int2* entries = p.entries + at * p.cap + tile0 * p.per_tile;
+  const unsigned* masks = p.masks + (at * p.cap + tile0 * p.per_tile) * 2 * p.words;
   const bool b_on = pair.z > p.tile_tokens;            // the second row tile exists
 
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
@@ -488,34 +495,113 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       if (!mbar_wait(smem_u32(&o_full[w]), 0)) { s_abort = 1; atomicExch(p.status, 66); ok = false; }
       tc_fence_after();
     }
-    if (ok && (w == 0 || b_on)) {
-      const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-      bool odd = row_ok && !(l_run == l_run);
-      __nv_bfloat16* dst = row_ok ? p.out + (int64_t)t * p.ldo + (int64_t)(hk * p.group + r % p.group) * D : nullptr;
+    const bool rows_on = w == 0 || b_on;
+    bool odd = false;
+    __nv_bfloat16* dst = row_ok ? p.out + (int64_t)t * p.ldo + (int64_t)(hk * p.group + r % p.group) * D : nullptr;
+    auto write = [&](float (&o)[32], int c, float l, float inv) {
+      if (!row_ok) return;
+      if (l == 0.f)                                                 // a row that sees nothing
 #pragma unroll
-      for (int c = 0; c < D / 32; ++c) {
-        float o[32];
-        if (n_w > 0) {
-          tmem_ld32(o_addr + c * 32, o);
-          tmem_ld_wait();
-        }
-        if (l_run == 0.f)                                           // a row that sees nothing
+        for (int i = 0; i < 32; ++i) o[i] = 0.f;
 #pragma unroll
-          for (int i = 0; i < 32; ++i) o[i] = 0.f;
-        if (row_ok) {
+      for (int i = 0; i < 32; ++i) odd |= !isfinite(o[i]);
 #pragma unroll
-          for (int i = 0; i < 32; ++i) odd |= !isfinite(o[i]);
+      for (int q4 = 0; q4 < 4; ++q4) {
+        uint4 v;
+        v.x = pack_bf16(o[q4 * 8] * inv, o[q4 * 8 + 1] * inv); v.y = pack_bf16(o[q4 * 8 + 2] * inv, o[q4 * 8 + 3] * inv);
+        v.z = pack_bf16(o[q4 * 8 + 4] * inv, o[q4 * 8 + 5] * inv); v.w = pack_bf16(o[q4 * 8 + 6] * inv, o[q4 * 8 + 7] * inv);
+        reinterpret_cast<uint4*>(dst + c * 32)[q4] = v;
+      }
+    };
+    if (p.ksplit == 1) {
+      if (ok && rows_on) {
+        const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+        odd = row_ok && !(l_run == l_run);
 #pragma unroll
-          for (int q4 = 0; q4 < 4; ++q4) {
-            uint4 v;
-            v.x = pack_bf16(o[q4 * 8] * inv, o[q4 * 8 + 1] * inv); v.y = pack_bf16(o[q4 * 8 + 2] * inv, o[q4 * 8 + 3] * inv);
-            v.z = pack_bf16(o[q4 * 8 + 4] * inv, o[q4 * 8 + 5] * inv); v.w = pack_bf16(o[q4 * 8 + 6] * inv, o[q4 * 8 + 7] * inv);
-            reinterpret_cast<uint4*>(dst + c * 32)[q4] = v;
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (n_w > 0) {
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_ld_wait();
           }
+          write(o, c, l_run, inv);
         }
       }
-      if (odd) s_odd = 1;
+    } else {
+      // The rows are dealt out in runs of 32 (one warp's): block `dest` writes the run out, the others send it their unnormalised O, their
+      // reference maximum and their sum, into the stages and P, which are free once every block's products are complete (the
+      // first barrier).  What a block receives: [sender][4-column group][row of the block's runs] float4.
+      constexpr int C4 = D / 4;
+      const int run = w * 4 + quarter, runs_per = 8 / p.ksplit, dest = run / runs_per, rows_r = runs_per * 32;
+      const int rloc = (run % runs_per) * 32 + lane;
+      const bool mine = ok && n_w > 0;                              // O_w of this block holds something
+      cluster_sync_all();
+      if (dest != rank) {
+        const int slot = rank < dest ? rank : rank - 1;
+        if (mine) {
+          const uint32_t remote = map_to_rank(sK, (uint32_t)dest) + (uint32_t)((slot * C4 * rows_r + rloc) * 16);
+#pragma unroll
+          for (int c = 0; c < D / 32; ++c) {
+            float o[32];
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_ld_wait();
+#pragma unroll
+            for (int q4 = 0; q4 < 8; ++q4)
+              st_cluster_f32x4(remote + (uint32_t)((c * 8 + q4) * rows_r * 16), o[q4 * 4], o[q4 * 4 + 1], o[q4 * 4 + 2], o[q4 * 4 + 3]);
+          }
+        }
+        st_cluster_f32(map_to_rank(smem_u32(&x_max[slot * rows_r + rloc]), (uint32_t)dest), mine ? m_run : -INFINITY);
+        st_cluster_f32(map_to_rank(smem_u32(&x_sum[slot * rows_r + rloc]), (uint32_t)dest), mine ? l_run : 0.f);
+      }
+      cluster_sync_all();
+      if (dest == rank && rows_on && ok) {
+        float m_all = mine ? m_run : -INFINITY;
+        for (int sl = 0; sl < p.ksplit - 1; ++sl) m_all = fmaxf(m_all, x_max[sl * rows_r + rloc]);
+        const float base_m = m_all == -INFINITY ? 0.f : m_all;
+        const float a_own = mine && l_run != 0.f ? fast_exp2(m_run - base_m) : 0.f;
+        float l_all = mine ? l_run * a_own : 0.f;
+        for (int sl = 0; sl < p.ksplit - 1; ++sl) {
+          const float l_p = x_sum[sl * rows_r + rloc];
+          if (l_p != 0.f) l_all += l_p * fast_exp2(x_max[sl * rows_r + rloc] - base_m);
+        }
+        const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
+        odd = row_ok && !(l_all == l_all);
+        const float4* recv = reinterpret_cast<const float4*>(smem_dyn + (sK - smem_u32(smem_dyn)));
+#pragma unroll
+        for (int c = 0; c < D / 32; ++c) {
+          float o[32];
+          if (mine) {                                               // the whole warp or none of it: tcgen05.ld is a warp's instruction
+            tmem_ld32(o_addr + c * 32, o);
+            tmem_ld_wait();
+          }
+          // (a block none of whose keys a row sees holds sums of zeros for it, or what is not a finite number; its part counts only
+          // where that shows)
+#pragma unroll
+          for (int i = 0; i < 32; ++i) {
+            if (mine) odd |= row_ok && !isfinite(o[i]);
+            o[i] = a_own != 0.f ? o[i] * a_own : 0.f;
+          }
+          for (int sl = 0; sl < p.ksplit - 1; ++sl) {
+            const float l_p = x_sum[sl * rows_r + rloc];
+            if (l_p != 0.f) {
+              const float a_p = fast_exp2(x_max[sl * rows_r + rloc] - base_m);
+#pragma unroll
+              for (int q4 = 0; q4 < 8; ++q4) {
+                const float4 v = recv[(sl * C4 + c * 8 + q4) * rows_r + rloc];
+                o[q4 * 4] = fmaf(a_p, v.x, o[q4 * 4]); o[q4 * 4 + 1] = fmaf(a_p, v.y, o[q4 * 4 + 1]);
+                o[q4 * 4 + 2] = fmaf(a_p, v.z, o[q4 * 4 + 2]); o[q4 * 4 + 3] = fmaf(a_p, v.w, o[q4 * 4 + 3]);
+              }
+            }
+          }
+          write(o, c, l_all, inv);
+        }
+      }
     }
+    if (odd) s_odd = 1;
+  }
+  if (p.ksplit > 1 && (warp < 2 || warp >= MMA_WARP_B)) {           // the other warps pass the cluster's two barriers too
+    cluster_sync_all();
+    cluster_sync_all();
   }
 
   tc_fence_before();
@@ -527,7 +613,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     tc_fence_after();
     asm volatile("tcgen05.dealloc.cta_group::1.sync.aligned.b32 %0, %1;" ::"r"(tmem), "r"(TMEM_COLS) : "memory");
   }
-  if (s_odd) rows_again<D>(p, pair.x, pair.y, pair.z, hk);
+  if (s_odd) rows_again<D>(p, pair.x, pair.y, pair.z, hk, rank * (2 * BM / p.ksplit), (rank + 1) * (2 * BM / p.ksplit));
 }
 
 typedef CUresult (*EncodeTiledFn)(CUtensorMap*, CUtensorMapDataType, cuuint32_t, void*, const cuuint64_t*, const cuuint64_t*,
@@ -545,6 +631,7 @@ EncodeTiledFn encode_fn() {
 
 template <int D, int NP>
 int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const Params& p, cudaStream_t stream) {
+  static_assert((size_t)2 * STAGES * BN * D * 2 + 2 * BM * BN * 2 >= (size_t)7 * 32 * D * 4, "the stages and P hold what seven senders bring");
   auto k = attention_pages_umma_kernel<D, NP>;
   constexpr size_t sm = smem_bytes<D>();
   static thread_local int set_for = -1;                    // the attribute belongs to the device
@@ -556,7 +643,7 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const Params& p, cudaS
     set_for = dev;
   }
   launch_pdl(page_lists_kernel, dim3(p.Hkv, p.pairs), dim3(LIST_NT), 0, stream, p);
-  launch_pdl(k, dim3(p.Hkv, p.pairs), dim3(NTHREADS), sm, stream, mq, mkv, p);
+  launch_pdl_cluster(k, dim3(p.Hkv * p.ksplit, p.pairs), dim3(NTHREADS), dim3(p.ksplit), sm, stream, mq, mkv, p);
   return cuda_status("attention_pages_umma");
 }
 
@@ -565,7 +652,8 @@ int64_t room(Params& p, unsigned char* at) {
   p.words = (p.tile_tokens + 31) / 32;
   p.unit = p.page_size < BN ? p.page_size : BN;
   p.per_tile = BN / p.unit;
-  const int64_t pairs = (int64_t)p.T / (2 * p.tile_tokens) + (p.B < p.T ? p.B : p.T);     // of every way the tokens may be dealt out
+  // pairs of every way the tokens may be dealt out: a request's last one may be all but empty
+  const int64_t tile = 2 * p.tile_tokens, pairs = (p.T + (tile - 1) * (p.B < p.T ? p.B : p.T)) / tile;
   p.pairs = (int)(pairs > INT32_MAX ? INT32_MAX : pairs);
   const int64_t most = (int64_t)2 * p.tile_tokens * p.top, pages = most < p.width ? most : p.width;
   p.cap = (int)((pages * (p.page_size / p.unit) + p.per_tile - 1) / p.per_tile * p.per_tile);
@@ -613,6 +701,7 @@ struct AttentionPagesArgs {
   void* workspace;
   int64_t workspace_bytes;
   int* status;
+  int64_t sms;
   cudaStream_t stream;
 };
 
@@ -631,6 +720,7 @@ DINFER_API int dinfer_attention_pages_umma(const AttentionPagesArgs* a) {
   void* workspace = a->workspace;
   const int64_t workspace_bytes = a->workspace_bytes;
   int* status = a->status;
+  const int sms = (int)a->sms;
   const int64_t need = dinfer_attention_pages_umma_workspace(num_reqs, width, top, T, H, Hkv, D, page_size);
   if (need == 0) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d width=%d", T, H, Hkv, D, page_size, top, width);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255) || !status)
@@ -648,6 +738,9 @@ DINFER_API int dinfer_attention_pages_umma(const AttentionPagesArgs* a) {
   p.chosen = chosen; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.page_size = page_size; p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   room(p, (unsigned char*)workspace);
+  // blocks that share a list: as far as all run at the same time (one an SM), each with four key tiles of the longest list there may be
+  p.ksplit = 1;
+  while (p.ksplit < 8 && (int64_t)p.pairs * Hkv * p.ksplit * 2 <= sms && p.cap / p.per_tile >= p.ksplit * 2 * 4) p.ksplit *= 2;
   CUtensorMap mq, mkv;
   {
     cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};

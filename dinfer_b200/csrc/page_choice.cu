@@ -151,7 +151,7 @@ page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const _
 // bounded.  Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2.  @SCORES@
 constexpr int U_ROWS = 128, U_COLS = 128, U_NT = 256;
 // from so many tokens on, and so many a request
-constexpr int MANY_TOKENS = 64, MANY_TOKENS_A_REQUEST = 16;
+constexpr int MANY_TOKENS = 16, MANY_TOKENS_A_REQUEST = 2;
 
 template <int D, int GP>
 __global__ void __launch_bounds__(U_NT, 2)

@@ -31,7 +31,7 @@ _PACK = {
     "dinfer_page_scores": struct.Struct("22q").pack,
     "dinfer_choose_pages": struct.Struct("13q").pack,
     "dinfer_attention_pages": struct.Struct("18qd3q").pack,
-    "dinfer_attention_pages_umma": struct.Struct("18qd4q").pack,
+    "dinfer_attention_pages_umma": struct.Struct("18qd5q").pack,
 }
 _BOUND = {}
 _SMS = {}                               # multiprocessors by device
@@ -274,7 +274,7 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
         if size:
             work = torch.empty(size, dtype=torch.uint8, device=q.device)
             _call("attention_pages_umma", "dinfer_attention_pages_umma", "attention_pages_umma", *head, work.data_ptr(), size,
-                  gemm_ops._state(q.device)["status"].data_ptr())
+                  gemm_ops._state(q.device)["status"].data_ptr(), _multiprocessors())
             return out
     _call("attention_pages", "dinfer_attention_pages", what, *head, _multiprocessors(), code)
     return out
