@@ -24,6 +24,7 @@
 // only from keys that they see.  The same goes for a block one of whose tokens names a page twice (it then counts twice, which a bit
 // cannot say).
 #include <cuda.h>
+#include <math.h>
 
 #include "common.cuh"
 #include "umma_attention.cuh"
@@ -629,8 +630,32 @@ EncodeTiledFn encode_fn() {
   return fn;
 }
 
+// Clusters of so many blocks that the device runs at a time (an SM holds one block, a cluster's SMs are neighbours), asked once a device.
 template <int D, int NP>
-int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const Params& p, cudaStream_t stream) {
+int max_clusters(int ksplit) {
+  static thread_local int asked_for = -1, found[4];
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (asked_for != dev) {
+    for (int i = 1; i < 4; ++i) {
+      cudaLaunchConfig_t cfg = {};
+      cfg.gridDim = dim3(64 << i); cfg.blockDim = dim3(NTHREADS); cfg.dynamicSmemBytes = smem_bytes<D>();
+      cudaLaunchAttribute attr[1];
+      attr[0].id = cudaLaunchAttributeClusterDimension;
+      attr[0].val.clusterDim.x = 1 << i; attr[0].val.clusterDim.y = 1; attr[0].val.clusterDim.z = 1;
+      cfg.attrs = attr; cfg.numAttrs = 1;
+      if (cudaOccupancyMaxActiveClusters(&found[i], attention_pages_umma_kernel<D, NP>, &cfg) != cudaSuccess) {
+        cudaGetLastError();
+        found[i] = 0;                                      // none: lists are not shared
+      }
+    }
+    asked_for = dev;
+  }
+  return found[ksplit == 2 ? 1 : ksplit == 4 ? 2 : 3];
+}
+
+template <int D, int NP>
+int launch(const CUtensorMap& mq, const CUtensorMap& mkv, Params& p, cudaStream_t stream) {
   static_assert((size_t)2 * STAGES * BN * D * 2 + 2 * BM * BN * 2 >= (size_t)7 * 32 * D * 4, "the stages and P hold what seven senders bring");
   auto k = attention_pages_umma_kernel<D, NP>;
   constexpr size_t sm = smem_bytes<D>();
@@ -642,6 +667,9 @@ int launch(const CUtensorMap& mq, const CUtensorMap& mkv, const Params& p, cudaS
       return cuda_status("attention_pages_umma: shared memory");
     set_for = dev;
   }
+  // blocks that share a list: as far as all clusters run at the same time, each with four key tiles of the longest list there may be
+  p.ksplit = 1;
+  for (int ks = 2; ks <= 8 && p.cap / p.per_tile >= ks * 4 && (int64_t)p.pairs * p.Hkv <= max_clusters<D, NP>(ks); ks *= 2) p.ksplit = ks;
   launch_pdl(page_lists_kernel, dim3(p.Hkv, p.pairs), dim3(LIST_NT), 0, stream, p);
   launch_pdl_cluster(k, dim3(p.Hkv * p.ksplit, p.pairs), dim3(NTHREADS), dim3(p.ksplit), sm, stream, mq, mkv, p);
   return cuda_status("attention_pages_umma");
@@ -672,14 +700,33 @@ constexpr int64_t MAX_ROOM = 1ll << 30;
 
 DINFER_DEFINE_LAST_ERROR()
 
-// Bytes of workspace that the call wants, 0 where it does not take the sizes.
-DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size) {
+static int64_t workspace_of(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size, Params& p) {
   if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > BM || top <= 0 || width <= 0 || num_reqs <= 0 || (D != 64 && D != 128)) return 0;
   if (page_size < 16 || page_size > 128 || (page_size & (page_size - 1)) || (int64_t)width * page_size > INT32_MAX) return 0;
-  Params p{};
   p.width = width; p.B = num_reqs; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.page_size = page_size;
   const int64_t bytes = room(p, nullptr);
   return p.pairs > 65535 || bytes > MAX_ROOM ? 0 : bytes;
+}
+
+// Bytes of workspace that the call wants; 0 where it does not take the sizes, or (sms > 0, the device's multiprocessors) where token by
+// token is the shorter way.  Both are estimated, in microseconds.  Token by token every page is read for each token that chose it, at what L2 gives:
+//     7 + T Hkv top page_size D 4 / 6.3e6
+// Here a block takes 1.3 a key tile of 64, 20 pass before and after, and n neighbouring tokens choose some top n^0.4 pages among them.
+// The longest list (one request may bring all tokens but one each of the others) ends the step, or the lists of all do:
+//     20 + 1.3 max(tiles of the longest / ksplit, tiles of all / SMs)
+// Measured at 32 heads of 128 over 8, 16 pages of 64 behind 8000 tokens (us, token by token and here): 32 tokens 26 and 29, 64 tokens 51
+// and 36, 256 tokens 173 and 48, 64 tokens beside 16 single ones 70 and 120, 256 beside 16 190 and 120, 64 single ones 54 and 107.
+DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size, int sms) {
+  Params p{};
+  const int64_t bytes = workspace_of(num_reqs, width, top, T, H, Hkv, D, page_size, p);
+  if (bytes == 0 || sms <= 0) return bytes;
+  const double by_token = 7.0 + (double)T * Hkv * (top < width ? top : width) * page_size * D * 4 / 6.3e6;
+  auto tiles = [&](double n) { return fmin((double)width, top * pow(fmax(n, 1.0), 0.4)) * page_size / BN; };
+  const double most = 2.0 * p.tile_tokens, longest = fmin(T - num_reqs + 1.0, most), mean = fmin((double)T / num_reqs, most);
+  const double lists = fmax((double)T / most, (double)(num_reqs < T ? num_reqs : T)) * Hkv;
+  int ks = 1;
+  while (ks < 8 && lists * ks * 2 <= sms && tiles(longest) >= ks * 8) ks *= 2;
+  return 20.0 + 1.3 * fmax(tiles(longest) / ks, lists * tiles(mean) / sms) < by_token ? bytes : 0;
 }
 
 // What the call takes, 8 bytes a field (a caller packs them and hands over one address).  As
@@ -701,7 +748,6 @@ struct AttentionPagesArgs {
   void* workspace;
   int64_t workspace_bytes;
   int* status;
-  int64_t sms;
   cudaStream_t stream;
 };
 
@@ -720,8 +766,8 @@ DINFER_API int dinfer_attention_pages_umma(const AttentionPagesArgs* a) {
   void* workspace = a->workspace;
   const int64_t workspace_bytes = a->workspace_bytes;
   int* status = a->status;
-  const int sms = (int)a->sms;
-  const int64_t need = dinfer_attention_pages_umma_workspace(num_reqs, width, top, T, H, Hkv, D, page_size);
+  Params p{};
+  const int64_t need = workspace_of(num_reqs, width, top, T, H, Hkv, D, page_size, p);
   if (need == 0) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d width=%d", T, H, Hkv, D, page_size, top, width);
   if (!workspace || workspace_bytes < need || ((uintptr_t)workspace & 255) || !status)
     return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: a workspace of %lld bytes and a status word are required", (long long)need);
@@ -732,15 +778,11 @@ DINFER_API int dinfer_attention_pages_umma(const AttentionPagesArgs* a) {
   if (num_pages <= 0 || cache_rows > INT32_MAX) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: %d pages are too many rows for a tensor map's coordinate", num_pages);
   EncodeTiledFn fn = encode_fn();
   if (!fn) return refuse(DINFER_BAD_ARGUMENT, "attention_pages_umma: cuTensorMapEncodeTiled is not available from this driver");
-  Params p{};
   p.q = (const __nv_bfloat16*)q; p.ldq = ldq; p.out = (__nv_bfloat16*)out; p.ldo = ldo; p.cache = (const __nv_bfloat16*)cache;
   p.num_pages = num_pages; p.table = table; p.width = width; p.cu = cu_seqlens; p.B = num_reqs; p.positions = positions;
   p.chosen = chosen; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.page_size = page_size; p.scale = scale;
   p.scale_log2 = scale * 1.4426950408889634f; p.status = status;
   room(p, (unsigned char*)workspace);
-  // blocks that share a list: as far as all run at the same time (one an SM), each with four key tiles of the longest list there may be
-  p.ksplit = 1;
-  while (p.ksplit < 8 && (int64_t)p.pairs * Hkv * p.ksplit * 2 <= sms && p.cap / p.per_tile >= p.ksplit * 2 * 4) p.ksplit *= 2;
   CUtensorMap mq, mkv;
   {
     cuuint64_t dims[3] = {(cuuint64_t)D, (cuuint64_t)H, (cuuint64_t)T};

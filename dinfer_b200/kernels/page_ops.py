@@ -31,7 +31,7 @@ _PACK = {
     "dinfer_page_scores": struct.Struct("22q").pack,
     "dinfer_choose_pages": struct.Struct("13q").pack,
     "dinfer_attention_pages": struct.Struct("18qd3q").pack,
-    "dinfer_attention_pages_umma": struct.Struct("18qd5q").pack,
+    "dinfer_attention_pages_umma": struct.Struct("18qd4q").pack,
 }
 _BOUND = {}
 _SMS = {}                               # multiprocessors by device
@@ -66,19 +66,19 @@ def _stream() -> int:
     return _raw_stream(_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-# Steps of at least so many tokens, and so many a request, walk the pages that neighbouring tokens chose together
-PORTION_TOKENS = 64
-PORTION_TOKENS_A_REQUEST = 4
+# Steps of fewer tokens are not asked about: token by token is the shorter way for them
+PORTION_TOKENS = 24
 
 
-def _portions(head) -> int:
-    """Bytes of workspace of the kernel for portions where it takes this call, else 0: rows that TMA can address, a positive scale."""
+def _portions(head, always: bool = False) -> int:
+    """Bytes of workspace of the kernel in which neighbouring tokens walk the pages they chose together, where it takes this call (rows that
+    TMA can address, a positive scale) and is the shorter way (or ``always``); else 0."""
     q, ldq, out, ldo, cache, num_pages, _, width, _, B, _, _, top, T, H, Hkv, D, page_size, scale = head
     if not scale > 0 or ldq % 8 or ldo % 8 or (q | out | cache) % 16 or num_pages * 2 * Hkv * page_size > 0x7fffffff:
         return 0
     f = library("attention_pages_umma").dinfer_attention_pages_umma_workspace
-    f.argtypes, f.restype = [c_int] * 8, c_int64
-    return f(B, width, top, T, H, Hkv, D, page_size)
+    f.argtypes, f.restype = [c_int] * 9, c_int64
+    return f(B, width, top, T, H, Hkv, D, page_size, 0 if always else _multiprocessors())
 
 
 def _here(what: str, *tensors) -> None:
@@ -210,7 +210,7 @@ def page_scores(q: torch.Tensor, means: torch.Tensor, block_table: torch.Tensor,
         ldt, ldg, _ = out.stride()
     _call("page_choice", "dinfer_page_scores", what, q.data_ptr(), ldq, means.data_ptr(), num_pages, block_table.data_ptr(), width,
           cu_seqlens.data_ptr(), B, positions.data_ptr(), out.data_ptr(), ldt, ldg, T, num_heads, Hkv, D, page_size, pages,
-          _code(what, q.dtype), _multiprocessors(), gemm_ops._state(q.device)["status"].data_ptr())
+          _code(what, q.dtype), *((_multiprocessors(), gemm_ops._state(q.device)["status"].data_ptr()) if T >= 16 else (0, 0)))
     return out
 
 
@@ -269,12 +269,12 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     top = shape[2]
     head = (q.data_ptr(), ldq, out.data_ptr(), ldo, cache.data_ptr(), num_pages, block_table.data_ptr(), width, cu_seqlens.data_ptr(), B,
             positions.data_ptr(), chosen.data_ptr(), top, T, num_heads, Hkv, D, page_size, scale)
-    if T >= PORTION_TOKENS and T >= PORTION_TOKENS_A_REQUEST * B and dt == _BF16:
+    if T >= PORTION_TOKENS and T > B and dt == _BF16:
         size = _portions(head)
         if size:
             work = torch.empty(size, dtype=torch.uint8, device=q.device)
             _call("attention_pages_umma", "dinfer_attention_pages_umma", "attention_pages_umma", *head, work.data_ptr(), size,
-                  gemm_ops._state(q.device)["status"].data_ptr(), _multiprocessors())
+                  gemm_ops._state(q.device)["status"].data_ptr())
             return out
     _call("attention_pages", "dinfer_attention_pages", what, *head, _multiprocessors(), code)
     return out

@@ -213,13 +213,31 @@ def choices(b, G, top, g, kind):
 ATTENTION = SIZES + [([(2000, 200), (0, 300)], 16, 8, 2, 128), ([(777, 300)], 64, 16, 1, 64), ([(640, 150)], 32, 12, 4, 128),
                      ([(256, 130), (31, 1), (100, 1), (2, 2)], 64, 8, 8, 128), ([(400, 90)], 128, 4, 2, 64), ([(50, 40)] * 5, 16, 10, 2, 128),
                      ([(3000, 500), (20, 90), (500, 1)], 64, 8, 2, 128), ([(70, 300)], 32, 6, 2, 64), ([(0, 129), (4000, 64)], 16, 32, 2, 64),
-                     ([(1, 200)], 16, 3, 3, 128)]
+                     ([(1, 200)], 16, 3, 3, 128), ([(900, 700)], 64, 8, 1, 64), ([(300, 20), (5, 3)], 64, 48, 3, 128)]
+
+
+@pytest.fixture(params=["by rule", "together"])
+def form(request, monkeypatch):
+    """Which kernel runs: the one that the sizes choose, or, wherever it takes the call, the one in which neighbouring tokens walk the
+    pages that they chose together (at these sizes the rule seldom takes it)."""
+    from dinfer_b200.kernels import page_ops
+    calls, real = [], page_ops._call
+
+    def counted(lib, *args):
+        calls.append(lib)
+        return real(lib, *args)
+    monkeypatch.setattr(page_ops, "_call", counted)
+    if request.param == "together":
+        rule = page_ops._portions
+        monkeypatch.setattr(page_ops, "_portions", lambda head: rule(head, True))
+        monkeypatch.setattr(page_ops, "PORTION_TOKENS", 1)
+    return request.param, calls
 
 
 @pytest.mark.parametrize("kind", ["usual", "far", "odd"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("size", ATTENTION, ids=str)
-def test_attention(size, dtype, kind):
+def test_attention(size, dtype, kind, form):
     from dinfer_b200.kernels import page_ops
     requests, P, H, G, D = size
     if dtype == F32 and sum(n for _, n in requests) > 120:
@@ -245,12 +263,14 @@ def test_attention(size, dtype, kind):
     off = (got[:b.live, :H * D].double() - want).abs()
     bound = attention_bound(dtype, D, want, size_, qk)
     assert bool((off <= bound).all()), float((off / bound).max())
+    if form[0] == "together" and dtype == BF16 and D in (64, 128) and P in (16, 32, 64, 128) and b.T > len(requests):
+        assert form[1] == ["attention_pages_umma"]
 
 
 @pytest.mark.parametrize("new", [1, 5, 100, 400])
 @pytest.mark.parametrize("what", ["value", "key"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_no_token_sees_a_later_one(dtype, what, new):
+def test_no_token_sees_a_later_one(dtype, what, new, form):
     """A NaN in a token's own key or value reaches the tokens from it on that read its page, and nothing before or beside: those are
     what they are without it, up to the bound that every result keeps (the kernel for portions makes the rows beside such a value
     again, one by one, with sums in another order)."""
@@ -277,7 +297,7 @@ def test_no_token_sees_a_later_one(dtype, what, new):
 
 @pytest.mark.parametrize("new", [1, 200])
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_large_scores(dtype, new):
+def test_large_scores(dtype, new, form):
     """Scores far apart (a softmax that keeps one key) and far from zero, and keys of the type's lowest value."""
     from dinfer_b200.kernels import page_ops
     P, H, G, D = 32, 8, 2, 64
@@ -297,7 +317,7 @@ def test_large_scores(dtype, new):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
-def test_a_layer_prompt_whole_and_token_by_token(dtype):
+def test_a_layer_prompt_whole_and_token_by_token(dtype, form):
     """The four calls as a layer makes them: a prompt in portions and then single tokens, beside another request, against the plain
     form of every token on the cache and means that were built."""
     from dinfer_b200.kernels import page_ops
@@ -333,7 +353,7 @@ def test_a_layer_prompt_whole_and_token_by_token(dtype):
 
 
 @pytest.mark.parametrize("new", [[(700, 1), (90, 1), (300, 1)], [(700, 200), (90, 1), (0, 90)]])
-def test_replayed_from_a_graph_on_another_stream(new):
+def test_replayed_from_a_graph_on_another_stream(new, form):
     """The four calls captured once and replayed on other inputs, and eager calls on a stream of their own: the same as eager."""
     from dinfer_b200.kernels import page_ops
     P, H, G, D, top = 32, 8, 2, 128, 6
