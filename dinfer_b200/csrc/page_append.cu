@@ -131,9 +131,18 @@ template <typename T> __device__ __forceinline__ void store_lane(T* row, int a, 
   *reinterpret_cast<Vec4<T>*>(row + a) = x.a;
   *reinterpret_cast<Vec4<T>*>(row + b) = x.b;
 }
-template <typename T> __device__ __forceinline__ void widen(const Lane8<T>& x, float (&v)[8]) {
+template <typename T> __device__ __forceinline__ void widen(const Lane8<T>& x, float (&v)[8]);
+template <> __device__ __forceinline__ void widen<float>(const Lane8<float>& x, float (&v)[8]) {
 #pragma unroll
-  for (int j = 0; j < 4; ++j) { v[j] = to_f32<T>(x.a.v[j]); v[4 + j] = to_f32<T>(x.b.v[j]); }
+  for (int j = 0; j < 4; ++j) { v[j] = x.a.v[j]; v[4 + j] = x.b.v[j]; }
+}
+template <> __device__ __forceinline__ void widen<__nv_bfloat16>(const Lane8<__nv_bfloat16>& x, float (&v)[8]) {
+  const unsigned *a = reinterpret_cast<const unsigned*>(x.a.v), *b = reinterpret_cast<const unsigned*>(x.b.v);
+#pragma unroll
+  for (int j = 0; j < 2; ++j) {                                // a bfloat16 is the upper half of the number it stands for
+    v[2 * j] = __uint_as_float(a[j] << 16); v[2 * j + 1] = __uint_as_float(a[j] & 0xffff0000u);
+    v[4 + 2 * j] = __uint_as_float(b[j] << 16); v[5 + 2 * j] = __uint_as_float(b[j] & 0xffff0000u);
+  }
 }
 template <typename T> __device__ __forceinline__ Lane8<T> narrow(const float (&v)[8]);
 template <> __device__ __forceinline__ Lane8<float> narrow<float>(const float (&v)[8]) {
@@ -185,16 +194,16 @@ __device__ __forceinline__ void finish(float (&v)[8], bool norm, const float (&w
 }
 
 constexpr int MAX_PAGE = 128;        // tokens of a page
-constexpr int FEW_TOKENS = 512;
+constexpr int FEW_TOKENS = 512, FEW_SPAN = 8;
 
-// Of eight tokens from t0 on, those whose slot is a page's last.
-__device__ __forceinline__ unsigned page_ends(const Append& p, int t0, int T, int& slot) {
-  const int lane = threadIdx.x & 31, t = t0 + (lane & 7);
-  slot = t < T ? p.slots[t] : -1;
-  return __ballot_sync(0xffffffffu, lane < 8 && slot >= 0 && slot % p.page_size == p.page_size - 1 && slot / p.page_size < p.num_pages);
+// Of `span` tokens from t0 on (32 at most), those whose slot is a page's last.
+__device__ __forceinline__ unsigned page_ends(const Append& p, int t0, int T, int span, int& slot) {
+  const int t = t0 + (threadIdx.x & 31);
+  slot = t < T && t < t0 + span ? p.slots[t] : -1;
+  return __ballot_sync(0xffffffffu, slot >= 0 && slot % p.page_size == p.page_size - 1 && slot / p.page_size < p.num_pages);
 }
 
-// The means of key head g of the pages that the eight tokens from t0 on fill, by a block: its warps' groups of lanes take the offsets
+// The means of key head g of the pages that a span of tokens from t0 on fills, by a block: its warps' groups of lanes take the offsets
 // in turn and come together in an order that depends on nothing but the page size.  ROWS: keys that this step brings are made again from
 // its rows; else all come from the cache (behind the launch that wrote them).
 template <typename TA, typename TW, int D, bool ROWS>
@@ -203,7 +212,7 @@ __device__ __forceinline__ void make_means(const TA* qkv, const TW* k_weight, co
   __shared__ float s_sum[WARPS][D];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, side = lane / LANES;
   int slots;
-  unsigned ends = page_ends(p, t0, T, slots);
+  unsigned ends = page_ends(p, t0, T, ROWS ? FEW_SPAN : 32, slots);
   if (!ends) return;
   const Place at = place_of(p, l);
   const bool norm = k_weight != nullptr;
@@ -270,7 +279,7 @@ template <typename TA, int D>
 __global__ void __launch_bounds__(WARPS * 32)
 page_means_kernel(const TA* __restrict__ cache, TA* __restrict__ means, int T, const Append p) {
   pdl_enter();
-  make_means<TA, TA, D, false>(nullptr, nullptr, cache, means, blockIdx.x * 8, blockIdx.y, T, p);
+  make_means<TA, TA, D, false>(nullptr, nullptr, cache, means, blockIdx.x * 32, blockIdx.y, T, p);
 }
 
 // WPT: warps that share a token's heads.  MEANS: the first `mean_blocks` blocks make the means, from this step's rows and the cache.
@@ -287,7 +296,7 @@ append_lanes_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW
   const Place at = place_of(p, l);
   float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
   if (MEANS && (int)blockIdx.x < mean_blocks) {
-    make_means<TA, TW, D, true>(qkv, k_weight, cache, means, blockIdx.x / p.Hkv * 8, blockIdx.x % p.Hkv, T, p);
+    make_means<TA, TW, D, true>(qkv, k_weight, cache, means, blockIdx.x / p.Hkv * FEW_SPAN, blockIdx.x % p.Hkv, T, p);
     return;
   }
   const int t = ((int)blockIdx.x - mean_blocks) * (WARPS / WPT) + warp / WPT;
@@ -295,36 +304,45 @@ append_lanes_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW
   // everything that waits for nothing goes out first: slot, position, the first heads, the weights; then the angles
   const int slot = p.slots[t], pos = p.rot ? p.positions[t] : 0;
   const int heads = p.H + 2 * p.Hkv;
-  const TA* row = qkv + (int64_t)t * p.ld;
   const int first = warp % WPT * PER + side;
+  constexpr int STEP = WPT * PER;                              // heads from one of a lane's to the next
+  const TA* src = qkv + (int64_t)t * p.ld + first * D;
   Lane8<TA> in[AHEAD];
   auto load = [&](int h0) {
+    if (h0 - side + (AHEAD - 1) * STEP + PER <= heads) {
 #pragma unroll
-    for (int u = 0; u < AHEAD; ++u)                            // (no branch between the loads)
-      in[u] = load_lane<TA>(row + min(h0 + u * WPT * PER, heads - 1) * D, at.a, at.b);
+      for (int u = 0; u < AHEAD; ++u) in[u] = load_lane<TA>(src + u * STEP * D, at.a, at.b);
+    } else {
+#pragma unroll
+      for (int u = 0; u < AHEAD; ++u)                          // (no branch between the loads)
+        in[u] = load_lane<TA>(src + (min(h0 + u * STEP, heads - 1) - h0) * D, at.a, at.b);
+    }
+    src += AHEAD * STEP * D;
   };
   load(first);
-  Lane8<TW> wq, wk;
-  if (norm) {
-    wq = load_lane<TW>(q_weight, at.a, at.b);
-    wk = load_lane<TW>(k_weight, at.a, at.b);
-  }
+  float w[8];
+  if (norm) widen<TW>(load_lane<TW>(first < p.H ? q_weight : k_weight, at.a, at.b), w);
   if (p.rot) load_turn(p.cos_sin + (int64_t)(pos >= 0 && pos < p.table_rows ? pos : 0) * p.rot, at, p.rot, l, c, s);
   const int page = slot / p.page_size, off = slot - page * p.page_size;
   const bool kept = slot >= 0 && page < p.num_pages;
   TA* q_row = q_out + (int64_t)t * p.ldq;
   TA* c_row = cache + (kept ? (int64_t)page * 2 * plane + (int64_t)off * D : 0);
   const int head_step = p.page_size * D;                       // (the values follow the keys as key heads Hkv on)
-  for (int h0 = first; h0 - side < heads; h0 += WPT * PER * AHEAD) {
+  bool keys = first >= p.H;                                    // whose weights w holds
+  for (int h0 = first; h0 - side < heads; h0 += STEP * AHEAD) {
     if (h0 != first) load(h0);
 #pragma unroll
     for (int u = 0; u < AHEAD; ++u) {
-      const int head = h0 + u * WPT * PER;
+      const int head = h0 + u * STEP;
       if (head - side >= heads) break;                         // (the whole warp alike)
       if (head - side < p.H + p.Hkv) {                         // values are left as they are
-        float v[8], w[8];
+        if (norm && !keys && head >= p.H) {
+          keys = true;
+          widen<TW>(load_lane<TW>(k_weight, at.a, at.b), w);
+        }
+        __syncwarp();
+        float v[8];
         widen<TA>(in[u], v);
-        if (norm) widen<TW>(head < p.H ? wq : wk, w);
         finish<LANES>(v, norm, w, p.eps, at, c, s);
         if (head < p.H + p.Hkv) in[u] = narrow<TA>(v);
       }
@@ -341,15 +359,15 @@ int run(const void* qkv, void* q_out, const void* qw, const void* kw, void* cach
                        p.ld % 8 == 0 && p.ldq % 8 == 0;
   if (aligned && (p.D == 64 || p.D == 128) && p.page_size <= MAX_PAGE && p.rot % 8 == 0 && p.Hkv <= 65535) {
     // few tokens: a block each, so that a token's heads are all under way at once; many: a warp's start (slot, angles, weights) is
-    // paid for a quarter of a token's heads
+    // paid for half of a token's heads
     const bool few = T <= FEW_TOKENS;
     auto kernel = few ? (p.D == 64 ? append_lanes_kernel<TA, TW, 64, 8, true> : append_lanes_kernel<TA, TW, 128, 8, true>)
-                      : (p.D == 64 ? append_lanes_kernel<TA, TW, 64, 4, false> : append_lanes_kernel<TA, TW, 128, 4, false>);
-    const int mean_blocks = few ? (T + 7) / 8 * p.Hkv : 0, per = few ? 1 : WARPS / 4;
+                      : (p.D == 64 ? append_lanes_kernel<TA, TW, 64, 2, false> : append_lanes_kernel<TA, TW, 128, 2, false>);
+    const int mean_blocks = few ? (T + FEW_SPAN - 1) / FEW_SPAN * p.Hkv : 0, per = few ? 1 : WARPS / 2;
     launch_pdl(kernel, dim3(mean_blocks + (T + per - 1) / per), dim3(WARPS * 32), 0, stream, (const TA*)qkv, (TA*)q_out, (const TW*)qw,
                (const TW*)kw, (TA*)cache, (TA*)means, T, mean_blocks, p);
     if (!few)
-      launch_pdl(p.D == 64 ? page_means_kernel<TA, 64> : page_means_kernel<TA, 128>, dim3((T + 7) / 8, p.Hkv), dim3(WARPS * 32), 0, stream,
+      launch_pdl(p.D == 64 ? page_means_kernel<TA, 64> : page_means_kernel<TA, 128>, dim3((T + 31) / 32, p.Hkv), dim3(WARPS * 32), 0, stream,
                  (const TA*)cache, (TA*)means, T, p);
     return cuda_status("page_append");
   }

@@ -101,10 +101,12 @@ def _ints(what: str, names: str, *tensors) -> None:
 
 def _batch(what: str, T: int, block_table, cu_seqlens, positions):
     """(requests, table width)"""
-    _ints(what, "block_table, cu_seqlens and positions", block_table, cu_seqlens, positions)
     shape = block_table.shape
-    if len(shape) != 2 or cu_seqlens.dim() != 1 or cu_seqlens.numel() != shape[0] + 1 or positions.numel() != T or shape[0] == 0:
+    if len(shape) != 2 or cu_seqlens.shape != (shape[0] + 1,) or positions.numel() != T or shape[0] == 0:
         raise KernelError(f"{what}: block_table [B, width] with B > 0, cu_seqlens [B + 1], positions [T]")
+    if block_table.dtype != _I32 or cu_seqlens.dtype != _I32 or positions.dtype != _I32 or not block_table.is_contiguous() \
+            or not cu_seqlens.is_contiguous() or not positions.is_contiguous():
+        raise KernelError(f"{what}: block_table, cu_seqlens and positions must be contiguous int32")
     return shape
 
 
@@ -202,7 +204,7 @@ def page_scores(q: torch.Tensor, means: torch.Tensor, block_table: torch.Tensor,
     if not 0 <= pages <= width or page_size <= 0:
         raise KernelError(f"{what}: {pages} pages of {page_size} tokens, the table holds {width}")
     if out is None:
-        out = torch.empty((T, Hkv, pages), dtype=_F32, device=q.device)
+        out = torch.empty(T, Hkv, pages, dtype=_F32, device=q.device)
         ldt, ldg = Hkv * pages, pages
     else:
         if out.dtype != _F32 or out.shape != (T, Hkv, pages) or (pages > 1 and out.stride(2) != 1):
@@ -233,7 +235,7 @@ def choose_pages(scores: torch.Tensor, positions: torch.Tensor, page_size: int, 
     if page_size <= 0 or first < 0 or recent < 1 or top < first + recent:
         raise KernelError(f"{what}: {first} first and {recent} recent pages of {top}, pages of {page_size} tokens")
     if out is None:
-        out = torch.empty((T, Hkv, top), dtype=_I32, device=scores.device)
+        out = torch.empty(T, Hkv, top, dtype=_I32, device=scores.device)
     elif out.dtype != _I32 or out.shape != (T, Hkv, top) or not out.is_contiguous():
         raise KernelError(f"{what}: out int32 [T, Hkv, top], contiguous")
     _call("page_choice", "dinfer_choose_pages", what, scores.data_ptr(), stride[0], stride[1], positions.data_ptr(), page_size, first,
