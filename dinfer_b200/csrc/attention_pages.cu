@@ -124,8 +124,8 @@ constexpr int F_TOKENS = 4, F_NT = F_TOKENS * 64, F_KEYS = 32, F_PICKS = 1024, F
 template <int D, int G>              // G: at least the group
 __global__ void __launch_bounds__(F_NT, G > 4 ? 2 : 3)
 pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const float* __restrict__ cache, const Pages p) {
-  extern __shared__ __align__(16) unsigned char smem_raw[];
-  float* sK = reinterpret_cast<float*>(smem_raw);          // [F_STAGES][F_KEYS][D], 16-byte pieces exchanged by key & 7: eight rows' in different banks
+  extern __shared__ __align__(16) unsigned char smem_float[];
+  float* sK = reinterpret_cast<float*>(smem_float);          // [F_STAGES][F_KEYS][D], 16-byte pieces exchanged by key & 7: eight rows' in different banks
   float* sV = sK + F_STAGES * F_KEYS * D;                  // [F_STAGES][F_KEYS][D]
   float* sQ = sV + F_STAGES * F_KEYS * D;                       // [F_TOKENS][group][D]
   // (page, token), sorted; all ones: none

@@ -323,11 +323,11 @@ int run_scores_umma(const __nv_bfloat16* q, int64_t ldq, const __nv_bfloat16* me
   return cuda_status("page_scores (many tokens)");
 }
 
-// Scores as whole numbers of the same order; 0 for what is not a number, 1 for -inf.
+// Scores as whole numbers of the same order, the lowest for what is not a number; none is 0.
 __device__ __forceinline__ unsigned order_of(float s) {
   const int b = __float_as_int(s + 0.f);                      // -0 counts as 0
-  const unsigned k = (unsigned)(b ^ ((b >> 31) | (int)0x80000000)) - 0x007ffffeu;
-  return s == s ? k : 0u;
+  const unsigned k = (unsigned)(b ^ ((b >> 31) | (int)0x80000000));
+  return s == s ? k : 1u;
 }
 
 // Any sizes: a warp per (token, key head), the best of the rest again and again.
@@ -378,11 +378,11 @@ choose_pages_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
   for (int i = at + lane; i < top; i += 32) dst[i] = -1;
 }
 
-// Up to 2048 pages: a warp per (token, key head) with the candidates' orders in registers (page lo + 32 i + lane), read once.
-// First a bound that few more candidates reach than there are picks, to the upper 16 bits: up to 32 picks by the lanes' own maxima
-// (as many lanes as picks reach it), else counted over all.  The candidates that reach it go to a list in shared memory in ascending
-// order and are ranked against one another; a pick's place among the picks is its place in the list.  Where too many reach the bound
-// (equal scores) the order of the last pick is found bit by bit, and of the candidates of that order the lowest are taken.
+// Up to 2048 pages: a warp per (token, key head), the candidates' orders in registers (page lo + 32 i + lane; 0: none), read once.
+// First a bound that few more candidates reach than there are picks, to the upper bits: up to 32 picks by the lanes' own maxima (as
+// many lanes as picks reach it), else counted over all.  The candidates that reach it go to a list in shared memory, ascending, and are
+// ranked against one another; a pick's place among the picks is its place in the list.  Where too many reach the bound (equal
+// scores) the order of the last pick is found bit by bit, and of the candidates of that order the lowest are taken.
 // Bound by instructions: @CHOOSE@
 constexpr int SHORT_LIST = 64;
 
@@ -390,13 +390,12 @@ template <int NPL>
 __global__ void __launch_bounds__(WARPS * 32)
 choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, const int* __restrict__ positions, int page_size,
                         int first, int recent, int top, int pages, int* __restrict__ out, int rows, int Hkv) {
-  __shared__ __align__(16) unsigned s_key[WARPS][SHORT_LIST];
-  __shared__ int s_page[WARPS][SHORT_LIST];
+  __shared__ __align__(16) uint2 s_list[WARPS][SHORT_LIST + 2];   // (order, page)
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int row = blockIdx.x * WARPS + warp;
   if (row >= rows) return;
-  const int t = row / Hkv, g = row % Hkv;
+  const int t = row / Hkv, g = row - t * Hkv;
   const int pos = positions[t];
   const int own = pos < 0 ? -1 : min(pos / page_size, pages - 1);
   const int lo = min(first, own + 1), hi = max(own + 1 - recent, lo);   // candidates are [lo, hi)
@@ -410,18 +409,19 @@ choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t l
     at = hi;
   } else if (picks > 0) {
     const float* s = scores + (int64_t)t * ldt + (int64_t)g * ldg + lo + lane;
-    unsigned key[NPL], best = 0;                             // 0: no candidate
+    const int n_mine = hi - lo - lane;                       // this lane's candidates are 32 i < n_mine
+    unsigned key[NPL], best = 0;
 #pragma unroll
-    for (int i = 0; i < NPL; ++i) key[i] = __float_as_uint(lo + 32 * i + lane < hi ? s[32 * i] : 0.f);
+    for (int i = 0; i < NPL; ++i) key[i] = __float_as_uint(32 * i < n_mine ? s[32 * i] : 0.f);
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      key[i] = lo + 32 * i + lane < hi ? order_of(__uint_as_float(key[i])) + 1u : 0u;
+      key[i] = 32 * i < n_mine ? order_of(__uint_as_float(key[i])) : 0u;
       best = max(best, key[i]);
     }
     unsigned bound = 0;
     if (picks <= 32) {
 #pragma unroll
-      for (int bit = 31; bit >= 16; --bit) {
+      for (int bit = 31; bit >= 18; --bit) {
         const unsigned tried = bound | (1u << bit);
         if (__popc(__ballot_sync(0xffffffffu, best >= tried)) >= picks) bound = tried;
       }
@@ -437,31 +437,31 @@ choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t l
     }
     bound = max(bound, 1u);
     int n = 0;
+    uint2* list = s_list[warp];
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
-      const unsigned in = __ballot_sync(0xffffffffu, key[i] >= bound);
-      if (in) {
-        const int k = n + __popc(in & below);
-        if (key[i] >= bound && k < SHORT_LIST) { s_key[warp][k] = key[i]; s_page[warp][k] = lo + 32 * i + lane; }
-        n += __popc(in);
-      }
+      const bool mine = key[i] >= bound;
+      const unsigned in = __ballot_sync(0xffffffffu, mine);
+      const int k = n + __popc(in & below);
+      if (mine && k < SHORT_LIST) list[k] = make_uint2(key[i], (unsigned)(lo + 32 * i + lane));
+      n += __popc(in);
     }
     if (n <= SHORT_LIST) {
-      if (lane < (-n & 3)) s_key[warp][n + lane] = 0;
+      if (lane == 0) list[n] = make_uint2(0u, 0u);
       __syncwarp();
 #pragma unroll
       for (int half = 0; half < 2; ++half) {
         const int me = lane + 32 * half;
         if (32 * half >= n) break;
-        const unsigned a = me < n ? s_key[warp][me] : 0u;
+        const uint2 a = me < n ? list[me] : make_uint2(0u, 0u);
         int above = 0;                                       // larger ones, and equal ones lower down
-        for (int i = 0; i < n; i += 4) {
-          const uint4 v = *reinterpret_cast<const uint4*>(&s_key[warp][i]);
-          above += (v.x > a - (i < me)) + (v.y > a - (i + 1 < me)) + (v.z > a - (i + 2 < me)) + (v.w > a - (i + 3 < me));
+        for (int i = 0; i < n; i += 2) {
+          const uint4 v = *reinterpret_cast<const uint4*>(list + i);
+          above += (v.x > a.x - (i < me)) + (v.z > a.x - (i + 1 < me));
         }
         const bool in = me < n && above < picks;
         const unsigned mask = __ballot_sync(0xffffffffu, in);
-        if (in) dst[at + __popc(mask & below)] = s_page[warp][me];
+        if (in) dst[at + __popc(mask & below)] = (int)a.y;
         at += __popc(mask);
       }
     } else {
@@ -536,7 +536,7 @@ choose_block_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
 #pragma unroll
     for (int i = 0; i < NPL; ++i) {
       const int j = lo + i * WARPS * 32 + threadIdx.x;
-      key[i] = j < hi ? order_of(s[j]) + 1u : 0u;
+      key[i] = j < hi ? order_of(s[j]) : 0u;
     }
     unsigned last = 0;
 #pragma unroll 1
