@@ -8,7 +8,7 @@
 // bit per token that says whether it did.  The block then walks that list as the attention over a whole context walks its keys:
 //     S[128, 64]  = Q K^T          tcgen05.mma, Q and K K-major in shared memory, S in tensor memory (two buffers)
 //     P = softmax step             one thread per row (= TMEM lane): tcgen05.ld, keys of pages that the row's token did not choose
-//                                  (or that lie behind it) to -inf, exp2, P -> shared memory (bfloat16)
+//                                  (or that lie behind it) to -inf, exp2, P as bfloat16 over the columns of its S
 //     O[128, D]  += P V            tcgen05.mma accumulating in tensor memory; O is rescaled in place only when a row's maximum grows
 //                                  by more than 2^8
 // A page is read once for the 256 rows, not once for each token that chose it.  A warp none of whose rows sees a tile passes it with zeros.
@@ -34,7 +34,7 @@ using namespace dinfer_umma;
 
 namespace {
 
-constexpr int BM = 128, BN = 64, STAGES = 3, NTHREADS = 384;    // BM rows of a row tile, two row tiles a block
+constexpr int BM = 128, BN = 64, STAGES = 4, NTHREADS = 384;    // BM rows of a row tile, two row tiles a block
 constexpr int MMA_WARP_B = 10, V_WARP = 11;                     // the second MMA issuer, the V producer
 constexpr int LIST_SLOTS = 1024;                                // entries of a list in shared memory (fewer where a row tile has more than 32 tokens)
 constexpr int TWICE = 1 << 30;                                  // in a list's count: some token names a page twice
@@ -201,8 +201,10 @@ __device__ __noinline__ void rows_again(const Params& p, int request, int first,
 }
 
 template <int D> constexpr size_t smem_bytes() {
-  return (size_t)(2 * BM * D * 2 + 2 * STAGES * BN * D * 2 + 2 * BM * BN * 2) + 1024;
+  return (size_t)(2 * BM * D * 2 + 2 * STAGES * BN * D * 2) + 1024;
 }
+
+__device__ __forceinline__ uint64_t pair_f32(float lo, float hi) { return (uint64_t)__float_as_uint(hi) << 32 | __float_as_uint(lo); }
 
 // NP: entries of a key tile
 template <int D, int NP>
@@ -210,11 +212,11 @@ __global__ void __launch_bounds__(NTHREADS, 1)
 attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __grid_constant__ CUtensorMap map_kv, const Params p) {
   constexpr int NH = D / 64;                          // 64-wide halves of the head
   constexpr uint32_t Q_HALF = BM * 128, KV_HALF = BN * 128;
-  constexpr uint32_t Q_BYTES = NH * Q_HALF, KV_BYTES = NH * KV_HALF, P_BYTES = BM * BN * 2;
+  constexpr uint32_t Q_BYTES = NH * Q_HALF, KV_BYTES = NH * KV_HALF;
   constexpr int TMEM_COLS = 512, O_COL = 256;         // S of (row tile w, buffer b) at (2w + b) * 64; O of A 256, of B 384
   extern __shared__ unsigned char smem_dyn[];
   __shared__ __align__(8) uint64_t q_full, k_full[STAGES], k_empty[STAGES], v_full[STAGES], v_empty[STAGES],
-      s_full[2][2], p_full[2], pv_done[2], o_full[2];
+      s_full[2][2], p_full[2][2], pv_done[2], o_full[2];
   __shared__ uint32_t s_tmem_base;
   __shared__ int s_abort, s_odd;
   __shared__ int s_first[LIST_SLOTS];                  // the list's beginning: first positions and bits
@@ -234,7 +236,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   const bool b_on = pair.z > p.tile_tokens;            // the second row tile exists
 
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
-  const uint32_t sQ = base, sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES, sP = sV + STAGES * KV_BYTES;
+  const uint32_t sQ = base, sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES;
   {
     // zeroed K/V stages: an entry that is no page leaves its slot as it was, and it must hold finite numbers
     uint4* z = reinterpret_cast<uint4*>(smem_dyn + (sK - smem_u32(smem_dyn)));
@@ -254,7 +256,8 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     for (int w = 0; w < 2; ++w) {
       mbar_init(smem_u32(&s_full[w][0]), 1);
       mbar_init(smem_u32(&s_full[w][1]), 1);
-      mbar_init(smem_u32(&p_full[w]), 128);
+      mbar_init(smem_u32(&p_full[w][0]), 4);               // an arrival a warp; one for each buffer, since a warp may be a tile ahead
+      mbar_init(smem_u32(&p_full[w][1]), 4);
       mbar_init(smem_u32(&pv_done[w]), 1);
       mbar_init(smem_u32(&o_full[w]), 1);
     }
@@ -315,7 +318,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const bool on = w == 0 || b_on;
       constexpr uint32_t idesc_qk = idesc_bf16(BM, BN, 0), idesc_pv = idesc_bf16(BM, D, 1);
       const uint64_t dq = desc_k_major(sQ + w * Q_BYTES), dk = desc_k_major(sK);
-      const uint64_t dp = desc_k_major(sP + w * P_BYTES), dv = desc_mn_major(sV, KV_HALF);
+      const uint64_t dv = desc_mn_major(sV, KV_HALF);
       const uint32_t o_tmem = tmem + O_COL + w * 128;
       auto issue_qk = [&](int t) {                                  // S_w[t % 2] = Q_w K(t)^T
         const uint64_t dks = dk + (uint64_t)((t % STAGES) * (KV_BYTES >> 4));
@@ -326,11 +329,12 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
                  dks + (uint64_t)(((k / 4) * KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
         tc_commit(smem_u32(&s_full[w][t & 1]));
       };
-      auto issue_pv = [&](int s, int j) {
+      auto issue_pv = [&](int s, int j) {                           // O_w += P_w V(j), P from the columns of S_w[j % 2]
+        const uint32_t p_tmem = tmem + (2 * w + (j & 1)) * BN;
         const uint64_t dvs = dv + (uint64_t)(s * (KV_BYTES >> 4));
 #pragma unroll
         for (int k = 0; k < BN / 16; ++k)
-          tc_mma(o_tmem, dp + (uint64_t)(k * 2), dvs + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+          tc_mma_ts(o_tmem, p_tmem + k * 8, dvs + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
       };
       bool ok = true;
       if (on && !mbar_wait(smem_u32(&q_full), 0)) { s_abort = 1; atomicExch(p.status, 62); ok = false; }
@@ -347,12 +351,12 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       for (int t = 0; t < 2 && t < n_tiles && ok; ++t) take_k(t);
       for (int j = 0; j < n_tiles && ok; ++j) {
         const int s = j % STAGES;
-        if (on && !mbar_spin(smem_u32(&p_full[w]), j & 1)) { s_abort = 1; atomicExch(p.status, 64); ok = false; break; }
+        if (on && !mbar_spin(smem_u32(&p_full[w][j & 1]), (j >> 1) & 1)) { s_abort = 1; atomicExch(p.status, 64); ok = false; break; }
         if (!mbar_wait(smem_u32(&v_full[s]), (j / STAGES) & 1)) { s_abort = 1; atomicExch(p.status, 63); ok = false; break; }
         if (on) {
           tc_fence_after();
           issue_pv(s, j);
-          tc_commit(smem_u32(&pv_done[w]));                         // P_w is free again, O_w is quiet until the next P V
+          tc_commit(smem_u32(&pv_done[w]));                         // O_w is quiet until the next P V
           if (j + 1 == n_tiles) tc_commit(smem_u32(&o_full[w]));     // this row tile's last P V
           tc_commit(smem_u32(&v_empty[s]));
         } else {
@@ -372,7 +376,6 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const int n_w = w == 0 || b_on ? n_tiles : 0;
     const uint32_t lane_addr = tmem + ((uint32_t)(quarter * 32) << 16);
     const uint32_t s_addr = lane_addr + 2 * w * BN, o_addr = lane_addr + O_COL + w * 128;
-    unsigned char* prow = smem_dyn + (sP - smem_u32(smem_dyn)) + w * P_BYTES + r * 128;
     float m_run = -INFINITY, l_run = 0.f;                           // reference maximum (scaled, log2 units), running sum
     bool ok = true;
     const int my_word = w * p.words + (row_ok ? token >> 5 : 0), my_bit = token & 31, bits = 2 * p.words;
@@ -389,6 +392,13 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         seen[x] = row_ok && (word >> my_bit & 1) ? max(0, min(UNIT, pos - first + 1)) : 0;
       }
     };
+    // the weights are in tensor memory before a warp's lane says so
+    auto hand_over = [&](int j) {
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&p_full[w][j & 1]));
+    };
     if (n_w > 0) look(0);
     for (int j = 0; j < n_w; ++j) {
       if (!mbar_wait(smem_u32(&s_full[w][j & 1]), (j >> 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
@@ -400,12 +410,12 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         part |= seen[x] > 0 && seen[x] < UNIT;
       }
       if (!__any_sync(0xffffffffu, some)) {                         // nothing here for the warp's rows: weights of zero
-        if (j > 0 && !mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
+        uint32_t zero[16];
 #pragma unroll
-        for (int c = 0; c < 8; ++c) *reinterpret_cast<uint4*>(prow + (c << 4)) = make_uint4(0, 0, 0, 0);
-        tc_fence_before();
-        asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-        mbar_arrive(smem_u32(&p_full[w]));
+        for (int i = 0; i < 16; ++i) zero[i] = 0;
+        tmem_st16(s_addr + (j & 1) * BN, zero);
+        tmem_st16(s_addr + (j & 1) * BN + 16, zero);
+        hand_over(j);
         if (j + 1 < n_w) look(j + 1);
         continue;
       }
@@ -437,12 +447,10 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       mx *= p.scale_log2;
       // raise the reference maximum only when it grows by more than 8 (in log2 units)
       const bool raise = mx > m_run + 8.f;
-      bool pv_seen = j == 0;                                        // P V of tile j-1 known to be complete
       if (j > 0 && __any_sync(0xffffffffu, raise)) {
-        // O_w must be quiet: P V of tile j-1 complete (P V of tile j waits for our P)
+        // O_w must be quiet: P V of tile j-1 complete (P V of tile j waits for our P, and S of tile j came behind P V of tile j-2)
         if (!mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
         tc_fence_after();
-        pv_seen = true;
         const float alpha = raise ? fast_exp2(m_run - mx) : 1.f;     // m_run = -inf gives 0
         l_run *= alpha;
 #pragma unroll
@@ -460,36 +468,28 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       const float neg_m = m_run == -INFINITY ? 0.f : -m_run;
       // 2^(s * scale - m); of an entry that the row does not see 2^-inf = 0 (a score there that is not a finite number makes the row's
       // sums one that is not, and the block's rows are made again)
-      float sq[8];                                                  // eight partial sums: short dependency chains
-#pragma unroll
-      for (int i = 0; i < 8; ++i) sq[i] = 0.f;
+      uint32_t pw[BN / 2];                                          // P: 64 keys = 32 columns
+      uint64_t sq[4] = {};                                          // eight partial sums: short dependency chains
+      const uint64_t scale2 = pair_f32(p.scale_log2, p.scale_log2);
 #pragma unroll
       for (int x = 0; x < NP; ++x) {
         const float neg = seen[x] > 0 ? neg_m : -INFINITY;
+        const uint64_t neg2 = pair_f32(neg, neg);
 #pragma unroll
-        for (int i = x * UNIT; i < (x + 1) * UNIT; ++i) {
-          s0[i] = fast_exp2(fmaf(s0[i], p.scale_log2, neg));
-          sq[i & 7] += s0[i];
+        for (int i = x * UNIT; i < (x + 1) * UNIT; i += 2) {
+          uint64_t e;
+          asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(pair_f32(s0[i], s0[i + 1])), "l"(scale2), "l"(neg2));
+          const float lo = fast_exp2(__uint_as_float((unsigned)e)), hi = fast_exp2(__uint_as_float((unsigned)(e >> 32)));
+          asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sq[i / 2 & 3]) : "l"(pair_f32(lo, hi)));
+          pw[i / 2] = pack_bf16(lo, hi);                            // (2^-9 of each weight; their sum is of the weights before)
         }
       }
-      l_run += ((sq[0] + sq[1]) + (sq[2] + sq[3])) + ((sq[4] + sq[5]) + (sq[6] + sq[7]));
-      // the P V of tile j-1 must have read P before it is overwritten
-      if (!pv_seen) {
-        if (!mbar_wait(smem_u32(&pv_done[w]), (j - 1) & 1)) { s_abort = 1; atomicExch(p.status, 65); ok = false; break; }
-      }
-      // P row r: 64 keys = 8 chunks of 16 bytes, swizzled like a K-major tile with 128-byte rows (rounded to bfloat16: 2^-9 of each
-      // weight; their sum is taken before)
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        const float* src = s0 + c * 8;
-        uint4 v;
-        v.x = pack_bf16(src[0], src[1]); v.y = pack_bf16(src[2], src[3]);
-        v.z = pack_bf16(src[4], src[5]); v.w = pack_bf16(src[6], src[7]);
-        *reinterpret_cast<uint4*>(prow + ((c ^ (r & 7)) << 4)) = v;
-      }
-      tc_fence_before();
-      asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
-      mbar_arrive(smem_u32(&p_full[w]));
+      asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sq[0]) : "l"(sq[1]));
+      asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sq[2]) : "l"(sq[3]));
+      asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sq[0]) : "l"(sq[2]));
+      l_run += __uint_as_float((unsigned)sq[0]) + __uint_as_float((unsigned)(sq[0] >> 32));
+      tmem_st32(s_addr + (j & 1) * BN, reinterpret_cast<const float(&)[32]>(pw));
+      hand_over(j);
       if (j + 1 < n_w) look(j + 1);
     }
     if (ok && n_w > 0) {
@@ -530,8 +530,8 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       }
     } else {
       // The rows are dealt out in runs of 32 (one warp's): block `dest` writes the run out, the others send it their unnormalised O, their
-      // reference maximum and their sum, into the stages and P, which are free once every block's products are complete (the
-      // first barrier).  What a block receives: [sender][4-column group][row of the block's runs] float4.
+      // reference maximum and their sum, into the stages, which are free once every block's products are complete (the first
+      // barrier).  What a block receives: [sender][4-column group][row of the block's runs] float4.
       constexpr int C4 = D / 4;
       const int run = w * 4 + quarter, runs_per = 8 / p.ksplit, dest = run / runs_per, rows_r = runs_per * 32;
       const int rloc = (run % runs_per) * 32 + lane;
@@ -656,7 +656,7 @@ int max_clusters(int ksplit) {
 
 template <int D, int NP>
 int launch(const CUtensorMap& mq, const CUtensorMap& mkv, Params& p, cudaStream_t stream) {
-  static_assert((size_t)2 * STAGES * BN * D * 2 + 2 * BM * BN * 2 >= (size_t)7 * 32 * D * 4, "the stages and P hold what seven senders bring");
+  static_assert((size_t)2 * STAGES * BN * D * 2 >= (size_t)7 * 32 * D * 4, "the stages hold what seven senders bring");
   auto k = attention_pages_umma_kernel<D, NP>;
   constexpr size_t sm = smem_bytes<D>();
   static thread_local int set_for = -1;                    // the attribute belongs to the device
