@@ -27,10 +27,16 @@
 #include <math.h>
 
 #include "common.cuh"
+#include "split_umma.cuh"
 #include "umma_attention.cuh"
 
 using namespace dinfer;
 using namespace dinfer_umma;
+using dinfer_split::commit_if;
+using dinfer_split::elect_lane;
+using dinfer_split::mma_if;
+using dinfer_split::mma_ts_if;
+using dinfer_split::uniform;
 
 namespace {
 
@@ -310,60 +316,63 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       row = next;
     }
   } else if (warp == 1 || warp == MMA_WARP_B) {
-    if (lane == 0) {
-      // ---- MMA issue: one thread per row tile.  Each runs its tile's chain on its own, so neither waits for the other's softmax; the
-      // K and V stages go back to the producers when both have committed (or, without a second row tile, plainly arrived on) their
-      // empty barriers.
-      const int w = warp == 1 ? 0 : 1;
-      const bool on = w == 0 || b_on;
-      constexpr uint32_t idesc_qk = idesc_bf16(BM, BN, 0), idesc_pv = idesc_bf16(BM, D, 1);
-      const uint64_t dq = desc_k_major(sQ + w * Q_BYTES), dk = desc_k_major(sK);
-      const uint64_t dv = desc_mn_major(sV, KV_HALF);
-      const uint32_t o_tmem = tmem + O_COL + w * 128;
-      auto issue_qk = [&](int t) {                                  // S_w[t % 2] = Q_w K(t)^T
-        const uint64_t dks = dk + (uint64_t)((t % STAGES) * (KV_BYTES >> 4));
-        const uint32_t s_tmem = tmem + (2 * w + (t & 1)) * BN;
+    // ---- MMA issue: a warp per row tile, one lane of which issues.  Each runs its tile's chain on its own, so neither waits for the
+    // other's softmax; the K and V stages go back to the producers when both have committed (or, without a second row tile, plainly
+    // arrived on) their empty barriers.
+    const int w = uniform(warp == 1 ? 0 : 1);
+    const bool on = w == 0 || b_on;
+    const uint32_t lead = elect_lane(), tm = uniform(tmem);
+    constexpr uint32_t idesc_qk = idesc_bf16(BM, BN, 0), idesc_pv = idesc_bf16(BM, D, 1);
+    const uint64_t dq = desc_k_major(uniform(sQ + w * Q_BYTES)), dk = desc_k_major(uniform(sK)), dv = desc_mn_major(uniform(sV), KV_HALF);
+    const uint32_t o_tmem = tm + O_COL + w * 128;
+    auto issue_qk = [&](int t) {                                    // S_w[t % 2] = Q_w K(t)^T
+      const uint64_t dks = dk + (uint64_t)((t % STAGES) * (KV_BYTES >> 4));
+      const uint32_t s_tmem = tm + (2 * w + (t & 1)) * BN;
 #pragma unroll
-        for (int k = 0; k < D / 16; ++k)
-          tc_mma(s_tmem, dq + (uint64_t)(((k / 4) * Q_HALF + (k % 4) * 32) >> 4),
-                 dks + (uint64_t)(((k / 4) * KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
-        tc_commit(smem_u32(&s_full[w][t & 1]));
-      };
-      auto issue_pv = [&](int s, int j) {                           // O_w += P_w V(j), P from the columns of S_w[j % 2]
-        const uint32_t p_tmem = tmem + (2 * w + (j & 1)) * BN;
-        const uint64_t dvs = dv + (uint64_t)(s * (KV_BYTES >> 4));
+      for (int k = 0; k < D / 16; ++k)
+        mma_if(lead, s_tmem, dq + (uint64_t)(((k / 4) * Q_HALF + (k % 4) * 32) >> 4),
+               dks + (uint64_t)(((k / 4) * KV_HALF + (k % 4) * 32) >> 4), idesc_qk, k > 0 ? 1u : 0u);
+      commit_if(lead, smem_u32(&s_full[w][t & 1]));
+    };
+    auto issue_pv = [&](int s, int j) {                             // O_w += P_w V(j), P from the columns of S_w[j % 2]
+      const uint32_t p_tmem = tm + (2 * w + (j & 1)) * BN;
+      const uint64_t dvs = dv + (uint64_t)(s * (KV_BYTES >> 4));
 #pragma unroll
-        for (int k = 0; k < BN / 16; ++k)
-          tc_mma_ts(o_tmem, p_tmem + k * 8, dvs + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
-      };
-      bool ok = true;
-      if (on && !mbar_wait(smem_u32(&q_full), 0)) { s_abort = 1; atomicExch(p.status, 62); ok = false; }
-      auto take_k = [&](int t) {                                    // S of key tile t, or the stage handed back once it is full
-        if (!mbar_wait(smem_u32(&k_full[t % STAGES]), (t / STAGES) & 1)) { s_abort = 1; atomicExch(p.status, 63); ok = false; return; }
-        if (on) {
-          tc_fence_after();
-          issue_qk(t);
-          tc_commit(smem_u32(&k_empty[t % STAGES]));
-        } else {
-          mbar_arrive(smem_u32(&k_empty[t % STAGES]));
-        }
-      };
-      for (int t = 0; t < 2 && t < n_tiles && ok; ++t) take_k(t);
-      for (int j = 0; j < n_tiles && ok; ++j) {
-        const int s = j % STAGES;
-        if (on && !mbar_spin(smem_u32(&p_full[w][j & 1]), (j >> 1) & 1)) { s_abort = 1; atomicExch(p.status, 64); ok = false; break; }
-        if (!mbar_wait(smem_u32(&v_full[s]), (j / STAGES) & 1)) { s_abort = 1; atomicExch(p.status, 63); ok = false; break; }
-        if (on) {
-          tc_fence_after();
-          issue_pv(s, j);
-          tc_commit(smem_u32(&pv_done[w]));                         // O_w is quiet until the next P V
-          if (j + 1 == n_tiles) tc_commit(smem_u32(&o_full[w]));     // this row tile's last P V
-          tc_commit(smem_u32(&v_empty[s]));
-        } else {
-          mbar_arrive(smem_u32(&v_empty[s]));
-        }
-        if (j + 2 < n_tiles) take_k(j + 2);                          // into the buffer of S that tile j just left
+      for (int k = 0; k < BN / 16; ++k)
+        mma_ts_if(lead, o_tmem, p_tmem + k * 8, dvs + (uint64_t)((k * 16 * 128) >> 4), idesc_pv, (j > 0 || k > 0) ? 1u : 0u);
+    };
+    bool ok = true;
+    auto fail = [&](int code) {
+      if (lead) { s_abort = 1; atomicExch(p.status, code); }
+      ok = false;
+    };
+    // (the lanes wait each for itself and go on together: what one saw, all saw)
+    if (on && !__all_sync(0xffffffffu, mbar_wait(smem_u32(&q_full), 0))) fail(62);
+    auto take_k = [&](int t) {                                      // S of key tile t, or the stage handed back once it is full
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&k_full[t % STAGES]), (t / STAGES) & 1))) { fail(63); return; }
+      if (on) {
+        tc_fence_after();
+        issue_qk(t);
+        commit_if(lead, smem_u32(&k_empty[t % STAGES]));
+      } else if (lead) {
+        mbar_arrive(smem_u32(&k_empty[t % STAGES]));
       }
+    };
+    for (int t = 0; t < 2 && t < n_tiles && ok; ++t) take_k(t);
+    for (int j = 0; j < n_tiles && ok; ++j) {
+      const int s = j % STAGES;
+      if (on && !__all_sync(0xffffffffu, mbar_spin(smem_u32(&p_full[w][j & 1]), (j >> 1) & 1))) { fail(64); break; }
+      if (!__all_sync(0xffffffffu, mbar_wait(smem_u32(&v_full[s]), (j / STAGES) & 1))) { fail(63); break; }
+      if (on) {
+        tc_fence_after();
+        issue_pv(s, j);
+        commit_if(lead, smem_u32(&pv_done[w]));                     // O_w is quiet until the next P V
+        if (j + 1 == n_tiles) commit_if(lead, smem_u32(&o_full[w]));   // this row tile's last P V
+        commit_if(lead, smem_u32(&v_empty[s]));
+      } else if (lead) {
+        mbar_arrive(smem_u32(&v_empty[s]));
+      }
+      if (j + 2 < n_tiles) take_k(j + 2);                           // into the buffer of S that tile j just left
     }
   } else {                                                          // ---- softmax and output: one thread per row
     const int w = (warp - 2) >> 2;                                  // row tile A (warps 2..5) or B (warps 6..9)
