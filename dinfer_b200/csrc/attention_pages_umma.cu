@@ -230,27 +230,6 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   __shared__ float x_max[2 * BM], x_sum[2 * BM];       // what the other blocks of a cluster found for the rows that this one writes
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = p.ksplit > 1 ? (int)cluster_ctarank() : 0, hk = blockIdx.x / p.ksplit;
-  pdl_enter();
-  const int3 pair = pair_of(p, blockIdx.y);
-  if (pair.x < 0) return;                              // beyond the batch's pairs
-  const int64_t at = (int64_t)blockIdx.y * p.Hkv + hk;
-  // this block's run of the list's key tiles
-  const int count = p.counts[at], all_tiles = (count & ~TWICE) / p.per_tile, per = (all_tiles + p.ksplit - 1) / p.ksplit;
-  const int tile0 = min(rank * per, all_tiles), n_tiles = min(per, all_tiles - tile0);
-  const int2* entries = p.entries + at * p.cap + tile0 * p.per_tile;
-  const unsigned* masks = p.masks + (at * p.cap + tile0 * p.per_tile) * 2 * p.words;
-  const bool b_on = pair.z > p.tile_tokens;            // the second row tile exists
-
-  const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
-  const uint32_t sQ = base, sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES;
-  {
-    // zeroed K/V stages: an entry that is no page leaves its slot as it was, and it must hold finite numbers
-    uint4* z = reinterpret_cast<uint4*>(smem_dyn + (sK - smem_u32(smem_dyn)));
-    for (int i = threadIdx.x; i < (int)(2 * STAGES * KV_BYTES / 16); i += NTHREADS) z[i] = make_uint4(0, 0, 0, 0);
-  }
-  const int held = min(n_tiles * p.per_tile, LIST_SLOTS / p.words);
-  for (int i = threadIdx.x; i < held; i += NTHREADS) s_first[i] = entries[i].y;
-  for (int i = threadIdx.x; i < held * 2 * p.words; i += NTHREADS) s_bits[i] = masks[i];
   if (threadIdx.x == 0) {
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_q) : "memory");
     asm volatile("prefetch.tensormap [%0];" ::"l"(&map_kv) : "memory");
@@ -268,17 +247,49 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       mbar_init(smem_u32(&o_full[w]), 1);
     }
     s_abort = 0;
-    s_odd = count & TWICE ? 1 : 0;
     asm volatile("fence.mbarrier_init.release.cluster;" ::: "memory");
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");
   }
-  if (warp == 1) {
-    asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(TMEM_COLS) : "memory");
-    asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+  pdl_enter();
+  const int3 pair = pair_of(p, blockIdx.y);
+  if (pair.x < 0) return;                              // beyond the batch's pairs
+  const int64_t at = (int64_t)blockIdx.y * p.Hkv + hk;
+  // this block's run of the list's key tiles
+  const int count = p.counts[at], all_tiles = (count & ~TWICE) / p.per_tile, per = (all_tiles + p.ksplit - 1) / p.ksplit;
+  const int tile0 = min(rank * per, all_tiles), n_tiles = min(per, all_tiles - tile0);
+  const int2* entries = p.entries + at * p.cap + tile0 * p.per_tile;
+  const unsigned* masks = p.masks + (at * p.cap + tile0 * p.per_tile) * 2 * p.words;
+  const bool b_on = pair.z > p.tile_tokens;            // the second row tile exists
+
+  const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
+  const uint32_t sQ = base, sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES;
+  if (NP > 1 && n_tiles > 0 && n_tiles <= STAGES) {
+    // the last tile may have entries that are no page, and their slots hold what was there: finite numbers, please (behind the first
+    // tiles those of an earlier one; what is not finite would have the rows made again, for nothing)
+    const uint32_t at0 = (n_tiles - 1) * KV_BYTES;
+    for (int i = threadIdx.x; i < (int)(2 * KV_BYTES / 16); i += NTHREADS) {
+      const uint32_t off = i < (int)(KV_BYTES / 16) ? sK + at0 + i * 16 : sV + at0 + i * 16 - KV_BYTES;
+      *reinterpret_cast<uint4*>(smem_dyn + (off - smem_u32(smem_dyn))) = make_uint4(0, 0, 0, 0);
+    }
+    asm volatile("fence.proxy.async.shared::cta;" ::: "memory");   // before TMA writes the same bytes
+    __syncthreads();
   }
-  asm volatile("fence.proxy.async.shared::cta;" ::: "memory");     // the zero fill above, before TMA writes the same bytes
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
+  const int held = min(n_tiles * p.per_tile, LIST_SLOTS / p.words), bits = 2 * p.words;
+  if (warp == 0) {                                                 // the producer of Q and K needs no more than the barriers it has set up
+    if (lane == 0) s_odd = count & TWICE ? 1 : 0;
+    asm volatile("bar.arrive 1, %0;" ::"n"(NTHREADS) : "memory");
+  } else {
+    if (warp == 1) {
+      asm volatile("tcgen05.alloc.cta_group::1.sync.aligned.shared::cta.b32 [%0], %1;" ::"r"(smem_u32(&s_tmem_base)), "r"(TMEM_COLS) : "memory");
+      asm volatile("tcgen05.relinquish_alloc_permit.cta_group::1.sync.aligned;" ::: "memory");
+    } else {
+      for (int i = threadIdx.x - 64; i < held; i += NTHREADS - 64) s_first[i] = entries[i].y;
+      for (int i = threadIdx.x - 64; i < held * bits; i += NTHREADS - 64) s_bits[i] = masks[i];
+    }
+    tc_fence_before();
+    asm volatile("bar.sync 1, %0;" ::"n"(NTHREADS) : "memory");
+    tc_fence_after();
+  }
   const uint32_t tmem = s_tmem_base;
 
   if (warp == 0 || warp == V_WARP) {
@@ -387,7 +398,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
     const uint32_t s_addr = lane_addr + 2 * w * BN, o_addr = lane_addr + O_COL + w * 128;
     float m_run = -INFINITY, l_run = 0.f;                           // reference maximum (scaled, log2 units), running sum
     bool ok = true;
-    const int my_word = w * p.words + (row_ok ? token >> 5 : 0), my_bit = token & 31, bits = 2 * p.words;
+    const int my_word = w * p.words + (row_ok ? token >> 5 : 0), my_bit = token & 31;
     constexpr int UNIT = BN / NP;
     // the keys of each entry of a tile that this row sees, by its bit and by what is not behind it; made for the next tile
     // when a tile's weights have been handed over
@@ -501,26 +512,37 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       hand_over(j);
       if (j + 1 < n_w) look(j + 1);
     }
-    if (ok && n_w > 0) {
-      if (!mbar_wait(smem_u32(&o_full[w]), 0)) { s_abort = 1; atomicExch(p.status, 66); ok = false; }
+    if (ok) {                                                       // (without a tile Q's rows, which the output goes through, have to be there)
+      if (!mbar_wait(smem_u32(n_w > 0 ? &o_full[w] : &q_full), 0)) { s_abort = 1; atomicExch(p.status, 66); ok = false; }
       tc_fence_after();
     }
     const bool rows_on = w == 0 || b_on;
     bool odd = false;
     __nv_bfloat16* dst = row_ok ? p.out + (int64_t)t * p.ldo + (int64_t)(hk * p.group + r % p.group) * D : nullptr;
-    auto write = [&](float (&o)[32], int c, float l, float inv) {
-      if (!row_ok) return;
+    // a warp's rows go through the shared memory of Q, which is free now, so that neighbouring lanes store neighbouring pieces
+    unsigned char* stage = smem_dyn + (sQ - smem_u32(smem_dyn)) + w * Q_BYTES + quarter * 32 * D * 2;
+    constexpr int ROW16 = D / 8;                                    // 16-byte pieces of a row; piece c of row i lies at c ^ (i & 7)
+    auto keep = [&](float (&o)[32], int c, float l, float inv) {
       if (l == 0.f)                                                 // a row that sees nothing
 #pragma unroll
         for (int i = 0; i < 32; ++i) o[i] = 0.f;
 #pragma unroll
-      for (int i = 0; i < 32; ++i) odd |= !isfinite(o[i]);
+      for (int i = 0; i < 32; ++i) odd |= row_ok && !isfinite(o[i]);
 #pragma unroll
       for (int q4 = 0; q4 < 4; ++q4) {
         uint4 v;
         v.x = pack_bf16(o[q4 * 8] * inv, o[q4 * 8 + 1] * inv); v.y = pack_bf16(o[q4 * 8 + 2] * inv, o[q4 * 8 + 3] * inv);
         v.z = pack_bf16(o[q4 * 8 + 4] * inv, o[q4 * 8 + 5] * inv); v.w = pack_bf16(o[q4 * 8 + 6] * inv, o[q4 * 8 + 7] * inv);
-        reinterpret_cast<uint4*>(dst + c * 32)[q4] = v;
+        *reinterpret_cast<uint4*>(stage + lane * D * 2 + (((c * 4 + q4) ^ (lane & 7)) << 4)) = v;
+      }
+    };
+    auto write = [&]() {
+      __syncwarp();
+#pragma unroll 4
+      for (int i0 = 0; i0 < 32; i0 += 32 / ROW16) {
+        const int i = i0 + lane / ROW16, c = lane % ROW16;
+        __nv_bfloat16* to = reinterpret_cast<__nv_bfloat16*>(__shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(dst), i));
+        if (to) reinterpret_cast<uint4*>(to)[c] = *reinterpret_cast<const uint4*>(stage + i * D * 2 + ((c ^ (i & 7)) << 4));
       }
     };
     if (p.ksplit == 1) {
@@ -534,8 +556,9 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
             tmem_ld32(o_addr + c * 32, o);
             tmem_ld_wait();
           }
-          write(o, c, l_run, inv);
+          keep(o, c, l_run, inv);
         }
+        write();
       }
     } else {
       // The rows are dealt out in runs of 32 (one warp's): block `dest` writes the run out, the others send it their unnormalised O, their
@@ -603,8 +626,9 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
               }
             }
           }
-          write(o, c, l_all, inv);
+          keep(o, c, l_all, inv);
         }
+        write();
       }
     }
     if (odd) s_odd = 1;
