@@ -113,236 +113,192 @@ int run(const void* q, void* out, const void* cache, const Pages& p, cudaStream_
 
 
 // ------------------------------------------------------------------------------------------------
-// 32-bit, head sizes 64 and 128, groups of up to 8 heads: several tokens a request.  Four neighbouring tokens share a block and walk
-// the pages that any of them chose in ascending order (their choices, sorted in shared memory), each page read once for all; two warps own a
-// token, half of a tile's keys each, and pass over the pages it did not choose.  Tiles of up to 32 keys ride a ring of cp.async stages.  A score is the sum of the
-// lanes that share a key's row; for O the lanes split the elements and the keys that the token sees come one by one.  All of it multiply-adds in 32
-// bits.  Bound by shared memory's reads (a key's row once for the group's scores, a value's once for its sums).
-// @FLOAT@
-constexpr int F_TOKENS = 4, F_NT = F_TOKENS * 64, F_KEYS = 32, F_PICKS = 1024, F_STAGES = 2;
+// 32-bit, head sizes 64 and 128, groups of up to 8 heads: a token and key head to a block, or to a cluster of up to eight that share its
+// keys.  The warps take runs of eight keys in turn, straight from memory: a lane holds D / 32 elements of every row, sixteen rows on
+// their way at once.  A run's 8 x G scores are summed over the lanes by exchanging halves (a lane ends with the sums it owns: 31 exchanges
+// for 32 sums instead of 160), the softmax's statistics live with the owner, and the weights go round lane by lane.  The warps, then the
+// blocks of the cluster, come together in shared memory.  Bound by the rows' way from memory: 64 single tokens of 8 key heads, 16
+// pages of 64 keys of 128 (537 MB) take 88 us, 93 % of a copy's rate; a single one 9.5 us, 300 neighbouring ones 230 us (2.5 GB,
+// from L2).  A block that walked the pages of four neighbouring tokens together, each page read once into shared memory for all, took
+// 77, 93 and 338 us there: the products with what lies in shared memory bound it.
+constexpr int L_KEYS = 8;
 
-template <int D, int G>              // G: at least the group
-__global__ void __launch_bounds__(F_NT, G > 4 ? 2 : 3)
-pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const float* __restrict__ cache, const Pages p) {
-  extern __shared__ __align__(16) unsigned char smem_float[];
-  float* sK = reinterpret_cast<float*>(smem_float);          // [F_STAGES][F_KEYS][D], 16-byte pieces exchanged by key & 7: eight rows' in different banks
-  float* sV = sK + F_STAGES * F_KEYS * D;                  // [F_STAGES][F_KEYS][D]
-  float* sQ = sV + F_STAGES * F_KEYS * D;                       // [F_TOKENS][group][D]
-  // (page, token), sorted; all ones: none
-  unsigned long long* s_pick = reinterpret_cast<unsigned long long*>(sQ + F_TOKENS * (p.H / p.Hkv) * D);
-  __shared__ int s_warp[F_NT / 32];
+template <int D, int G>
+__global__ void __launch_bounds__(WARPS * 32, 2)
+pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const float* __restrict__ cache, const Pages p, int splits) {
+  constexpr int E = D / 32, N = L_KEYS * G, OWN = N > 32 ? N / 32 : 1, STEPS = N >= 32 ? 5 : N == 16 ? 4 : 3;
+  struct alignas(E * 4) Vec { float v[E]; };
+  __shared__ float s_acc[WARPS][G][D + 2];
+  __shared__ float c_o[G][D], c_ml[G][2];
   pdl_enter();
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, g = blockIdx.y;
-  const int3 tile = token_tile(p.cu, p.num_reqs, F_TOKENS, blockIdx.x);
-  if (tile.x < 0) return;
-  const int* table = p.table + (int64_t)tile.x * p.width;
-  const int group = p.H / p.Hkv, P = p.page_size, picks = F_TOKENS * p.top;
-  int n2 = 1;                                              // what is sorted: a power of two
-  while (n2 < picks) n2 <<= 1;
-  int2* s_visit = reinterpret_cast<int2*>(s_pick + n2);    // (number in the request, page)
-  unsigned char* s_tokens = reinterpret_cast<unsigned char*>(s_visit + n2);
-  for (int i = threadIdx.x; i < n2; i += F_NT) {
-    const int tl = i / p.top, t = tile.y + tl;
-    unsigned long long key = ~0ull;
-    if (i < picks && tl < tile.z) {
-      const int j = p.chosen[((int64_t)t * p.Hkv + g) * p.top + i - tl * p.top];
-      if (j >= 0 && j < p.width && (int64_t)j * P <= p.positions[t]) key = (unsigned long long)j << 8 | tl;
-    }
-    s_pick[i] = key;
-  }
-  for (int i = threadIdx.x; i < tile.z * group * (D / 4); i += F_NT) {
-    const int row = i / (D / 4), e = i % (D / 4) * 4;      // (token, head)
-    *reinterpret_cast<float4*>(sQ + row * D + e) =
-        *reinterpret_cast<const float4*>(q + (int64_t)(tile.y + row / group) * p.ldq + (int64_t)(g * group + row % group) * D + e);
-  }
-  __syncthreads();
-  for (int k = 2; k <= n2; k <<= 1)                        // a bitonic sort
-    for (int m = k >> 1; m > 0; m >>= 1) {
-      for (int i = threadIdx.x; i < n2; i += F_NT) {
-        const int o = i ^ m;
-        if (o > i) {
-          const unsigned long long a = s_pick[i], b = s_pick[o];
-          if ((a > b) == !(i & k)) { s_pick[i] = b; s_pick[o] = a; }
-        }
-      }
-      __syncthreads();
-    }
-  // Visits: a page with the tokens that chose it (a token that names a page twice begins another visit), in order.
-  const int KT = P < F_KEYS ? P : F_KEYS, per_page = P / KT;
+  const int t = blockIdx.x / splits, split = blockIdx.x - t * splits, group = p.H / p.Hkv, P = p.page_size;
+  const int r = request_of(p.cu, p.num_reqs, t);
+  if (r < 0) return;                                       // (the whole cluster alike)
+  const int* table = p.table + (int64_t)r * p.width;
+  const int* chosen = p.chosen + ((int64_t)t * p.Hkv + g) * p.top;
   const int64_t plane = (int64_t)p.Hkv * P * D;
-  int visits = 0;
-  for (int i0 = 0; i0 < n2; i0 += F_NT) {
-    const int i = i0 + threadIdx.x;
-    const unsigned long long key = i < n2 ? s_pick[i] : ~0ull;
-    const bool begins = key != ~0ull && (i == 0 || s_pick[i - 1] >> 8 != key >> 8 || s_pick[i - 1] == key);
-    int3 v = make_int3((int)(key >> 8), -1, 0);
-    if (begins) {
-      int last = -1;
-      for (int k = i; k < n2 && s_pick[k] >> 8 == key >> 8; ++k) {
-        const int tl = (int)(s_pick[k] & 255);
-        if (tl == last) break;
-        v.z |= 1 << tl;
-        last = tl;
-      }
-      v.y = table[v.x];
-    }
-    const bool in = begins && v.y >= 0 && v.y < p.num_pages;
-    const unsigned ball = __ballot_sync(0xffffffffu, in);
-    if (lane == 0) s_warp[warp] = __popc(ball);
-    __syncthreads();
-    int below = 0, all = 0;
-#pragma unroll
-    for (int w = 0; w < F_NT / 32; ++w) {
-      below += w < warp ? s_warp[w] : 0;
-      all += s_warp[w];
-    }
-    if (in) {
-      const int at = visits + below + __popc(ball & ((1u << lane) - 1));
-      s_visit[at] = make_int2(v.x, v.y);
-      s_tokens[at] = (unsigned char)v.z;
-    }
-    visits += all;
-    __syncthreads();
-  }
-  auto load = [&](const int2& v, int part, int stage) {
-    const float* k = cache + (int64_t)v.y * 2 * plane + ((int64_t)g * P + part * KT) * D;
-    for (int i = threadIdx.x; i < KT * (D / 4); i += F_NT) {
-      const int row = i / (D / 4), e = i % (D / 4) * 4;
-      cp_async16(sK + (stage * F_KEYS + row) * D + (e ^ ((row & 7) << 2)), k + row * D + e, true);
-      cp_async16(sV + (stage * F_KEYS + row) * D + e, k + plane + row * D + e, true);
-    }
-  };
-  const int tl = warp >> 1, half = warp & 1, t = tile.y + tl;
-  const bool live = tl < tile.z;
-  const int pos = live ? p.positions[t] : -1;
-  // a warp's keys: half of the tile's, with as many lanes to a key as that leaves
-  const int keys = KT >> 1, sharing = 32 / keys, key = lane & (keys - 1), share = lane / keys, depth = D / sharing;
-  const float* mine = sQ + tl * group * D + share * depth;
-  constexpr int E = D / 32;                                // elements a lane
-  struct alignas(E * 4) Vec { float v[E]; };
-  float acc[G][E], m[G], l[G];
-#pragma unroll
-  for (int h = 0; h < G; ++h) {
-    m[h] = -INFINITY;
-    l[h] = 0.f;
-#pragma unroll
-    for (int e = 0; e < E; ++e) acc[h][e] = 0.f;
-  }
-  const int tiles = visits * per_page;
-#pragma unroll
-  for (int i = 0; i < F_STAGES - 1; ++i) {
-    if (i < tiles) load(s_visit[i / per_page], i % per_page, i);
-    cp_async_commit();
-  }
-  for (int i0 = 0; i0 < tiles; ++i0) {
-    const int stage = i0 % F_STAGES, ahead = i0 + F_STAGES - 1, part = i0 % per_page;
-    const int2 now = s_visit[i0 / per_page];
-    const unsigned tokens = s_tokens[i0 / per_page];
-    cp_async_wait<F_STAGES - 2>();
-    __syncthreads();                                       // the tile is here, and everyone is done with the one before
-    if (ahead < tiles) load(s_visit[ahead / per_page], ahead % per_page, ahead % F_STAGES);
-    cp_async_commit();
-    const int n = min(keys, pos - now.x * P - part * KT - half * keys + 1);        // of the warp's keys, those that the token sees
-    if (live && (tokens >> tl & 1) && n > 0) {
-      const int row = half * keys + key, swap = (row & 7) << 2;
-      const float *k = sK + (stage * F_KEYS + row) * D, *v = sV + (stage * F_KEYS + half * keys) * D + lane * E;
-      float s[G];
-#pragma unroll
-      for (int h = 0; h < G; ++h) s[h] = 0.f;
-#pragma unroll 8
-      for (int e = 0; e < depth; e += 4) {
-        const float4 x = *reinterpret_cast<const float4*>(k + ((share * depth + e) ^ swap));
-#pragma unroll
-        for (int h = 0; h < G; ++h)
-          if (h < group) {
-            const float4 y = *reinterpret_cast<const float4*>(mine + h * D + e);
-            s[h] = fmaf(x.x, y.x, s[h]); s[h] = fmaf(x.y, y.y, s[h]); s[h] = fmaf(x.z, y.z, s[h]); s[h] = fmaf(x.w, y.w, s[h]);
-          }
-      }
-      for (int o = keys; o < 32; o <<= 1)
-#pragma unroll
-        for (int h = 0; h < G; ++h) s[h] += __shfl_xor_sync(0xffffffffu, s[h], o);
-#pragma unroll
-      for (int h = 0; h < G; ++h)
-        if (h < group) {
-          s[h] = key < n ? s[h] * p.scale : -INFINITY;
-          const float top = fmaxf(m[h], warp_max(s[h])), base = top == -INFINITY ? 0.f : top, alpha = expf(m[h] - base);
-          m[h] = top;
-          s[h] = key < n ? expf(s[h] - base) : 0.f;
-          l[h] = fmaf(l[h], alpha, share == 0 ? s[h] : 0.f);       // (a lane's own keys; the lanes come together at the end)
-#pragma unroll
-          for (int e = 0; e < E; ++e) acc[h][e] *= alpha;
-        }
-      auto add = [&](int i) {
-        const Vec x = *reinterpret_cast<const Vec*>(v + i * D);
-#pragma unroll
-        for (int h = 0; h < G; ++h)
-          if (h < group) {
-            const float w = __shfl_sync(0xffffffffu, s[h], i);
-#pragma unroll
-            for (int e = 0; e < E; ++e) acc[h][e] = fmaf(w, x.v[e], acc[h][e]);
-          }
-      };
-      int i = 0;
-      for (; i + 8 <= n; i += 8)
-#pragma unroll
-        for (int u = 0; u < 8; ++u) add(i + u);
-      for (; i < n; ++i) add(i);
-    }
-  }
-  cp_async_wait<0>();
-  __syncthreads();
-  // the two warps of a token come together in the tiles' memory
-  float* s_acc = sK + tl * G * (D + 2);
-#pragma unroll
-  for (int h = 0; h < G; ++h) l[h] = warp_sum(l[h]);
-  if (half == 1)
-#pragma unroll
-    for (int h = 0; h < G; ++h) {
-#pragma unroll
-      for (int e = 0; e < E; ++e) s_acc[h * (D + 2) + lane * E + e] = acc[h][e];
-      if (lane == 0) { s_acc[h * (D + 2) + D] = m[h]; s_acc[h * (D + 2) + D + 1] = l[h]; }
-    }
-  __syncthreads();
-  if (!live || half == 1) return;
+  const int pos = p.positions[t];
+  Vec x[G];
 #pragma unroll
   for (int h = 0; h < G; ++h)
-    if (h < group) {
-      const float* o = s_acc + h * (D + 2);
-      const float top = fmaxf(m[h], o[D]), base = top == -INFINITY ? 0.f : top, a = expf(m[h] - base), b = expf(o[D] - base);
-      const float sum = l[h] * a + o[D + 1] * b, inv = sum == 0.f ? 0.f : 1.f / sum;
-      Vec x;
+    x[h] = *reinterpret_cast<const Vec*>(q + (int64_t)t * p.ldq + (int64_t)(g * group + min(h, group - 1)) * D + lane * E);
+  float acc[G][E], m[OWN], l[OWN];
 #pragma unroll
-      for (int e = 0; e < E; ++e) x.v[e] = (acc[h][e] * a + o[lane * E + e] * b) * inv;
-      *reinterpret_cast<Vec*>(out + (int64_t)t * p.ldo + (int64_t)(g * group + h) * D + lane * E) = x;
+  for (int h = 0; h < G; ++h)
+#pragma unroll
+    for (int e = 0; e < E; ++e) acc[h][e] = 0.f;
+#pragma unroll
+  for (int o = 0; o < OWN; ++o) { m[o] = -INFINITY; l[o] = 0.f; }
+  // Sum (key i, head h) is number h * 8 + i; what halving by lane bits 16, 8, ... leaves with a lane: its upper STEPS bits, and the OWN last
+  // ones side by side.
+  const int own = N >= 32 ? lane * OWN : lane >> (5 - STEPS);
+  const int key = own % L_KEYS;                            // of the lane's first sum; the heads of all of them are one
+  const int runs = P / L_KEYS;
+  for (int u = split * WARPS + warp; u < p.top * runs; u += splits * WARPS) {
+    const int j = chosen[u / runs], part = u % runs * L_KEYS;
+    if (j < 0 || j >= p.width || (int64_t)j * P + part > pos) continue;
+    const int page = table[j];
+    if (page < 0 || page >= p.num_pages) continue;
+    const int n = min(L_KEYS, pos - j * P - part + 1);     // keys that the token sees
+    const float* rows = cache + (int64_t)page * 2 * plane + ((int64_t)g * P + part) * D + lane * E;
+    Vec k[L_KEYS], v[L_KEYS];
+#pragma unroll
+    for (int i = 0; i < L_KEYS; ++i) k[i] = *reinterpret_cast<const Vec*>(rows + min(i, n - 1) * D);
+#pragma unroll
+    for (int i = 0; i < L_KEYS; ++i) v[i] = *reinterpret_cast<const Vec*>(rows + plane + min(i, n - 1) * D);
+    float s[N];
+#pragma unroll
+    for (int h = 0; h < G; ++h)
+#pragma unroll
+      for (int i = 0; i < L_KEYS; ++i) {
+        float d = 0.f;
+#pragma unroll
+        for (int e = 0; e < E; ++e) d = fmaf(x[h].v[e], k[i].v[e], d);
+        s[h * L_KEYS + i] = d;
+      }
+#pragma unroll
+    for (int step = 0; step < STEPS; ++step) {
+      const int bit = 16 >> step, half = N >> (step + 1);
+      const bool upper = lane & bit;
+#pragma unroll
+      for (int i = 0; i < N / 2; ++i)
+        if (i < half) {
+          const float give = upper ? s[i] : s[i + half], keep = upper ? s[i + half] : s[i];
+          s[i] = keep + __shfl_xor_sync(0xffffffffu, give, bit);
+        }
     }
+#pragma unroll
+    for (int bit = 16 >> STEPS; bit > 0; bit >>= 1) s[0] += __shfl_xor_sync(0xffffffffu, s[0], bit);
+    // softmax of the lane's sums; the eight keys of a head lie in neighbouring lanes
+    float top = -INFINITY;
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      s[o] = key + o < n ? s[o] * p.scale : -INFINITY;
+      top = fmaxf(top, s[o]);
+    }
+#pragma unroll
+    for (int bit = N >= 32 ? 4 / OWN : (1 << (5 - STEPS)) * 4; bit >= (N >= 32 ? 1 : 1 << (5 - STEPS)); bit >>= 1)
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, bit));
+    top = fmaxf(top, m[0]);
+    const float base = top == -INFINITY ? 0.f : top, alpha = expf(m[0] - base);
+#pragma unroll
+    for (int o = 0; o < OWN; ++o) {
+      s[o] = key + o < n ? expf(s[o] - base) : 0.f;
+      l[o] = fmaf(l[o], alpha, s[o]);
+    }
+    m[0] = top;
+#pragma unroll
+    for (int h = 0; h < G; ++h) {
+      const float a = __shfl_sync(0xffffffffu, alpha, N >= 32 ? h * L_KEYS / OWN : (h * L_KEYS) << (5 - STEPS));
+#pragma unroll
+      for (int e = 0; e < E; ++e) acc[h][e] *= a;
+    }
+#pragma unroll
+    for (int i = 0; i < L_KEYS; ++i)
+      if (i < n) {                                         // (a warp alike; what is not seen is not multiplied)
+#pragma unroll
+        for (int h = 0; h < G; ++h) {
+          const int at = h * L_KEYS + i;
+          const float w = __shfl_sync(0xffffffffu, s[N >= 32 ? at % OWN : 0], N >= 32 ? at / OWN : at << (5 - STEPS));
+#pragma unroll
+          for (int e = 0; e < E; ++e) acc[h][e] = fmaf(w, v[i].v[e], acc[h][e]);
+        }
+      }
+  }
+  // a head's sum over its owners: eight keys, lanes that hold the same sum (fewer than 32 sums) counted once
+  float sum = l[0];
+#pragma unroll
+  for (int o = 1; o < OWN; ++o) sum += l[o];
+#pragma unroll
+  for (int bit = N >= 32 ? 4 / OWN : (1 << (5 - STEPS)) * 4; bit >= (N >= 32 ? 1 : 1 << (5 - STEPS)); bit >>= 1)
+    sum += __shfl_xor_sync(0xffffffffu, sum, bit);
+#pragma unroll
+  for (int h = 0; h < G; ++h) {
+    const int src = N >= 32 ? h * L_KEYS / OWN : (h * L_KEYS) << (5 - STEPS);
+    const float m_h = __shfl_sync(0xffffffffu, m[0], src), l_h = __shfl_sync(0xffffffffu, sum, src);
+#pragma unroll
+    for (int e = 0; e < E; ++e) s_acc[warp][h][lane * E + e] = acc[h][e];
+    if (lane == 0) { s_acc[warp][h][D] = m_h; s_acc[warp][h][D + 1] = l_h; }
+  }
+  __syncthreads();
+  float* orow = out + (int64_t)t * p.ldo + (int64_t)g * group * D;
+  for (int idx = threadIdx.x; idx < group * D; idx += WARPS * 32) {
+    const int h = idx / D, d = idx % D;
+    float M = -INFINITY;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) M = fmaxf(M, s_acc[w][h][D]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o = 0.f;
+#pragma unroll
+    for (int w = 0; w < WARPS; ++w) {
+      const float f = expf(s_acc[w][h][D] - base);
+      L = fmaf(s_acc[w][h][D + 1], f, L);
+      o = fmaf(s_acc[w][h][d], f, o);
+    }
+    if (splits == 1) orow[idx] = L == 0.f ? 0.f : o / L;
+    else {
+      c_o[h][d] = o;
+      if (d == 0) { c_ml[h][0] = M; c_ml[h][1] = L; }
+    }
+  }
+  if (splits == 1) return;
+  namespace cg = cooperative_groups;
+  cg::cluster_group cluster = cg::this_cluster();
+  cluster.sync();
+  const int share = (group * D + splits - 1) / splits;
+  for (int idx = split * share + threadIdx.x; idx < min(group * D, (split + 1) * share); idx += WARPS * 32) {
+    const int h = idx / D;
+    float M = -INFINITY;
+    for (int r2 = 0; r2 < splits; ++r2) M = fmaxf(M, cluster.map_shared_rank(&c_ml[0][0], r2)[h * 2]);
+    const float base = M == -INFINITY ? 0.f : M;
+    float L = 0.f, o = 0.f;
+    for (int r2 = 0; r2 < splits; ++r2) {
+      const float* ml = cluster.map_shared_rank(&c_ml[0][0], r2) + h * 2;
+      const float f = expf(ml[0] - base);
+      L = fmaf(ml[1], f, L);
+      o = fmaf(cluster.map_shared_rank(&c_o[0][0], r2)[idx], f, o);
+    }
+    orow[idx] = L == 0.f ? 0.f : o / L;
+  }
+  cluster.sync();                                          // nobody leaves while another reads its memory
 }
 
 template <int D, int G>
-int run_float(const void* q, void* out, const void* cache, const Pages& p, cudaStream_t stream) {
-  const int group = p.H / p.Hkv;
-  int n2 = 1;
-  while (n2 < F_TOKENS * p.top) n2 <<= 1;
-  const size_t smem = (size_t)(2 * F_STAGES * F_KEYS * D + F_TOKENS * group * D) * 4 + (size_t)n2 * 17;
-  auto kernel = pages_float_kernel<D, G>;
-  static thread_local int set_for = -1;                    // the attribute belongs to the device
-  int dev = 0;
-  cudaGetDevice(&dev);
-  if (set_for != dev) {
-    if (cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (2 * F_STAGES * F_KEYS * D + F_TOKENS * G * D) * 4 + F_PICKS * 17) != cudaSuccess)
-      return cuda_status("attention_pages: shared memory");
-    set_for = dev;
-  }
-  const int tiles = p.T / F_TOKENS + (p.num_reqs < p.T ? p.num_reqs : p.T);
-  launch_pdl(kernel, dim3(tiles, p.Hkv), dim3(F_NT), smem, stream, (const float*)q, (float*)out, (const float*)cache, p);
+int run_float(const void* q, void* out, const void* cache, const Pages& p, int sms, cudaStream_t stream) {
+  // blocks that share a token's keys: as far as all run at the same time (two an SM), each with a run of keys a warp at least
+  int splits = 1;
+  while (splits < 8 && (int64_t)p.T * p.Hkv * splits * 2 <= 2 * sms && (int64_t)splits * 2 * WARPS * L_KEYS <= (int64_t)p.top * p.page_size) splits *= 2;
+  launch_pdl_cluster(pages_float_kernel<D, G>, dim3((unsigned)(p.T * splits), p.Hkv), dim3(WARPS * 32), dim3(splits), 0, stream,
+                     (const float*)q, (float*)out, (const float*)cache, p, splits);
   return cuda_status("attention_pages (32-bit)");
 }
 
-// Whether the 32-bit kernel for several tokens a request takes the call.
-bool float_tiles(const void* q, const void* out, const void* cache, const Pages& p) {
-  return (p.D == 64 || p.D == 128) && p.page_size >= 16 && !(p.page_size & (p.page_size - 1)) && p.H / p.Hkv <= 8 && p.top * F_TOKENS <= F_PICKS &&
-         p.ldq % 4 == 0 && p.ldo % 4 == 0 && (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15) == 0 && p.Hkv <= 65535 &&
-         p.T >= 2 * (int64_t)p.num_reqs;
+// Whether the 32-bit kernel takes the call.
+bool float_rows(const void* q, const void* out, const void* cache, const Pages& p) {
+  return (p.D == 64 || p.D == 128) && p.page_size % L_KEYS == 0 && p.H / p.Hkv <= 8 && p.ldq % 4 == 0 && p.ldo % 4 == 0 &&
+         (((uintptr_t)q | (uintptr_t)out | (uintptr_t)cache) & 15) == 0 && p.Hkv <= 65535 &&
+         (int64_t)p.top * (p.page_size / L_KEYS) < 0x7fffff00;
 }
 
 // ------------------------------------------------------------------------------------------------
@@ -658,9 +614,9 @@ DINFER_API int dinfer_attention_pages(const AttentionPagesArgs* a) {
     if (D == 128) return H / Hkv <= 8 ? run_token<128, 1>(q, out, cache, p, splits, stream) : run_token<128, 2>(q, out, cache, p, splits, stream);
     return H / Hkv <= 8 ? run_token<64, 1>(q, out, cache, p, splits, stream) : run_token<64, 2>(q, out, cache, p, splits, stream);
   }
-  if (dtype == DINFER_F32 && float_tiles(q, out, cache, p)) {
+  if (dtype == DINFER_F32 && float_rows(q, out, cache, p)) {
     const int group = H / Hkv;
-#define DINFER_FLOAT(G) return D == 64 ? run_float<64, G>(q, out, cache, p, stream) : run_float<128, G>(q, out, cache, p, stream)
+#define DINFER_FLOAT(G) return D == 64 ? run_float<64, G>(q, out, cache, p, sms, stream) : run_float<128, G>(q, out, cache, p, sms, stream)
     if (group == 1) DINFER_FLOAT(1);
     if (group == 2) DINFER_FLOAT(2);
     if (group <= 4) DINFER_FLOAT(4);

@@ -744,11 +744,12 @@ static int64_t workspace_of(int num_reqs, int width, int top, int T, int H, int 
 // Bytes of workspace that the call wants; 0 where it does not take the sizes, or (sms > 0, the device's multiprocessors) where token by
 // token is the shorter way.  Both are estimated, in microseconds.  Token by token every page is read for each token that chose it, at what L2 gives:
 //     7 + T Hkv top page_size D 4 / 6.3e6
-// Here a block takes 1.3 a key tile of 64, 20 pass before and after, and n neighbouring tokens choose some top n^0.4 pages among them.
+// Here a block takes 1 a key tile of 64, 20 pass before and after, and n neighbouring tokens choose some top n^0.4 pages among them.
 // The longest list (one request may bring all tokens but one each of the others) ends the step, or the lists of all do:
-//     20 + 1.3 max(tiles of the longest / ksplit, tiles of all / SMs)
-// Measured at 32 heads of 128 over 8, 16 pages of 64 behind 8000 tokens (us, token by token and here): 32 tokens 26 and 29, 64 tokens 51
-// and 36, 256 tokens 173 and 48, 64 tokens beside 16 single ones 70 and 120, 256 beside 16 190 and 120, 64 single ones 54 and 107.
+//     20 + max(tiles of the longest / ksplit, tiles of all / SMs)
+// Measured at 32 heads of 128 over 8, 16 pages of 64 behind 8000 tokens (us, token by token and here): 32 tokens 26 and 26, 48 tokens 47
+// and 31, 64 tokens 51 and 32, 256 tokens 173 and 38, 512 tokens 343 and 54, 64 tokens beside 16 single ones 70 and 77, 256 beside 16 190 and
+// 78, 256 beside 64 224 and 102, 64 single ones 55 and 54; 32 heads of 64 over 4, 24 pages of 32: 32 tokens 12 and 23, 128 tokens 20 and 30.
 DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size, int sms) {
   Params p{};
   const int64_t bytes = workspace_of(num_reqs, width, top, T, H, Hkv, D, page_size, p);
@@ -759,7 +760,7 @@ DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width
   const double lists = fmax((double)T / most, (double)(num_reqs < T ? num_reqs : T)) * Hkv;
   int ks = 1;
   while (ks < 8 && lists * ks * 2 <= sms && tiles(longest) >= ks * 8) ks *= 2;
-  return 20.0 + 1.3 * fmax(tiles(longest) / ks, lists * tiles(mean) / sms) < by_token ? bytes : 0;
+  return 20.0 + fmax(tiles(longest) / ks, lists * tiles(mean) / sms) < by_token ? bytes : 0;
 }
 
 // What the call takes, 8 bytes a field (a caller packs them and hands over one address).  As
