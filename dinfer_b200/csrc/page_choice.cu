@@ -495,12 +495,17 @@ choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t l
   for (int i = at + lane; i < top; i += 32) dst[i] = -1;
 }
 
-// More pages, up to 8192: a block per (token, key head), the order of the last pick bit by bit.
+// More pages, up to 8192: a block per (token, key head).  Up to 32 picks as above: the bound from the maxima of the block's threads, the
+// candidates that reach it into a list (in no order: a rank among equals, and a place among the picks, go by the page), which one
+// warp ranks.  Otherwise, or where too many reach the bound, the order of the last pick bit by bit over the block.
 template <int NPL>
 __global__ void __launch_bounds__(WARPS * 32)
 choose_block_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, const int* __restrict__ positions, int page_size,
                     int first, int recent, int top, int pages, int* __restrict__ out, int Hkv) {
   __shared__ int s_count[2][WARPS];
+  __shared__ unsigned s_best[WARPS * 32], s_bound;
+  __shared__ uint2 s_list[SHORT_LIST];
+  __shared__ int s_n;
   pdl_enter();
   const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
   const int64_t row = blockIdx.x;
@@ -538,33 +543,101 @@ choose_block_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
       const int j = lo + i * WARPS * 32 + threadIdx.x;
       key[i] = j < hi ? order_of(s[j]) : 0u;
     }
-    unsigned last = 0;
-#pragma unroll 1
-    for (int bit = 31; bit >= 0; --bit) {
-      const unsigned tried = last | (1u << bit);
-      int n = 0;
+    bool listed = false;
+    if (picks <= 32) {
+      unsigned best = 0;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) n += key[i] >= tried;
-      if (total(n, nullptr) >= picks) last = tried;
+      for (int i = 0; i < NPL; ++i) best = max(best, key[i]);
+      s_best[threadIdx.x] = best;
+      if (threadIdx.x == 0) s_n = 0;
+      __syncthreads();
+      if (warp == 0) {
+        unsigned b[WARPS], bound = 0;
+#pragma unroll
+        for (int w = 0; w < WARPS; ++w) b[w] = s_best[w * 32 + lane];
+#pragma unroll 1
+        for (int bit = 31; bit >= 16; --bit) {
+          const unsigned tried = bound | (1u << bit);
+          int n = 0;
+#pragma unroll
+          for (int w = 0; w < WARPS; ++w) n += b[w] >= tried;
+          if ((int)__reduce_add_sync(0xffffffffu, (unsigned)n) >= picks) bound = tried;
+        }
+        if (lane == 0) s_bound = max(bound, 1u);
+      }
+      __syncthreads();
+      const unsigned bound = s_bound;
+      if (best >= bound)
+#pragma unroll
+        for (int i = 0; i < NPL; ++i)
+          if (key[i] >= bound) {
+            const int k = atomicAdd(&s_n, 1);
+            if (k < SHORT_LIST) s_list[k] = make_uint2(key[i], (unsigned)(lo + i * WARPS * 32 + (int)threadIdx.x));
+          }
+      __syncthreads();
+      const int n = s_n;
+      listed = n <= SHORT_LIST;
+      if (listed && warp == 0) {
+        bool in[2];
+        uint2 a[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+          const int me = lane + 32 * half;
+          a[half] = me < n ? s_list[me] : make_uint2(0u, 0u);
+          int above = 0;                                     // larger ones, and equal ones of a lower page
+          for (int i = 0; i < n; ++i) {
+            const uint2 v = s_list[i];
+            above += v.x > a[half].x || (v.x == a[half].x && v.y < a[half].y);
+          }
+          in[half] = me < n && above < picks;
+        }
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          if (lane + 32 * half < n) s_list[lane + 32 * half].x = in[half];
+        __syncwarp();
+#pragma unroll
+        for (int half = 0; half < 2; ++half)
+          if (in[half]) {
+            int lower = 0;                                   // picks of a lower page
+            for (int i = 0; i < n; ++i) {
+              const uint2 v = s_list[i];
+              lower += v.x && v.y < a[half].y;
+            }
+            dst[at + lower] = (int)a[half].y;
+          }
+      }
+      if (listed) at += picks;
     }
-    int above = 0;
-#pragma unroll
-    for (int i = 0; i < NPL; ++i) above += key[i] > last;
-    int equal = picks - total(above, nullptr);
+    if (!listed) {
+      unsigned last = 0;
 #pragma unroll 1
-    for (int i0 = 0; i0 < NPL; ++i0) {
-      unsigned k = 0;
+      for (int bit = 31; bit >= 0; --bit) {
+        const unsigned tried = last | (1u << bit);
+        int n = 0;
 #pragma unroll
-      for (int i = 0; i < NPL; ++i) k = i == i0 ? key[i] : k;
-      int below;
-      const unsigned same = __ballot_sync(0xffffffffu, k == last);
-      const int sames = total(lane == 0 ? __popc(same) : 0, &below);
-      const bool in = k > last || (k == last && below + __popc(same & ((1u << lane) - 1)) < equal);
-      equal = max(0, equal - sames);
-      const unsigned mask = __ballot_sync(0xffffffffu, in);
-      const int ins = total(lane == 0 ? __popc(mask) : 0, &below);
-      if (in) dst[at + below + __popc(mask & ((1u << lane) - 1))] = lo + i0 * WARPS * 32 + threadIdx.x;
-      at += ins;
+        for (int i = 0; i < NPL; ++i) n += key[i] >= tried;
+        if (total(n, nullptr) >= picks) last = tried;
+      }
+      int above = 0;
+#pragma unroll
+      for (int i = 0; i < NPL; ++i) above += key[i] > last;
+      int equal = picks - total(above, nullptr);
+#pragma unroll 1
+      for (int i0 = 0; i0 < NPL; ++i0) {
+        unsigned k = 0;
+#pragma unroll
+        for (int i = 0; i < NPL; ++i) k = i == i0 ? key[i] : k;
+        int below;
+        const unsigned same = __ballot_sync(0xffffffffu, k == last);
+        const int sames = total(lane == 0 ? __popc(same) : 0, &below);
+        const bool in = k > last || (k == last && below + __popc(same & ((1u << lane) - 1)) < equal);
+        equal = max(0, equal - sames);
+        const unsigned mask = __ballot_sync(0xffffffffu, in);
+        const int ins = total(lane == 0 ? __popc(mask) : 0, &below);
+        if (in) dst[at + below + __popc(mask & ((1u << lane) - 1))] = lo + i0 * WARPS * 32 + threadIdx.x;
+        at += ins;
+      }
     }
   }
   for (int j = hi + threadIdx.x; j <= own; j += WARPS * 32) dst[at + j - hi] = j;
