@@ -148,9 +148,13 @@ page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const _
 // to a lane, so that a thread takes the maximum over a token's heads among its own registers and a warp writes 32 pages of a
 // token side by side.  A block keeps its pages and walks runs of tokens: while the products of a run are made, the next run's rows
 // of q are on their way and the results of the run before are written.  Two blocks share an SM.  The waits for the products are
-// bounded.  Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2.  @SCORES@
+// bounded.  Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2: 4096 tokens
+// of 32 heads of 128 over 8 against 512 pages (102 MB, 16 GFLOP) take 40 us, 39 % of a copy's rate (the kernel above 114): a run's rows are
+// waited for a good part of the time, and a third buffer for them would leave one block an SM.  Tensor pipe 19 %.
 constexpr int U_ROWS = 128, U_COLS = 128, U_NT = 256;
-// from so many tokens on, and so many a request
+// From so many tokens on, and so many a request.  us, the kernel above and this one, 32 heads of 128 over 8, pages of 64: 64 tokens behind 28000 18.9
+// and 6.2, 1024 tokens 26.8 and 13.4, 64 tokens behind 8000 beside 4 single ones 16.4 and 5.8, beside 62 20.6 and 15.1, 64 single ones 9.9 and
+// 21.5 (a run holds tokens of one request).
 constexpr int MANY_TOKENS = 16, MANY_TOKENS_A_REQUEST = 2;
 
 template <int D, int GP>
@@ -383,7 +387,8 @@ choose_pages_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, 
 // many lanes as picks reach it), else counted over all.  The candidates that reach it go to a list in shared memory, ascending, and are
 // ranked against one another; a pick's place among the picks is its place in the list.  Where too many reach the bound (equal
 // scores) the order of the last pick is found bit by bit, and of the candidates of that order the lowest are taken.
-// Bound by instructions: @CHOOSE@
+// Bound by instructions: 4096 tokens of 8 key heads choosing 16 of up to 512 pages (41 MB) take 29 us, 22 % of a copy's rate (27 M warp
+// instructions, issue slots 77 % busy); 8 single tokens 3.2.  A lane's pages side by side instead, for wider loads and no ballots, took 62.
 constexpr int SHORT_LIST = 64;
 
 template <int NPL>
@@ -497,7 +502,8 @@ choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t l
 
 // More pages, up to 8192: a block per (token, key head).  Up to 32 picks as above: the bound from the maxima of the block's threads, the
 // candidates that reach it into a list (in no order: a rank among equals, and a place among the picks, go by the page), which one
-// warp ranks.  Otherwise, or where too many reach the bound, the order of the last pick bit by bit over the block.
+// warp ranks.  512 tokens of 8 key heads over 2200 pages take 38 us (126 by the kernel for any sizes), over 4100 88 (228), one token 5.4 (35).
+// Otherwise, or where too many reach the bound, the order of the last pick bit by bit over the block.
 template <int NPL>
 __global__ void __launch_bounds__(WARPS * 32)
 choose_block_kernel(const float* __restrict__ scores, int64_t ldt, int64_t ldg, const int* __restrict__ positions, int page_size,
@@ -683,7 +689,6 @@ DINFER_API int dinfer_page_scores(const PageScoresArgs* a) {
   const int group = H / Hkv;
   const int64_t z = (pages + WARPS * 32 - 1) / (WARPS * 32);
   if (dtype == DINFER_BF16 && (D == 64 || D == 128) && group <= 16 && ldq % 8 == 0 && ((uintptr_t)q | (uintptr_t)means) % 16 == 0 && z <= 65535) {
-    // (measured: see MANY_TOKENS)
     if (a->status && T >= MANY_TOKENS && T >= MANY_TOKENS_A_REQUEST * (int64_t)num_reqs) {
       const __nv_bfloat16 *qb = (const __nv_bfloat16*)q, *mb = (const __nv_bfloat16*)means;
       const int sms = (int)a->sms;
