@@ -30,87 +30,105 @@ struct Pages {
 };
 
 constexpr int WARPS = 4;
-constexpr int KEYS = 4;
+constexpr int KEYS = 4, ANY_WARPS = 8;
 
-// Any sizes: a warp per (token, head), the lanes split the elements, four keys at a time.
+// Any sizes: a block per (token, head); its warps take runs of four keys in turn, the lanes split the elements, and the warps come
+// together in shared memory.  Bound by the rows' way from memory, which every head of a group goes alone; one token of 16 heads of 96,
+// 16 pages of 64, 36 us (a warp per head, key by key: 555); 32 single ones 107 (1046).
 template <typename T, int C>   // C >= ceil(D / 32)
-__global__ void __launch_bounds__(WARPS * 32)
+__global__ void __launch_bounds__(ANY_WARPS * 32)
 attention_pages_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __restrict__ cache, const Pages p) {
+  __shared__ float s_acc[ANY_WARPS][C * 32], s_m[ANY_WARPS], s_l[ANY_WARPS];
   pdl_enter();
-  const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int h = blockIdx.y * WARPS + warp;
-  if (h >= p.H) return;
+  const int t = blockIdx.x, h = blockIdx.y, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int r = request_of(p.cu, p.num_reqs, t);
-  if (r < 0) return;
+  if (r < 0) return;                                       // (the whole block alike)
   const int* table = p.table + (int64_t)r * p.width;
   const int g = h / (p.H / p.Hkv), pos = p.positions[t];
   const int* chosen = p.chosen + ((int64_t)t * p.Hkv + g) * p.top;
   const int64_t plane = (int64_t)p.Hkv * p.page_size * p.D;
   float qv[C], acc[C];
+  int at[C];                                               // the lane's elements; behind the last one the last one, against a zero
 #pragma unroll
   for (int c = 0; c < C; ++c) {
     const int e = lane + 32 * c;
+    at[c] = min(e, p.D - 1);
     qv[c] = e < p.D ? to_f32<T>(q[(int64_t)t * p.ldq + (int64_t)h * p.D + e]) * p.scale : 0.f;
     acc[c] = 0.f;
   }
   float m = -INFINITY, l = 0.f;
+  const unsigned runs = (p.page_size + KEYS - 1) / KEYS;
   for (int i = 0; i < p.top; ++i) {
     const int j = chosen[i];
     if (j < 0 || j >= p.width) continue;
     const int page = table[j];
     if (page < 0 || page >= p.num_pages) continue;
-    const int64_t keys = min((int64_t)p.page_size, pos - (int64_t)j * p.page_size + 1);
+    const int keys = (int)min((int64_t)p.page_size, pos - (int64_t)j * p.page_size + 1);
     const T* kp = cache + (int64_t)page * 2 * plane + (int64_t)g * p.page_size * p.D;
-    for (int o = 0; o < keys; o += KEYS) {
-      float s[KEYS];
+    // (the runs of all pages go round the warps, whatever a page holds of them)
+    for (int o = (int)((warp - i * runs) % ANY_WARPS) * KEYS; o < keys; o += ANY_WARPS * KEYS) {
+      T k[KEYS][C], v[KEYS][C];
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c) k[u][c] = kp[(int64_t)min(o + u, keys - 1) * p.D + at[c]];
+#pragma unroll
+      for (int u = 0; u < KEYS; ++u)
+#pragma unroll
+        for (int c = 0; c < C; ++c) v[u][c] = kp[plane + (int64_t)min(o + u, keys - 1) * p.D + at[c]];
+      float s[KEYS], n = m;
 #pragma unroll
       for (int u = 0; u < KEYS; ++u) {
         s[u] = 0.f;
-        if (o + u < keys)
 #pragma unroll
-          for (int c = 0; c < C; ++c)
-            if (lane + 32 * c < p.D) s[u] = fmaf(qv[c], to_f32<T>(kp[(int64_t)(o + u) * p.D + lane + 32 * c]), s[u]);
+        for (int c = 0; c < C; ++c)
+          if (lane + 32 * c < p.D) s[u] = fmaf(qv[c], to_f32<T>(k[u][c]), s[u]);
+        s[u] = warp_sum(s[u]);
+        if (o + u < keys) n = fmaxf(n, s[u]);
       }
-      float n = m;
-#pragma unroll
-      for (int u = 0; u < KEYS; ++u) {
-        s[u] = o + u < keys ? warp_sum(s[u]) : -INFINITY;
-        n = fmaxf(n, s[u]);
-      }
-      const float base = n == -INFINITY ? 0.f : n;
-      const float alpha = expf(m - base);
+      const float base = n == -INFINITY ? 0.f : n, alpha = expf(m - base);
       l *= alpha;
 #pragma unroll
       for (int c = 0; c < C; ++c) acc[c] *= alpha;
 #pragma unroll
-      for (int u = 0; u < KEYS; ++u) {
-        if (o + u >= keys) break;
-        const float w = expf(s[u] - base);
-        l += w;
+      for (int u = 0; u < KEYS; ++u)
+        if (o + u < keys) {
+          const float w = expf(s[u] - base);
+          l += w;
 #pragma unroll
-        for (int c = 0; c < C; ++c)
-          if (lane + 32 * c < p.D) acc[c] = fmaf(w, to_f32<T>(kp[plane + (int64_t)(o + u) * p.D + lane + 32 * c]), acc[c]);
-      }
+          for (int c = 0; c < C; ++c) acc[c] = fmaf(w, to_f32<T>(v[u][c]), acc[c]);
+        }
       m = n;
     }
   }
-  const float inv = l == 0.f ? 0.f : 1.f / l;
 #pragma unroll
-  for (int c = 0; c < C; ++c) {
-    const int e = lane + 32 * c;
-    if (e < p.D) out[(int64_t)t * p.ldo + (int64_t)h * p.D + e] = from_f32<T>(acc[c] * inv);
+  for (int c = 0; c < C; ++c) s_acc[warp][lane + 32 * c] = acc[c];
+  if (lane == 0) { s_m[warp] = m; s_l[warp] = l; }
+  __syncthreads();
+  float top = s_m[0], sum = 0.f;
+#pragma unroll
+  for (int w = 1; w < ANY_WARPS; ++w) top = fmaxf(top, s_m[w]);
+  const float base = top == -INFINITY ? 0.f : top;
+#pragma unroll
+  for (int w = 0; w < ANY_WARPS; ++w) sum = fmaf(s_l[w], expf(s_m[w] - base), sum);
+  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  for (int e = threadIdx.x; e < p.D; e += ANY_WARPS * 32) {
+    float o = 0.f;
+#pragma unroll
+    for (int w = 0; w < ANY_WARPS; ++w) o = fmaf(s_acc[w][e], expf(s_m[w] - base), o);
+    out[(int64_t)t * p.ldo + (int64_t)h * p.D + e] = from_f32<T>(sum == 0.f ? 0.f : o * inv);
   }
 }
 
 template <typename T>
 int run(const void* q, void* out, const void* cache, const Pages& p, cudaStream_t stream) {
-  const dim3 grid(p.T, (p.H + WARPS - 1) / WARPS), block(WARPS * 32);
+  const dim3 grid(p.T, p.H), block(ANY_WARPS * 32);
   if (p.D <= 64) launch_pdl(attention_pages_kernel<T, 2>, grid, block, 0, stream, (const T*)q, (T*)out, (const T*)cache, p);
   else if (p.D <= 128) launch_pdl(attention_pages_kernel<T, 4>, grid, block, 0, stream, (const T*)q, (T*)out, (const T*)cache, p);
+  else if (p.D <= 256) launch_pdl(attention_pages_kernel<T, 8>, grid, block, 0, stream, (const T*)q, (T*)out, (const T*)cache, p);
   else launch_pdl(attention_pages_kernel<T, 16>, grid, block, 0, stream, (const T*)q, (T*)out, (const T*)cache, p);
   return cuda_status("attention_pages");
 }
-
 
 // ------------------------------------------------------------------------------------------------
 // 32-bit, head sizes 64 and 128, groups of up to 8 heads: a token and key head to a block, or to a cluster of up to eight that share its
@@ -606,7 +624,7 @@ DINFER_API int dinfer_attention_pages(const AttentionPagesArgs* a) {
   const int sms = (int)a->sms, dtype = (int)a->dtype;
   if (T < 0 || H <= 0 || Hkv <= 0 || H % Hkv || D <= 0 || D > 512 || page_size <= 0 || num_reqs <= 0 || top <= 0 || width < 0)
     return refuse(DINFER_BAD_ARGUMENT, "attention_pages: sizes T=%d H=%d Hkv=%d D=%d page=%d top=%d", T, H, Hkv, D, page_size, top);
-  if ((H + WARPS - 1) / WARPS > 65535) return refuse(DINFER_BAD_ARGUMENT, "attention_pages: %d heads", H);
+  if (H > 65535) return refuse(DINFER_BAD_ARGUMENT, "attention_pages: %d heads", H);
   if (T == 0) return DINFER_OK;
   const Pages p{ldq, ldo, num_pages, table, width, cu_seqlens, num_reqs, positions, chosen, top, T, H, Hkv, D, page_size, scale};
   if (dtype == DINFER_BF16 && tensor_cores(q, out, cache, p)) {

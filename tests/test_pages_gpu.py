@@ -267,6 +267,32 @@ def test_attention(size, dtype, kind, form):
         assert form[1] == ["attention_pages_umma"]
 
 
+@pytest.mark.parametrize("requests", [[(700, 1)], [(300, 1)] * 40 + [(0, 1), (23, 1)], [(500, 3), (0, 0), (90, 30), (7, 1)]], ids=["one", "many", "mixed"])
+@pytest.mark.parametrize("P,H,G,D", [(8, 2, 2, 128), (24, 6, 3, 64), (40, 6, 2, 128), (64, 5, 1, 64), (16, 16, 2, 128), (200, 8, 1, 128),
+                                     (64, 18, 2, 128), (12, 4, 2, 64), (64, 6, 2, 96), (33, 3, 1, 512)])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+def test_attention_of_single_tokens(requests, P, H, G, D, dtype):
+    """Groups of one to nine heads, pages of any length, a token alone (a cluster shares its keys) and many."""
+    from dinfer_b200.kernels import page_ops
+    g = gen(P + H)
+    b = Batch(requests, P, seed=P, extra_width=1, pad=1)
+    q, cache = torch.randn(b.T, H * D, generator=g).to(dtype), torch.randn(b.num_pages, 2, G, P, D, generator=g).to(dtype)
+    seen = torch.zeros(b.num_pages, P, dtype=torch.bool)
+    for r, (h, n) in enumerate(requests):
+        for p in range(h + n):
+            seen[int(b.table[r, p // P]), p % P] = True
+    cache.transpose(2, 3).transpose(1, 2)[~seen] = math.inf
+    chosen = choices(b, G, 7, g, "odd")
+    out = torch.full((b.T, H * D), 3.0, dtype=dtype, device="cuda")
+    page_ops.attention_pages(c(q), out, c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, D ** -0.5)
+    got = out.cpu()
+    assert (got[b.live:] == 3.0).all()
+    want, size_, qk = plain_attention(q, cache, b, chosen, H, D ** -0.5)
+    bound = attention_bound(dtype, D, want, size_, qk)
+    off = (got[:b.live].double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
 @pytest.mark.parametrize("new", [1, 5, 100, 400])
 @pytest.mark.parametrize("what", ["value", "key"])
 @pytest.mark.parametrize("dtype", [BF16, F32])
