@@ -65,7 +65,7 @@ __device__ __forceinline__ const float* angles(const Append& p, int t) {
 template <typename TA, typename TW>
 __global__ void __launch_bounds__(WARPS * 32)
 append_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW* __restrict__ q_weight,
-              const TW* __restrict__ k_weight, TA* cache, TA* __restrict__ means, const Append p) {
+              const TW* __restrict__ k_weight, TA* __restrict__ cache, const Append p) {
   __shared__ float sm[WARPS][MAX_D];
   pdl_enter();
   const int t = blockIdx.x, warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
@@ -92,30 +92,24 @@ append_kernel(const TA* __restrict__ qkv, TA* __restrict__ q_out, const TW* __re
     for (int e = lane; e < p.D; e += 32) dst[e] = from_f32<TA>(xs[e]);
     __syncwarp();
   }
-  if (!kept || off != p.page_size - 1) return;
-  // the page is full: its mean, a warp per key head
-  for (int g = warp; g < p.Hkv; g += WARPS) {
-    float sum[MAX_D / 32] = {};
-    for (int o = 0; o < p.page_size; ++o) {
-      const int back = p.page_size - 1 - o, u = t - back;
-      if (u >= 0 && p.slots[u] == slot - back) {               // brought by this step
-        finish_row<TA, TW>(qkv + (int64_t)u * p.ld + (int64_t)(p.H + g) * p.D, k_weight, angles(p, u), p, xs, lane);
-#pragma unroll
-        for (int i = 0; i < MAX_D / 32; ++i)
-          if (lane + 32 * i < p.D) sum[i] += to_f32<TA>(from_f32<TA>(xs[lane + 32 * i]));
-        __syncwarp();
-      } else {
-        const TA* k = cache + (int64_t)page * 2 * plane + ((int64_t)g * p.page_size + o) * p.D;
-#pragma unroll
-        for (int i = 0; i < MAX_D / 32; ++i)
-          if (lane + 32 * i < p.D) sum[i] += to_f32<TA>(k[lane + 32 * i]);
-      }
+}
+
+// The means of the pages whose last offset the step wrote, from the cache, behind the launch that wrote it: a block per token, a warp per
+// key head.
+template <typename TA>
+__global__ void __launch_bounds__(WARPS * 32) any_means_kernel(const TA* __restrict__ cache, TA* __restrict__ means, const Append p) {
+  pdl_enter();
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, slot = p.slots[blockIdx.x], page = slot / p.page_size;
+  if (slot < 0 || page >= p.num_pages || slot % p.page_size != p.page_size - 1) return;
+  const int64_t plane = (int64_t)p.Hkv * p.page_size * p.D;
+  for (int g = warp; g < p.Hkv; g += WARPS)
+    for (int e = lane; e < p.D; e += 32) {
+      const TA* k = cache + (int64_t)page * 2 * plane + (int64_t)g * p.page_size * p.D + e;
+      float sum = 0.f;
+#pragma unroll 8
+      for (int o = 0; o < p.page_size; ++o) sum += to_f32<TA>(k[(int64_t)o * p.D]);
+      means[((int64_t)page * p.Hkv + g) * p.D + e] = from_f32<TA>(sum / (float)p.page_size);
     }
-    TA* dst = means + ((int64_t)page * p.Hkv + g) * p.D;
-#pragma unroll
-    for (int i = 0; i < MAX_D / 32; ++i)
-      if (lane + 32 * i < p.D) dst[lane + 32 * i] = from_f32<TA>(sum[i] / (float)p.page_size);
-  }
 }
 
 // ---- head sizes 64 and 128, rows on 16-byte boundaries, a rotation over a multiple of 8 elements.  A lane owns eight elements of a head
@@ -212,46 +206,60 @@ template <typename TA, typename TW, int D, bool ROWS>
 __device__ __forceinline__ void make_means(const TA* qkv, const TW* k_weight, const TA* cache, TA* means, int t0, int g, int T, const Append& p) {
   constexpr int LANES = D / 8, PER = 32 / LANES, AHEAD = 4;
   __shared__ float s_sum[WARPS][D];
+  __shared__ int s_token[ROWS ? MAX_PAGE : 1];               // the step's token that brings an offset's key, or -1
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LANES, side = lane / LANES;
-  int slots;
+  int slots, all_slots[ROWS ? FEW_TOKENS / (WARPS * 32) : 1];
+  if (ROWS)
+#pragma unroll
+    for (int i = 0; i < FEW_TOKENS / (WARPS * 32); ++i) {
+      const int u = threadIdx.x + i * WARPS * 32;
+      all_slots[i] = u < T ? p.slots[u] : -1;
+    }
   unsigned ends = page_ends(p, t0, T, ROWS ? FEW_SPAN : 32, slots);
   if (!ends) return;
   const Place at = place_of(p, l);
   const bool norm = k_weight != nullptr;
   for (; ends; ends &= ends - 1) {
-    const int from = __ffs(ends) - 1, t = t0 + from, slot = __shfl_sync(0xffffffffu, slots, from), page = slot / p.page_size;
+    const int slot = __shfl_sync(0xffffffffu, slots, __ffs(ends) - 1), page = slot / p.page_size;
     const TA* cached = cache + ((int64_t)page * 2 * p.Hkv + g) * p.page_size * D;
     float sum[8] = {};
+    if (ROWS) {                                              // (whatever order the batch has its tokens in)
+      if (threadIdx.x < MAX_PAGE) s_token[threadIdx.x] = -1;
+      __syncthreads();
+#pragma unroll
+      for (int i = 0; i < FEW_TOKENS / (WARPS * 32); ++i) {
+        const unsigned o = (unsigned)all_slots[i] - (unsigned)page * p.page_size;
+        if (all_slots[i] >= 0 && o < (unsigned)p.page_size) s_token[o] = threadIdx.x + i * WARPS * 32;
+      }
+      __syncthreads();
+    }
     for (int o0 = warp * PER; o0 < p.page_size; o0 += WARPS * PER * AHEAD) {
       Lane8<TA> in[AHEAD];
-      bool now[AHEAD];
+      int from[AHEAD];                                       // token of this step, or -1
 #pragma unroll
-      for (int u = 0; u < AHEAD; ++u) {                      // (no branch between the loads: they go out together)
-        const int o = o0 + u * WARPS * PER + side, back = p.page_size - 1 - o;
-        now[u] = ROWS && back >= 0 && t - back >= 0 && p.slots[max(t - max(back, 0), 0)] == slot - back;
-      }
+      for (int u = 0; u < AHEAD; ++u) from[u] = ROWS ? s_token[min(o0 + u * WARPS * PER + side, p.page_size - 1)] : -1;
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int o = min(o0 + u * WARPS * PER + side, p.page_size - 1);
-        in[u] = load_lane<TA>(now[u] ? qkv + (int64_t)(t - (p.page_size - 1 - o)) * p.ld + (int64_t)(p.H + g) * D : cached + o * D, at.a, at.b);
+        in[u] = load_lane<TA>(from[u] >= 0 ? qkv + (int64_t)from[u] * p.ld + (int64_t)(p.H + g) * D : cached + o * D, at.a, at.b);
       }
 #pragma unroll
       for (int u = 0; u < AHEAD; ++u) {
         const int o = o0 + u * WARPS * PER + side;
         float v[8];
         widen<TA>(in[u], v);
-        if (ROWS && __any_sync(0xffffffffu, now[u])) {
+        if (ROWS && __any_sync(0xffffffffu, from[u] >= 0)) {
           float w[8], x[8];
           if (norm) widen<TW>(load_lane<TW>(k_weight, at.a, at.b), w);
 #pragma unroll
           for (int j = 0; j < 8; ++j) x[j] = v[j];
           float4 c = make_float4(1.f, 1.f, 1.f, 1.f), s = make_float4(0.f, 0.f, 0.f, 0.f);
-          if (p.rot) load_turn(angles(p, now[u] ? t - (p.page_size - 1 - o) : t), at, p.rot, l, c, s);
+          if (p.rot) load_turn(angles(p, max(from[u], 0)), at, p.rot, l, c, s);
           finish<LANES>(x, norm, w, p.eps, at, c, s);
           float y[8];
           widen<TA>(narrow<TA>(x), y);
 #pragma unroll
-          for (int j = 0; j < 8; ++j) v[j] = now[u] ? y[j] : v[j];
+          for (int j = 0; j < 8; ++j) v[j] = from[u] >= 0 ? y[j] : v[j];
         }
         if (o < p.page_size)
 #pragma unroll
@@ -376,7 +384,8 @@ int run(const void* qkv, void* q_out, const void* qw, const void* kw, void* cach
     return cuda_status("page_append");
   }
   launch_pdl(append_kernel<TA, TW>, dim3(T), dim3(WARPS * 32), 0, stream, (const TA*)qkv, (TA*)q_out, (const TW*)qw,
-             (const TW*)kw, (TA*)cache, (TA*)means, p);
+             (const TW*)kw, (TA*)cache, p);
+  launch_pdl(any_means_kernel<TA>, dim3(T), dim3(WARPS * 32), 0, stream, (const TA*)cache, (TA*)means, p);
   return cuda_status("page_append");
 }
 

@@ -146,7 +146,7 @@ def append(qkv: torch.Tensor, positions: torch.Tensor, num_heads: int, num_kv_he
            interleaved: bool = False) -> torch.Tensor:
     """From the projection's rows ``qkv`` [T, (H + 2 Hkv) D] (q heads | k heads | v heads; only read): q, normed and turned, into
     ``q_out`` [T, H * D]; k, normed and turned, and v into ``cache`` [pages, 2, Hkv, page, D] at ``slots`` (int32 [T], page *
-    page_size + offset; -1: a row that is not kept); and the mean of the keys, as cached, of every page whose last offset this
+    page_size + offset; -1: a row that is not kept; the batch may have a page's tokens in any order); and the mean of the keys, as cached, of every page whose last offset this
     step writes into ``means`` [pages, Hkv, D].  Other pages' means are left as they are.  ``q_weight`` / ``k_weight`` [D]: head norm
     ``x / sqrt(mean(x^2) + eps) * w``, or None for both; ``cos_sin`` f32 [positions, rot]: the angle table (``cos | sin``) of the
     first ``rot`` elements, pairs (i, i + rot/2) or with ``interleaved`` (2i, 2i + 1), which reaches every position; None: no
@@ -251,7 +251,7 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     """``out[t, h] = softmax over the seen keys (scale * q[t, h] . k) v``: token t sees the keys of its request's pages
     ``chosen[t, g]`` (int32 [T, Hkv, top]; g the head's key/value head) at positions up to ``positions[t]``.  Numbers outside the
     table's columns and pages the table does not hold are no pages, a page named twice counts twice, and a token that sees
-    nothing gets zeros.  ``q`` and ``out`` [T, H * D] may be strided rows; ``cache`` [pages, 2, Hkv, page, D].  Rows behind
+    nothing gets zeros.  ``q`` and ``out`` [T, H * D] may be strided rows, of memory of their own; ``cache`` [pages, 2, Hkv, page, D].  Rows behind
     the last request's tokens are left as they are.  Returns ``out``."""
     what = "attention_pages"
     _here(what, q, out, cache, block_table, cu_seqlens, positions, chosen)
@@ -265,6 +265,8 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     rows, ldo = _rows(what, "out", out, num_heads * D)
     if rows != T:
         raise KernelError(f"{what}: out [T, H * D] of q's shape")
+    if T and out.data_ptr() == q.data_ptr():
+        raise KernelError(f"{what}: out must not be q's memory (a row may be made twice)")
     B, width = _batch(what, T, block_table, cu_seqlens, positions)
     _ints(what, "chosen", chosen)
     shape = chosen.shape

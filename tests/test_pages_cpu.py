@@ -150,3 +150,9 @@ def test_part_refusals(change):
     assert need.key_means and need.block_size == 16 and [d.shape for d in mixer.declare()] == [(64, 64), (32, 64), (32, 64), (64, 64)]
     with pytest.raises(ValueError):
         MIXERS.get("page_attention")({**params, **change}, env)
+
+
+def test_attention_does_not_write_over_its_queries():
+    a = args("attention_pages")
+    with pytest.raises(KernelError, match="out must not be q's memory"):
+        page_ops.attention_pages(**{**a, "out": a["q"]})

@@ -122,6 +122,33 @@ def test_means_do_not_depend_on_the_portions(D, dtype):
 
 
 @pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("D", [64, 80, 128])
+@pytest.mark.parametrize("n", [45, 500, 650])
+def test_tokens_of_a_page_in_any_order(n, D, dtype):
+    """The rows of a step lie in the batch in any order: the same cache and the same means, bit by bit."""
+    from dinfer_b200.kernels import page_ops
+    P, H, G, old = 32, 4, 2, 20
+    g = gen(n)
+    b = Batch([(0, old + n)], P, seed=2)
+    x = torch.randn(old + n, (H + 2 * G) * D, generator=g).to(dtype).cuda()
+    w = (1 + 0.1 * torch.randn(D, generator=g)).to(dtype).cuda()
+    table, slots, positions = angles(old + n, D).cuda(), c(b.slots), c(b.positions)
+    got = []
+    for order in (torch.arange(n), torch.arange(n).flip(0), torch.randperm(n, generator=g)):
+        cache = torch.zeros(b.num_pages, 2, G, P, D, dtype=dtype, device="cuda")
+        means = torch.zeros(b.num_pages, G, D, dtype=dtype, device="cuda")
+        for rows in (torch.arange(old), old + order):
+            rows = rows.cuda()
+            q = torch.empty(len(rows), H * D, dtype=dtype, device="cuda")
+            page_ops.append(x[rows], positions[rows], H, G, D, 1e-6, w, w, table, q, cache, slots[rows], means)
+        got.append((cache.cpu(), means.cpu()))
+    for other in got[1:]:
+        for a, z in zip(got[0], other):
+            assert torch.equal(a, z)
+    assert int((got[0][1].float().abs().sum((1, 2)) > 0).sum()) == (old + n) // P
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
 @pytest.mark.parametrize("size", SIZES + [([(1700, 40), (33, 1), (0, 90), (640, 3)], 16, 8, 2, 128), ([(900, 1)] * 9, 16, 4, 2, 64),
                                           ([(2500, 150), (0, 40), (4100, 300)], 16, 8, 2, 128), ([(300, 90)], 16, 5, 5, 64), ([(700, 200)], 32, 10, 2, 64),
                                           ([(600, 70)], 16, 12, 4, 128), ([(520, 66)], 16, 32, 2, 64), ([(0, 64), (64, 64)], 64, 16, 2, 64)], ids=str)
