@@ -149,8 +149,9 @@ page_scores_mma_kernel(const __nv_bfloat16* __restrict__ q, int64_t ldq, const _
 // token side by side.  A block keeps its pages and walks runs of tokens: while the products of a run are made, the next run's rows
 // of q are on their way and the results of the run before are written.  Two blocks share an SM.  The waits for the products are
 // bounded.  Bound by what it writes (4 bytes a token, key head and page) and by the rows of q from L2: 4096 tokens
-// of 32 heads of 128 over 8 against 512 pages (102 MB, 16 GFLOP) take 40 us, 39 % of a copy's rate (the kernel above 114): a run's rows are
-// waited for a good part of the time, and a third buffer for them would leave one block an SM.  Tensor pipe 19 %.
+// of 32 heads of 128 over 8 against 512 pages (102 MB, 16 GFLOP) take 40 us, 39 % of a copy's rate (the kernel above 114): the steps
+// of a run (products, tensor memory, maxima, stores) and its barrier, tensor pipe 19 %.  256 pages a block with three buffers of rows, one
+// block an SM, took 45 us.
 constexpr int U_ROWS = 128, U_COLS = 128, U_NT = 256;
 // From so many tokens on, and so many a request.  us, the kernel above and this one, 32 heads of 128 over 8, pages of 64: 64 tokens behind 28000 18.9
 // and 6.2, 1024 tokens 26.8 and 13.4, 64 tokens behind 8000 beside 4 single ones 16.4 and 5.8, beside 62 20.6 and 15.1, 64 single ones 9.9 and
