@@ -501,9 +501,10 @@ choose_registers_kernel(const float* __restrict__ scores, int64_t ldt, int64_t l
   for (int i = at + lane; i < top; i += 32) dst[i] = -1;
 }
 
-// More pages, up to 8192: a block per (token, key head).  Up to 32 picks as above: the bound from the maxima of the block's threads, the
+// More pages, up to 16384: a block per (token, key head).  Up to 32 picks as above: the bound from the maxima of the block's threads, the
 // candidates that reach it into a list (in no order: a rank among equals, and a place among the picks, go by the page), which one
-// warp ranks.  512 tokens of 8 key heads over 2200 pages take 38 us (126 by the kernel for any sizes), over 4100 88 (228), one token 5.4 (35).
+// warp ranks.  512 tokens of 8 key heads over 2200 pages take 38 us (126 by the kernel for any sizes), over 8100 119 (561), over 16200 333
+// (1072); one token 5.4 (35), 7 (160), 8.6 (376).
 // Otherwise, or where too many reach the bound, the order of the last pick bit by bit over the block.
 template <int NPL>
 __global__ void __launch_bounds__(WARPS * 32)
@@ -753,8 +754,8 @@ DINFER_API int dinfer_choose_pages(const ChoosePagesArgs* a) {
                   page_size, pages, first, recent, top);
   if (T == 0) return DINFER_OK;
   const int64_t rows = (int64_t)T * Hkv;
-  if (pages > 2048 && pages <= 8192 && rows <= 0x7fffffff) {
-    auto kernel = pages <= 4096 ? choose_block_kernel<16> : choose_block_kernel<32>;
+  if (pages > 2048 && pages <= 16384 && rows <= 0x7fffffff) {
+    auto kernel = pages <= 4096 ? choose_block_kernel<16> : pages <= 8192 ? choose_block_kernel<32> : choose_block_kernel<64>;
     launch_pdl(kernel, dim3((unsigned)rows), dim3(WARPS * 32), 0, stream, scores, ldt, ldg, positions, page_size, first, recent, top,
                pages, out, Hkv);
     return cuda_status("choose_pages");

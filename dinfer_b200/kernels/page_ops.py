@@ -10,7 +10,7 @@ All four take the step's tokens as one batch (portions of prompts beside decoded
 up to 512, any number of heads per key/value head, any page size.  Head sizes 64 and 128 on rows of 16-byte boundaries run on
 kernels of their own: appending both dtypes with pages of up to 128 tokens, scores in bfloat16 with groups of up to 16 heads, attention in
 bfloat16 with pages of 16, 32, 64 or 128 tokens (groups of up to 16 heads, of up to 128 in long portions) and in float32 with groups of up to
-8.  The choice has its own up to 8192 pages.  What is left runs on kernels for any sizes, many times slower.  Tensors lie on the current device; the calls run on its current stream.
+8.  The choice has its own up to 16384 pages.  What is left runs on kernels for any sizes, many times slower.  Tensors lie on the current device; the calls run on its current stream.
 """
 from __future__ import annotations
 

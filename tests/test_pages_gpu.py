@@ -196,7 +196,7 @@ def test_scores_of_what_is_no_number(new, dtype):
 
 
 @pytest.mark.parametrize("top,first,recent", [(1, 0, 1), (4, 1, 1), (8, 2, 3), (16, 1, 2), (31, 0, 1), (33, 1, 1), (64, 4, 4), (100, 1, 2), (300, 0, 1)])
-@pytest.mark.parametrize("pages", [1, 7, 31, 33, 100, 257, 700, 1500, 2100, 5000, 8300])
+@pytest.mark.parametrize("pages", [1, 7, 31, 33, 100, 257, 700, 1500, 2100, 5000, 8300, 16500])
 def test_choice(pages, top, first, recent):
     from dinfer_b200.kernels import page_ops
     P, T, G = 16, 24, 3
