@@ -30,7 +30,7 @@
 #include <cuda.h>
 #include <math.h>
 
-#include "common.cuh"
+#include "page_batch.cuh"
 #include "split_umma.cuh"
 #include "umma_attention.cuh"
 
@@ -72,30 +72,7 @@ struct Params {
 };
 
 // The pair of row tiles `y` of the batch (every lane of a full warp asks): request, first token, tokens; request -1 beyond the last.
-__device__ __forceinline__ int3 pair_of(const Params& p, int y) {
-  const int lane = threadIdx.x & 31, tile = 2 * p.tile_tokens;
-  int before = 0;
-  for (int i0 = 0; i0 < p.B; i0 += 32) {
-    const int i = i0 + lane;
-    const int begin = i < p.B ? p.cu[i] : 0, tokens = i < p.B ? p.cu[i + 1] - begin : 0;
-    const int n = (tokens + tile - 1) / tile;
-    int incl = n;
-#pragma unroll
-    for (int d = 1; d < 32; d <<= 1) {
-      const int v = __shfl_up_sync(0xffffffffu, incl, d);
-      if (lane >= d) incl += v;
-    }
-    const unsigned hit = __ballot_sync(0xffffffffu, y >= before + incl - n && y < before + incl);
-    if (hit) {
-      const int src = __ffs(hit) - 1;
-      const int at = y - before - __shfl_sync(0xffffffffu, incl - n, src);
-      const int b = __shfl_sync(0xffffffffu, begin, src), k = __shfl_sync(0xffffffffu, tokens, src);
-      return make_int3(i0 + src, b + at * tile, min(tile, k - at * tile));
-    }
-    before += __shfl_sync(0xffffffffu, incl, 31);
-  }
-  return make_int3(-1, 0, 0);
-}
+__device__ __forceinline__ int3 pair_of(const Params& p, int y) { return token_tile(p.cu, p.B, 2 * p.tile_tokens, y); }
 
 // The list of a pair of row tiles and key head: bits of the pages of a window in shared memory, then the pages that have any, in order.
 constexpr int LIST_NT = 256, WINDOW_WORDS = 8192;
@@ -268,8 +245,8 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
   const uint32_t base = (smem_u32(smem_dyn) + 1023u) & ~1023u;
   const uint32_t sQ = base, sK = sQ + 2 * Q_BYTES, sV = sK + STAGES * KV_BYTES;
   if (NP > 1 && n_tiles > 0 && n_tiles <= STAGES) {
-    // the last tile may have entries that are no page, and their slots hold what was there: finite numbers, please (behind the first
-    // tiles those of an earlier one; what is not finite would have the rows made again, for nothing)
+    // the last tile may have entries that are no page, whose slots hold what was there: zeros, if no tile came before on its stage
+    // (what is not a finite number would have the block's rows made again, for nothing)
     const uint32_t at0 = (n_tiles - 1) * KV_BYTES;
     for (int i = threadIdx.x; i < (int)(2 * KV_BYTES / 16); i += NTHREADS) {
       const uint32_t off = i < (int)(KV_BYTES / 16) ? sK + at0 + i * 16 : sV + at0 + i * 16 - KV_BYTES;
