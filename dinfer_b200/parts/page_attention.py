@@ -91,9 +91,8 @@ class PageAttention(Mixer):
         qkv = self.qkv(x)
         slots = g.slot_mapping
         if not cache.write:                                  # another layer's keys and values: only q is made
-            slots = ctx.derived.get("page_attention: no slots")
-            if slots is None:
-                slots = ctx.derived["page_attention: no slots"] = torch.full_like(g.slot_mapping, -1)
+            # made by every run: a graph has to own and fill what it reads (a tensor kept in the context would be its warm-up's)
+            slots = torch.full_like(slots, -1)
         q = torch.empty((qkv.shape[0], self.H * self.D), dtype=qkv.dtype, device=qkv.device)
         page_ops.append(qkv, ctx.positions, self.H, self.Hkv, self.D, self.eps, self.q_norm_w, self.k_norm_w,
                         self.position.fused_table(), q, cache.kv, slots, cache.means,
