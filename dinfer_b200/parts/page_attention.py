@@ -91,6 +91,9 @@ class PageAttention(Mixer):
         qkv = self.qkv(x)
         slots = g.slot_mapping
         if not cache.write:                                  # another layer's keys and values: only q is made
+            if cache.means is None or cache.kv.shape[3] != self.page:
+                raise ValueError(f"page attention in pages of {self.page} reads another entry's cache, which has to keep key means in "
+                                 f"pages as large (pages of {cache.kv.shape[3]}, {'no ' if cache.means is None else ''}means)")
             # made by every run: a graph has to own and fill what it reads (a tensor kept in the context would be its warm-up's)
             slots = torch.full_like(slots, -1)
         q = torch.empty((qkv.shape[0], self.H * self.D), dtype=qkv.dtype, device=qkv.device)

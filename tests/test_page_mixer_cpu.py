@@ -1,5 +1,4 @@
 """What the page-attention mixer hands to its calls (no GPU needed)."""
-import math
 from types import SimpleNamespace
 
 import pytest
@@ -61,3 +60,12 @@ def test_a_layer_that_reads_anothers_cache_keeps_no_tensor_beyond_its_run(calls)
     assert len({t.data_ptr() for t in slots}) == len(slots)
     m.forward(torch.zeros(TOKENS, 64), ctx, binding())
     assert calls[-4][1][11] is ctx.groups[0].slot_mapping
+
+
+@pytest.mark.parametrize("page,means", [(PAGE, False), (2 * PAGE, True), (PAGE // 2, True)])
+def test_another_entrys_cache_without_means_or_of_other_pages_is_refused(calls, page, means):
+    """Scores and choice count in the layer's own pages, attention in the cache's: unlike ones would read other keys than were chosen."""
+    m, ctx = mixer_and_step()
+    with pytest.raises(ValueError, match="another entry's cache"):
+        m.forward(torch.zeros(TOKENS, 64), ctx, binding(write=False, page=page, means=means))
+    assert calls == []
