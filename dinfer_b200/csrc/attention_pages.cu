@@ -4,9 +4,11 @@
 //     out[t, h] = sum_i softmax_i(scale q[t, h] . k_i) v_i      over  { i <= p : i / page_size in chosen[t, g] }
 //
 // A page named twice counts twice; a number outside the request's table, or a page the table does not hold, is no page; a token
-// that sees no key gets zeros; rows behind the last request's tokens are left as they are.  Scores, weights and sums in 32-bit.
+// that sees no key gets zeros, one all of whose scores are -inf what is not a number (0 / 0); rows behind the last request's tokens
+// are left as they are.  Scores, weights and sums in 32-bit.
 // What a token does not see is never multiplied, so that it may hold anything.
 #include <cooperative_groups.h>
+#include <float.h>
 
 #include "mma_tiles.cuh"
 #include "page_batch.cuh"
@@ -58,12 +60,14 @@ attention_pages_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __
   }
   float m = -INFINITY, l = 0.f;
   const unsigned runs = (p.page_size + KEYS - 1) / KEYS;
+  bool none = true;                                        // whether the token sees no key at all
   for (int i = 0; i < p.top; ++i) {
     const int j = chosen[i];
     if (j < 0 || j >= p.width) continue;
     const int page = table[j];
     if (page < 0 || page >= p.num_pages) continue;
     const int keys = (int)min((int64_t)p.page_size, pos - (int64_t)j * p.page_size + 1);
+    none &= keys <= 0;
     const T* kp = cache + (int64_t)page * 2 * plane + (int64_t)g * p.page_size * p.D;
     // (the runs of all pages go round the warps, whatever a page holds of them)
     for (int o = (int)((warp - i * runs) % ANY_WARPS) * KEYS; o < keys; o += ANY_WARPS * KEYS) {
@@ -111,12 +115,12 @@ attention_pages_kernel(const T* __restrict__ q, T* __restrict__ out, const T* __
   const float base = top == -INFINITY ? 0.f : top;
 #pragma unroll
   for (int w = 0; w < ANY_WARPS; ++w) sum = fmaf(s_l[w], expf(s_m[w] - base), sum);
-  const float inv = sum == 0.f ? 0.f : 1.f / sum;
+  const float inv = 1.f / sum;                             // (scores of -inf alone: 0 / 0)
   for (int e = threadIdx.x; e < p.D; e += ANY_WARPS * 32) {
     float o = 0.f;
 #pragma unroll
     for (int w = 0; w < ANY_WARPS; ++w) o = fmaf(s_acc[w][e], expf(s_m[w] - base), o);
-    out[(int64_t)t * p.ldo + (int64_t)h * p.D + e] = from_f32<T>(sum == 0.f ? 0.f : o * inv);
+    out[(int64_t)t * p.ldo + (int64_t)h * p.D + e] = from_f32<T>(none ? 0.f : o * inv);
   }
 }
 
@@ -173,12 +177,14 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
   const int own = N >= 32 ? lane * OWN : lane >> (5 - STEPS);
   const int key = own % L_KEYS;                            // of the lane's first sum; the heads of all of them are one
   const int runs = P / L_KEYS;
+  bool saw = false;                                        // a key
   for (int u = split * WARPS + warp; u < p.top * runs; u += splits * WARPS) {
     const int j = chosen[u / runs], part = u % runs * L_KEYS;
     if (j < 0 || j >= p.width || (int64_t)j * P + part > pos) continue;
     const int page = table[j];
     if (page < 0 || page >= p.num_pages) continue;
     const int n = min(L_KEYS, pos - j * P - part + 1);     // keys that the token sees
+    saw = true;
     const float* rows = cache + (int64_t)page * 2 * plane + ((int64_t)g * P + part) * D + lane * E;
     Vec k[L_KEYS], v[L_KEYS];
 #pragma unroll
@@ -254,7 +260,10 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
 #pragma unroll
   for (int h = 0; h < G; ++h) {
     const int src = N >= 32 ? h * L_KEYS / OWN : (h * L_KEYS) << (5 - STEPS);
-    const float m_h = __shfl_sync(0xffffffffu, m[0], src), l_h = __shfl_sync(0xffffffffu, sum, src);
+    const float m_w = __shfl_sync(0xffffffffu, m[0], src), l_h = __shfl_sync(0xffffffffu, sum, src);
+    // (-inf is the maximum of a warp that saw no key; of one all of whose scores are -inf it is the lowest number: where no score is
+    // larger the result is 0 / 0)
+    const float m_h = saw ? fmaxf(m_w, -FLT_MAX) : m_w;
 #pragma unroll
     for (int e = 0; e < E; ++e) s_acc[warp][h][lane * E + e] = acc[h][e];
     if (lane == 0) { s_acc[warp][h][D] = m_h; s_acc[warp][h][D + 1] = l_h; }
@@ -274,7 +283,7 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
       L = fmaf(s_acc[w][h][D + 1], f, L);
       o = fmaf(s_acc[w][h][d], f, o);
     }
-    if (splits == 1) orow[idx] = L == 0.f ? 0.f : o / L;
+    if (splits == 1) orow[idx] = M == -INFINITY ? 0.f : o / L;
     else {
       c_o[h][d] = o;
       if (d == 0) { c_ml[h][0] = M; c_ml[h][1] = L; }
@@ -297,7 +306,7 @@ pages_float_kernel(const float* __restrict__ q, float* __restrict__ out, const f
       L = fmaf(ml[1], f, L);
       o = fmaf(cluster.map_shared_rank(&c_o[0][0], r2)[idx], f, o);
     }
-    orow[idx] = L == 0.f ? 0.f : o / L;
+    orow[idx] = M == -INFINITY ? 0.f : o / L;
   }
   cluster.sync();                                          // nobody leaves while another reads its memory
 }
@@ -515,7 +524,7 @@ pages_token_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restric
     }
   }
   __syncthreads();
-  const int64_t orow = (int64_t)t * p.ldo + (int64_t)g * group * D;
+  const int64_t orow = (int64_t)t * p.ldo + (int64_t)g * group * D;     // (a page of the list holds a key that the token sees)
   for (int idx = threadIdx.x; idx < group * D; idx += NT) {
     const int head = idx / D, d = idx % D;
     float M = -INFINITY;
@@ -530,7 +539,7 @@ pages_token_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restric
       acc += w_o[(w * NHEADS + head) * D + d] * f;
     }
     if (splits == 1) {
-      out[orow + idx] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+      out[orow + idx] = __float2bfloat16_rn(n_pages == 0 ? 0.f : acc / L);
     } else {
       c_o[idx] = acc;
       if (d == 0) { c_ml[head * 2] = M; c_ml[head * 2 + 1] = L; }
@@ -555,7 +564,7 @@ pages_token_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restric
       L += ml[1] * f;
       acc += cluster.map_shared_rank(c_o, s)[idx] * f;
     }
-    out[orow + idx] = __float2bfloat16_rn(L == 0.f ? 0.f : acc / L);
+    out[orow + idx] = __float2bfloat16_rn(n_pages == 0 ? 0.f : acc / L);
   }
   cluster.sync();                                          // nobody leaves while another reads its memory
 }

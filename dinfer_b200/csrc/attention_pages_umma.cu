@@ -162,6 +162,7 @@ __device__ __noinline__ void rows_again(const Params& p, int request, int first,
       acc[c] = 0.f;
     }
     float m = -INFINITY, l = 0.f;
+    bool any = false;
     for (int i = 0; i < p.top; ++i) {
       const int j = p.chosen[((int64_t)t * p.Hkv + g) * p.top + i];
       if (j < 0 || j >= p.width || (int64_t)j * p.page_size > pos) continue;
@@ -169,6 +170,7 @@ __device__ __noinline__ void rows_again(const Params& p, int request, int first,
       if (page < 0 || page >= p.num_pages) continue;
       const __nv_bfloat16* kp = p.cache + (int64_t)page * 2 * plane + (int64_t)g * p.page_size * D;
       const int keys = min(p.page_size, pos - j * p.page_size + 1);
+      any = true;
       for (int o = 0; o < keys; ++o) {
         float s = 0.f;
 #pragma unroll
@@ -181,10 +183,23 @@ __device__ __noinline__ void rows_again(const Params& p, int request, int first,
         for (int c = 0; c < D / 32; ++c) acc[c] = fmaf(acc[c], alpha, w * __bfloat162float(kp[plane + o * D + lane + 32 * c]));
       }
     }
-    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const float inv = any ? 1.f / l : 0.f;                      // (scores of -inf alone: 0 / 0)
 #pragma unroll
     for (int c = 0; c < D / 32; ++c) p.out[(int64_t)t * p.ldo + (int64_t)h * D + lane + 32 * c] = __float2bfloat16_rn(acc[c] * inv);
   }
+}
+
+// Whether token t sees any key of the pages it chose.  (Not inlined: the registers of this rare way are not the kernel's.)
+__device__ __noinline__ bool sees_a_key(const Params& p, int request, int t, int g) {
+  const int *chosen = p.chosen + ((int64_t)t * p.Hkv + g) * p.top, *table = p.table + (int64_t)request * p.width;
+  const int width = p.width, num_pages = p.num_pages, page_size = p.page_size, top = p.top, pos = p.positions[t];
+  for (int i = 0; i < top; ++i) {
+    const int j = chosen[i];
+    if (j < 0 || j >= width || (int64_t)j * page_size > pos) continue;
+    const int page = table[j];
+    if (page >= 0 && page < num_pages) return true;
+  }
+  return false;
 }
 
 template <int D> constexpr size_t smem_bytes() {
@@ -498,7 +513,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       tc_fence_after();
     }
     const bool rows_on = w == 0 || b_on;
-    bool odd = false;
+    bool odd = false, none = false;                                 // to be made again; weights that add up to zero
     __nv_bfloat16* dst = row_ok ? p.out + (int64_t)t * p.ldo + (int64_t)(hk * p.group + r % p.group) * D : nullptr;
     // a warp's rows go through the shared memory of Q, which is free now, so that neighbouring lanes store neighbouring pieces
     unsigned char* stage = smem_dyn + (sQ - smem_u32(smem_dyn)) + w * Q_BYTES + quarter * 32 * D * 2;
@@ -530,6 +545,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
       if (ok && rows_on) {
         const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
         odd = row_ok && !(l_run == l_run);
+        none = row_ok && l_run == 0.f;
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
           float o[32];
@@ -580,6 +596,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         }
         const float inv = l_all == 0.f ? 0.f : 1.f / l_all;
         odd = row_ok && !(l_all == l_all);
+        none = row_ok && l_all == 0.f;
         const float4* recv = reinterpret_cast<const float4*>(smem_dyn + (sK - smem_u32(smem_dyn)));
 #pragma unroll
         for (int c = 0; c < D / 32; ++c) {
@@ -612,6 +629,8 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
         write();
       }
     }
+    // (a row that sees keys, whose scores are all -inf: made again, it is not a number)
+    if (none) odd |= sees_a_key(p, pair.x, t, hk);
     if (odd) s_odd = 1;
   }
   if (p.ksplit > 1 && (warp < 2 || warp >= MMA_WARP_B)) {           // the other warps pass the cluster's two barriers too

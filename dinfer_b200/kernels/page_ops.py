@@ -251,8 +251,9 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     """``out[t, h] = softmax over the seen keys (scale * q[t, h] . k) v``: token t sees the keys of its request's pages
     ``chosen[t, g]`` (int32 [T, Hkv, top]; g the head's key/value head) at positions up to ``positions[t]``.  Numbers outside the
     table's columns and pages the table does not hold are no pages, a page named twice counts twice, and a token that sees
-    nothing gets zeros.  ``q`` and ``out`` [T, H * D] may be strided rows, of memory of their own; ``cache`` [pages, 2, Hkv, page, D].  Rows behind
-    the last request's tokens are left as they are.  Returns ``out``."""
+    nothing gets zeros; one that sees keys whose scores are all -inf gets what is not a number, as the softmax does.  ``q`` and
+    ``out`` [T, H * D] may be strided rows, of memory of their own; ``cache`` [pages, 2, Hkv, page, D].  Rows behind the last request's
+    tokens are left as they are.  Returns ``out``."""
     what = "attention_pages"
     _here(what, q, out, cache, block_table, cu_seqlens, positions, chosen)
     dt = q.dtype
