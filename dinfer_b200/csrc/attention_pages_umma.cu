@@ -744,17 +744,24 @@ static int64_t workspace_of(int num_reqs, int width, int top, int T, int H, int 
 // Bytes of workspace that the call wants; 0 where it does not take the sizes, or (sms > 0, the device's multiprocessors) where token by
 // token is the shorter way.  Both are estimated, in microseconds.  Token by token every page is read for each token that chose it, at what L2 gives:
 //     7 + T Hkv top page_size D 4 / 6.3e6
+// or, where the tensor-core kernel for tokens does not take the call (groups above 16, more than 1024 chosen pages), for each head of each
+// token, which the kernel for any sizes does at half that, and at 26 keys of a token and head in a microsecond:
+//     7 + max(T H top page_size D 4 / 3e6, top page_size / 26)
 // Here a block takes 1 a key tile of 64, 20 pass before and after, and n neighbouring tokens choose some top n^0.4 pages among them.
 // The longest list (one request may bring all tokens but one each of the others) ends the step, or the lists of all do:
 //     20 + max(tiles of the longest / ksplit, tiles of all / SMs)
 // Measured at 32 heads of 128 over 8, 16 pages of 64 behind 8000 tokens (us, token by token and here): 32 tokens 26 and 26, 48 tokens 47
 // and 31, 64 tokens 51 and 32, 256 tokens 173 and 38, 512 tokens 343 and 54, 64 tokens beside 16 single ones 70 and 77, 256 beside 16 190 and
 // 78, 256 beside 64 224 and 102, 64 single ones 55 and 54; 32 heads of 64 over 4, 24 pages of 32: 32 tokens 12 and 23, 128 tokens 20 and 30.
+// By the kernel for any sizes and here: 64 heads of 128 over 1, 16 pages of 64: 2 tokens 39 and 21, 24 tokens 231 and 25, 300 tokens 2698 and 44,
+// 30 beside 30 single ones 548 and 31; 24 heads of 64 over 1, 8 pages of 16: 2 tokens 8 and 14, 24 tokens 14 and 17, 100 tokens 44 and
+// 17; 8 heads of 128 over 2, 1100 pages of 16: 2 tokens 682 and 55, 24 tokens 925 and 90.
 DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size, int sms) {
   Params p{};
   const int64_t bytes = workspace_of(num_reqs, width, top, T, H, Hkv, D, page_size, p);
   if (bytes == 0 || sms <= 0) return bytes;
-  const double by_token = 7.0 + (double)T * Hkv * (top < width ? top : width) * page_size * D * 4 / 6.3e6;
+  const double keys = (double)(top < width ? top : width) * page_size, row = D * 4;
+  const double by_token = 7.0 + (H / Hkv > 16 || top > 1024 ? fmax(T * H * keys * row / 3e6, keys / 26) : T * Hkv * keys * row / 6.3e6);
   auto tiles = [&](double n) { return fmin((double)width, top * pow(fmax(n, 1.0), 0.4)) * page_size / BN; };
   const double most = 2.0 * p.tile_tokens, longest = fmin(T - num_reqs + 1.0, most), mean = fmin((double)T / num_reqs, most);
   const double lists = fmax((double)T / most, (double)(num_reqs < T ? num_reqs : T)) * Hkv;

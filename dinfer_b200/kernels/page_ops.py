@@ -9,8 +9,9 @@ cheap score picks for it (per key/value head, shared by the heads of its group).
 All four take the step's tokens as one batch (portions of prompts beside decoded tokens), float32 or bfloat16, any head size
 up to 512, any number of heads per key/value head, any page size.  Head sizes 64 and 128 on rows of 16-byte boundaries run on
 kernels of their own: appending both dtypes with pages of up to 128 tokens, scores in bfloat16 with groups of up to 16 heads, attention in
-bfloat16 with pages of 16, 32, 64 or 128 tokens (groups of up to 16 heads, of up to 128 in long portions) and in float32 with groups of up to
-8.  The choice has its own up to 16384 pages.  What is left runs on kernels for any sizes, many times slower.  Tensors lie on the current device; the calls run on its current stream.
+bfloat16 with pages of 16, 32, 64 or 128 tokens and groups of up to 128 heads, in float32 with pages of a multiple of 8 tokens and groups of up
+to 8.  The choice has its own up to 16384 pages.  What is left, 32-bit scores among it, runs on kernels for any sizes, many times
+slower.  Tensors lie on the current device; the calls run on its current stream.
 """
 from __future__ import annotations
 
@@ -68,8 +69,10 @@ def _stream() -> int:
     return _raw_stream(_device()) if _raw_stream is not None else torch.cuda.current_stream().cuda_stream
 
 
-# Steps of fewer tokens are not asked about: token by token is the shorter way for them
+# Steps of fewer tokens, and of single tokens alone, are not asked about: token by token is the shorter way for them, where the tensor-core
+# kernel for tokens takes the call (groups of up to 16 heads, up to 1024 chosen pages)
 PORTION_TOKENS = 24
+TOKEN_GROUP, TOKEN_TOP = 16, 1024
 
 
 def _portions(head, always: bool = False) -> int:
@@ -276,7 +279,7 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     top = shape[2]
     head = (q.data_ptr(), ldq, out.data_ptr(), ldo, cache.data_ptr(), num_pages, block_table.data_ptr(), width, cu_seqlens.data_ptr(), B,
             positions.data_ptr(), chosen.data_ptr(), top, T, num_heads, Hkv, D, page_size, scale)
-    if T >= PORTION_TOKENS and T > B and dt == _BF16:
+    if dt == _BF16 and T and (T >= PORTION_TOKENS and T > B or num_heads > TOKEN_GROUP * Hkv or top > TOKEN_TOP):
         size = _portions(head)
         if size:
             work = torch.empty(size, dtype=torch.uint8, device=q.device)

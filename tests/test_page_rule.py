@@ -1,0 +1,49 @@
+"""Which kernel attention over chosen pages runs on (no GPU needed: the calls end where the library would be called)."""
+import pytest
+import torch
+
+from dinfer_b200.kernels import page_ops
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+@pytest.fixture
+def kernel_of(monkeypatch):
+    """The kernel library that a call names, for tensors that lie nowhere in particular."""
+    got = []
+    monkeypatch.setattr(page_ops, "_here", lambda what, *tensors: None)
+    monkeypatch.setattr(page_ops, "_device", lambda: 0)
+    monkeypatch.setattr(page_ops, "_multiprocessors", lambda: 148)
+    monkeypatch.setattr(page_ops, "_call", lambda lib, *args: got.append(lib))
+    monkeypatch.setattr(page_ops.gemm_ops, "_state", lambda device: {"status": torch.zeros(1, dtype=torch.int32)})
+
+    def kernel(new, history, H, G, D, top, page, dtype=BF16, scale=0.1, pages=None):
+        T, B, width = sum(new), len(new), -(-(history + max(new)) // page)
+        i = lambda *s: torch.zeros(*s, dtype=torch.int32)                            # noqa: E731
+        cache = torch.empty(2 if pages is None else pages, 2, G, page, D, dtype=dtype)
+        q = torch.empty(T, H * D, dtype=dtype)
+        page_ops.attention_pages(q, torch.empty_like(q), cache, i(B, width), i(B + 1), i(T), i(T, G, top), H, scale)
+        assert len(got) == 1
+        return got.pop()
+    return kernel
+
+
+# new tokens of the requests, history, heads, kv heads, head size, pages a token reads, tokens of a page
+@pytest.mark.parametrize("call,wanted", [
+    # the tensor-core kernel for tokens against neighbours together
+    (([1], 16000, 32, 8, 128, 16, 64), "attention_pages"), (([1] * 64, 8000, 32, 8, 128, 16, 64), "attention_pages"),
+    (([4096], 28672, 32, 8, 128, 16, 64), "attention_pages_umma"), (([256], 8000, 32, 8, 128, 16, 64), "attention_pages_umma"),
+    (([16], 8000, 32, 8, 128, 16, 64), "attention_pages"), (([64] + [1] * 16, 8000, 32, 8, 128, 16, 64), "attention_pages"),
+    # groups above 16 heads or more than 1024 pages: there is only the kernel for any sizes token by token, which is longer from few
+    # tokens on
+    (([100], 8000, 64, 1, 128, 16, 64), "attention_pages_umma"), (([300], 8000, 64, 1, 128, 16, 64), "attention_pages_umma"),
+    (([2], 8000, 64, 1, 128, 16, 64), "attention_pages_umma"), (([1] * 24, 8000, 64, 1, 128, 16, 64), "attention_pages_umma"),
+    (([100], 8000, 40, 2, 128, 16, 64), "attention_pages_umma"), (([300], 8000, 128, 1, 128, 8, 64), "attention_pages_umma"),
+    (([300], 8000, 48, 2, 64, 4, 64), "attention_pages_umma"), (([2], 20000, 8, 2, 128, 1100, 16), "attention_pages_umma"),
+    (([100], 20000, 8, 2, 128, 1100, 16), "attention_pages_umma"),
+    (([2], 8000, 24, 1, 64, 8, 16), "attention_pages"), (([24], 8000, 24, 1, 64, 8, 16), "attention_pages"), (([100], 8000, 24, 1, 64, 8, 16), "attention_pages_umma"),
+    # what the kernel of neighbours does not take
+    (([300], 8000, 129, 1, 128, 16, 64), "attention_pages"), (([300], 8000, 64, 1, 80, 16, 64), "attention_pages"),
+    (([300], 8000, 64, 1, 128, 16, 24), "attention_pages"), (([300], 8000, 64, 1, 128, 16, 64, F32), "attention_pages")], ids=str)
+def test_which_kernel_runs(kernel_of, call, wanted):
+    assert kernel_of(*call) == wanted

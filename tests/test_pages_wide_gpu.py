@@ -1,0 +1,50 @@
+"""Attention over chosen pages on groups of many heads and lists of many pages: the kernel in which neighbouring tokens walk their pages
+together, as the rule gives calls to it, with lists beyond what its shared memory holds."""
+import math
+
+import pytest
+import torch
+
+from page_cases import BF16, Batch, attention_bound, gen, plain_attention
+from test_pages_gpu import c, choices
+
+pytestmark = pytest.mark.gpu
+
+
+@pytest.fixture
+def libraries(monkeypatch):
+    """The kernel libraries that calls run on."""
+    from dinfer_b200.kernels import page_ops
+    got, real = [], page_ops._call
+
+    def counted(lib, *args):
+        got.append(lib)
+        return real(lib, *args)
+    monkeypatch.setattr(page_ops, "_call", counted)
+    return got
+
+
+def compare(b, q, cache, chosen, H):
+    from dinfer_b200.kernels import page_ops
+    D = cache.shape[-1]
+    got = page_ops.attention_pages(c(q), torch.full_like(c(q), 3.0), c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, D ** -0.5).cpu()
+    assert (got[b.live:] == 3.0).all()
+    want, size, qk = plain_attention(q, cache, b, chosen, H, D ** -0.5)
+    off, bound = (got[:b.live].double() - want).abs(), attention_bound(BF16, D, want, size, qk)
+    assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("requests,page,H,G,D,top", [
+    ([(700, 1)], 64, 64, 1, 128, 16), ([(700, 1)] * 5 + [(0, 1), (63, 1)], 64, 80, 2, 128, 16), ([(3000, 9)], 64, 64, 1, 128, 40),
+    ([(900, 30), (1500, 1), (20, 1)], 32, 48, 2, 64, 24), ([(2000, 60), (0, 0), (0, 5)], 16, 17, 1, 128, 100), ([(300, 20)], 128, 128, 1, 64, 3),
+    ([(20000, 2)], 16, 4, 2, 64, 1100), ([(17000, 1)] * 2, 16, 2, 2, 128, 1030)], ids=str)
+@pytest.mark.parametrize("kind", ["usual", "odd"])
+def test_what_the_kernel_for_tokens_does_not_take(requests, page, H, G, D, top, kind, libraries):
+    """Groups above 16 heads, more than 1024 pages: single tokens and portions, by rule."""
+    g = gen(H + page)
+    b = Batch(requests, page, seed=41, extra_width=1, pad=1)
+    q, cache = torch.randn(b.T, H * D, generator=g).to(BF16), torch.randn(b.num_pages, 2, G, page, D, generator=g).to(BF16)
+    if kind == "odd":
+        b.table[0, 1] = -1
+    compare(b, q, cache, choices(b, G, top, g, kind), H)
+    assert libraries == ["attention_pages_umma"]
