@@ -77,9 +77,9 @@ TOKEN_GROUP, TOKEN_TOP = 16, 1024
 
 def _portions(head, always: bool = False) -> int:
     """Bytes of workspace of the kernel in which neighbouring tokens walk the pages they chose together, where it takes this call (rows that
-    TMA can address, a positive scale) and is the shorter way (or ``always``); else 0."""
+    TMA can address, some pages, a scale that is positive in 32 bits) and is the shorter way (or ``always``); else 0."""
     q, ldq, out, ldo, cache, num_pages, _, width, _, B, _, _, top, T, H, Hkv, D, page_size, scale = head
-    if not scale > 0 or ldq % 8 or ldo % 8 or (q | out | cache) % 16 or num_pages * 2 * Hkv * page_size > 0x7fffffff:
+    if not scale > 2.0 ** -150 or num_pages == 0 or ldq % 8 or ldo % 8 or (q | out | cache) % 16 or num_pages * 2 * Hkv * page_size > 0x7fffffff:
         return 0
     f = library("attention_pages_umma").dinfer_attention_pages_umma_workspace
     f.argtypes, f.restype = [c_int] * 9, c_int64

@@ -47,3 +47,9 @@ def kernel_of(monkeypatch):
     (([300], 8000, 64, 1, 128, 16, 24), "attention_pages"), (([300], 8000, 64, 1, 128, 16, 64, F32), "attention_pages")], ids=str)
 def test_which_kernel_runs(kernel_of, call, wanted):
     assert kernel_of(*call) == wanted
+
+
+@pytest.mark.parametrize("more", [dict(pages=0), dict(scale=1e-46), dict(scale=0.0), dict(scale=-1.0)], ids=str)
+def test_a_cache_without_pages_and_a_scale_that_is_no_positive_number(kernel_of, more):
+    """The kernel of neighbouring tokens refuses them: the others give zeros, and weights that are right."""
+    assert kernel_of([256], 8000, 32, 8, 128, 16, 64, **more) == "attention_pages"

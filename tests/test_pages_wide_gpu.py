@@ -48,3 +48,29 @@ def test_what_the_kernel_for_tokens_does_not_take(requests, page, H, G, D, top, 
         b.table[0, 1] = -1
     compare(b, q, cache, choices(b, G, top, g, kind), H)
     assert libraries == ["attention_pages_umma"]
+
+
+@pytest.mark.parametrize("new", [1, 300])
+def test_a_cache_without_pages(new):
+    """Nothing is held, so nothing is seen: zeros, however many tokens."""
+    from dinfer_b200.kernels import page_ops
+    H, G, D, P = 8, 2, 128, 64
+    b = Batch([(900, new)], P, seed=42, pad=1)
+    q, cache = torch.randn(b.T, H * D, generator=gen(1)).to(BF16), torch.empty(0, 2, G, P, D, dtype=BF16)
+    chosen = choices(b, G, 16, gen(2), "usual")
+    got = page_ops.attention_pages(c(q), torch.full_like(c(q), 3.0), c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, 0.1).cpu()
+    assert (got[:b.live] == 0).all() and (got[b.live:] == 3.0).all()
+
+
+@pytest.mark.parametrize("scale", [1e-46, 1e-41, 0.0, -0.1])
+@pytest.mark.parametrize("new", [1, 300])
+def test_scales_that_are_not_positive_in_32_bits(new, scale):
+    from dinfer_b200.kernels import page_ops
+    H, G, D, P = 8, 2, 128, 64
+    b = Batch([(900, new)], P, seed=43)
+    g = gen(3)
+    q, cache = torch.randn(b.T, H * D, generator=g).to(BF16), torch.randn(b.num_pages, 2, G, P, D, generator=g).to(BF16)
+    chosen = choices(b, G, 16, g, "usual")
+    got = page_ops.attention_pages(c(q), torch.empty_like(c(q)), c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, scale).cpu()
+    want, size, qk = plain_attention(q, cache, b, chosen, H, scale)
+    assert bool(((got.double() - want).abs() <= attention_bound(BF16, D, want, size, qk.abs())).all())
