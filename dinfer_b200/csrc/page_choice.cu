@@ -322,7 +322,8 @@ int run_scores_umma(const __nv_bfloat16* q, int64_t ldq, const __nv_bfloat16* me
   }
   const int tiles = T / tokens + (num_reqs < T ? num_reqs : T), z = (pages + U_ROWS - 1) / U_ROWS;
   // a block's pages are loaded once for all its runs of tokens: as few blocks as fill the SMs twice over
-  const int blocks = 2 * sms / (Hkv * z) < 1 ? 1 : 2 * sms / (Hkv * z), per_block = (tiles + blocks - 1) / blocks;
+  const int64_t fill = 2 * (int64_t)sms / ((int64_t)Hkv * z);
+  const int blocks = fill < 1 ? 1 : (int)fill, per_block = (tiles + blocks - 1) / blocks;
   launch_pdl(kernel, dim3((tiles + per_block - 1) / per_block, Hkv, z), dim3(U_NT), smem, stream, q, ldq, means, num_pages, table, width, cu,
              num_reqs, positions, out, ldt, ldg, group, Hkv, page_size, pages, tiles, per_block, status);
   return cuda_status("page_scores (many tokens)");
@@ -689,9 +690,9 @@ DINFER_API int dinfer_page_scores(const PageScoresArgs* a) {
   if (T == 0 || pages == 0) return DINFER_OK;
   if (Hkv > 65535) return refuse(DINFER_BAD_ARGUMENT, "page_scores: %d key heads", Hkv);
   const int group = H / Hkv;
-  const int64_t z = (pages + WARPS * 32 - 1) / (WARPS * 32);
+  const int64_t z = ((int64_t)pages + WARPS * 32 - 1) / (WARPS * 32);
   if (dtype == DINFER_BF16 && (D == 64 || D == 128) && group <= 16 && ldq % 8 == 0 && ((uintptr_t)q | (uintptr_t)means) % 16 == 0 && z <= 65535) {
-    if (a->status && T >= MANY_TOKENS && T >= MANY_TOKENS_A_REQUEST * (int64_t)num_reqs) {
+    if (a->status && T >= MANY_TOKENS && T >= MANY_TOKENS_A_REQUEST * (int64_t)num_reqs && ((int64_t)pages + U_ROWS - 1) / U_ROWS <= 65535) {
       const __nv_bfloat16 *qb = (const __nv_bfloat16*)q, *mb = (const __nv_bfloat16*)means;
       const int sms = (int)a->sms;
 #define DINFER_SCORES(GP)                                                                                                              \

@@ -74,3 +74,25 @@ def test_scales_that_are_not_positive_in_32_bits(new, scale):
     got = page_ops.attention_pages(c(q), torch.empty_like(c(q)), c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, scale).cpu()
     want, size, qk = plain_attention(q, cache, b, chosen, H, scale)
     assert bool(((got.double() - want).abs() <= attention_bound(BF16, D, want, size, qk.abs())).all())
+
+
+@pytest.mark.parametrize("new", [3, 16])
+def test_scores_of_more_pages_than_a_grid_counts_by_the_128(new):
+    """8388481 pages of one token: the kernel with 128 pages a block would need more blocks than a launch may have."""
+    from dinfer_b200.kernels import page_ops
+    D, pages = 64, 128 * 65535 + 1
+    table = torch.full((1, pages), -1, dtype=torch.int32)
+    places = [0, 127, 128, 5000, pages // 2, pages - 2, pages - 1]
+    table[0, places] = torch.arange(len(places), dtype=torch.int32)
+    g = gen(5)
+    q, means = torch.randn(new, D, generator=g).to(BF16), torch.randn(len(places), 1, D, generator=g).to(BF16)
+    positions = torch.full((new,), pages - 1, dtype=torch.int32)
+    positions[0] = 5000
+    got = page_ops.page_scores(c(q), c(means), c(table), c(torch.tensor([0, new], dtype=torch.int32)), c(positions), 1, 1)[:, 0]
+    want = (q.double() @ means[:, 0].double().T).masked_fill(torch.tensor(places)[None] >= positions[:, None], -math.inf)
+    size = q.double().abs() @ means[:, 0].double().abs().T
+    found = got[:, c(torch.tensor(places))].cpu().double()
+    assert torch.equal(torch.isinf(found), torch.isinf(want))
+    fine = torch.isfinite(want)
+    assert bool(((found - want).abs()[fine] <= D * 2.0 ** -22 * size[fine]).all())
+    assert int(torch.isfinite(got).sum()) == int(fine.sum())
