@@ -736,6 +736,7 @@ DINFER_DEFINE_LAST_ERROR()
 static int64_t workspace_of(int num_reqs, int width, int top, int T, int H, int Hkv, int D, int page_size, Params& p) {
   if (T <= 0 || H <= 0 || Hkv <= 0 || H % Hkv || H / Hkv > BM || top <= 0 || width <= 0 || num_reqs <= 0 || (D != 64 && D != 128)) return 0;
   if (page_size < 16 || page_size > 128 || (page_size & (page_size - 1)) || (int64_t)width * page_size > INT32_MAX) return 0;
+  if ((int64_t)2 * (BM / (H / Hkv)) * top > INT32_MAX) return 0;        // (a block's tokens' entries, which the lists are made from)
   p.width = width; p.B = num_reqs; p.top = top; p.T = T; p.H = H; p.Hkv = Hkv; p.group = H / Hkv; p.page_size = page_size;
   const int64_t bytes = room(p, nullptr);
   return p.pairs > 65535 || bytes > MAX_ROOM ? 0 : bytes;

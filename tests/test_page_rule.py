@@ -53,3 +53,12 @@ def test_which_kernel_runs(kernel_of, call, wanted):
 def test_a_cache_without_pages_and_a_scale_that_is_no_positive_number(kernel_of, more):
     """The kernel of neighbouring tokens refuses them: the others give zeros, and weights that are right."""
     assert kernel_of([256], 8000, 32, 8, 128, 16, 64, **more) == "attention_pages"
+
+
+@pytest.mark.parametrize("top,takes", [(1 << 20, True), ((1 << 23) - 1, True), (1 << 23, False), (1 << 30, False)])
+def test_tokens_times_pages_beyond_31_bits(top, takes):
+    """The lists of a block's 256 tokens count their tokens' entries in 32 bits: a call with more goes to the other kernels."""
+    from dinfer_b200.kernels.lib import library
+    f = library("attention_pages_umma").dinfer_attention_pages_umma_workspace
+    f.argtypes, f.restype = [page_ops.c_int] * 9, page_ops.c_int64
+    assert (f(1, 5000, top, 300, 1, 1, 64, 16, 0) > 0) is takes      # 256 tokens of one head
