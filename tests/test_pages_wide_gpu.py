@@ -96,3 +96,31 @@ def test_scores_of_more_pages_than_a_grid_counts_by_the_128(new):
     fine = torch.isfinite(want)
     assert bool(((found - want).abs()[fine] <= D * 2.0 ** -22 * size[fine]).all())
     assert int(torch.isfinite(got).sum()) == int(fine.sum())
+
+
+# heads, kv heads, page, history, new tokens: lists of more entries than shared memory holds (256 for a group of one head, 1024 for four
+# and more) of contexts of more pages than one window of the lists' kernel (1024 and 4096)
+LONG = [(2, 2, 16, 40000, 300, 64), (16, 4, 16, 70000, 1300, 64), (2, 2, 32, 40000, 270, 128)]
+
+
+@pytest.mark.parametrize("H,G,page,history,new,D", LONG)
+@pytest.mark.parametrize("kind", ["usual", "odd"])
+def test_long_lists_over_several_windows(H, G, page, history, new, D, kind, libraries, monkeypatch):
+    """Prompt portions far along, 40 chosen pages of a token all over the context; odd: pages of the second window that are not held, and
+    one that a token names twice."""
+    from dinfer_b200.kernels import page_ops
+    rule = page_ops._portions
+    monkeypatch.setattr(page_ops, "_portions", lambda head: rule(head, True))
+    g = gen(H + new)
+    b = Batch([(history, new), (0, 3)], page, seed=44, extra_width=1)
+    window = 1024 if H == G else 4096
+    assert b.width > window + 100 or page != 16
+    q, cache = torch.randn(b.T, H * D, generator=g).to(BF16), torch.randn(b.num_pages, 2, G, page, D, generator=g).to(BF16)
+    chosen = choices(b, G, 40, g, "far")
+    far = history // page
+    if kind == "odd":
+        b.table[0, far - 50:far - 20] = -1
+        chosen[new // 2, :, 3] = chosen[new // 2, :, 30] = far - 5
+        chosen[new - 1, :, 7] = far - 30
+    compare(b, q, cache, chosen, H)
+    assert libraries == ["attention_pages_umma"]
