@@ -1,4 +1,4 @@
-"""Attention over chosen pages where keys or scores are infinite: what the softmax makes of them."""
+"""Attention over chosen pages where scores are infinite or large: what the softmax makes of them."""
 import math
 
 import pytest
@@ -46,3 +46,29 @@ def test_scores_of_minus_infinity(size, dtype, form):  # noqa: F811
     got, nan = got[:b.live].double(), torch.isnan(want)
     assert torch.equal(torch.isnan(got), nan)
     assert bool(((got - want).abs() <= attention_bound(dtype, D, want, size_, finite))[~nan].all())
+
+
+@pytest.mark.parametrize("scale", [1.0, 2.0 ** -9])
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_scores_of_whole_numbers(size, dtype, scale, form):  # noqa: F811
+    """Queries and keys of whole numbers, so that every partial sum of a score is one below 2^24 and exact in 32 bits in any order, cut off or
+    rounded, and the scale a power of two.  What is off then is the score's way through the exponential (log2 e times the scale, the
+    product, the maximum taken off: less than 8 x 2^-24 of the largest score), not the sum of its D products: a bound of a few percent
+    where scores lie thousands apart, of a rounding where many keys have weight."""
+    from dinfer_b200.kernels import page_ops
+    requests, P, H, G, D = size
+    g = gen(D + P + 1)
+    b = Batch(requests, P, seed=32, pad=1)
+    q = torch.randint(-40, 41, (b.T, H * D), generator=g).to(dtype)
+    cache = torch.randn(b.num_pages, 2, G, P, D, generator=g).to(dtype)
+    cache[:, 0] = torch.randint(-30, 31, (b.num_pages, G, P, D), generator=g).to(dtype)
+    chosen = choices(b, G, 5, g, "usual")
+    got = page_ops.attention_pages(c(q), torch.full_like(c(q), 3.0), c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, scale).cpu()
+    assert (got[b.live:] == 3.0).all()
+    want, size_, qk = plain_attention(q, cache, b, chosen, H, scale)
+    assert float(qk.max()) / scale < 2 ** 24
+    bound = attention_bound(dtype, 1, want, size_, 1.4427 * qk)          # 2 x 2^-22 of the largest score instead of 2 D x 2^-22
+    assert bool((bound <= (0.08 if dtype == F32 else 0.09) * size_ + 1e-30).all())
+    off = (got[:b.live].double() - want).abs()
+    assert bool((off <= bound).all()), float((off / bound).max())
