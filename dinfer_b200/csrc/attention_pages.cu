@@ -476,7 +476,8 @@ pages_token_kernel(const __nv_bfloat16* __restrict__ q, __nv_bfloat16* __restric
         st[nt][c] = p0;
         st[nt][c + 2] = p1;
       }
-      // the weights are rounded to bfloat16 for the second product (2^-9 of each; their sum is taken before)
+      // the weights are rounded to bfloat16, which the second product takes (half a step, 2^-8 of each; their sum is of the weights before):
+      // against 64 bits a result is off by 1.2 to 1.4 times what rounding it alone costs
       pb[nt][0] = movmatrix_trans(pack_bf16(st[nt][0], st[nt][1]));
       pb[nt][1] = movmatrix_trans(pack_bf16(st[nt][2], st[nt][3]));
     }

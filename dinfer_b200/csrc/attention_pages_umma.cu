@@ -12,10 +12,11 @@
 //     O[128, D]  += P V            tcgen05.mma accumulating in tensor memory; O is rescaled in place only when a row's maximum grows
 //                                  by more than 2^8
 // A page is read once for the 256 rows, not once for each token that chose it.  A warp none of whose rows sees a tile passes it with zeros.
-// 4096 tokens of 32 heads of 128 over 8, 16 pages of 64 each behind 28672, take 371 us (token by token 2700).  64 neighbouring tokens choose some
-// 85 pages among them, so that the products are five times what the tokens chose: 1.0 PFLOP/s, 59 % of a library product's rate.  Bound by
-// the hand-overs between products and softmax (1.1 us a key tile; the products alone 0.7) and by the last of four rounds of blocks,
-// half full.  A row tile that passed by the key tiles none of its tokens chose (a fifth) gained nothing, since both walk the same ring.
+// 4096 tokens of 32 heads of 128 over 8, 16 pages of 64 each behind 28672, take 354 to 378 us by the clock under load (token by token 2700).  64
+// neighbouring tokens choose some 85 pages among them, so that the products are five times what the tokens chose: 1.0 PFLOP/s, 59 % of a
+// library product's rate.  Bound by Q K^T and its place in the chain of a key tile (1.1 us; without the softmax as long, with one product of eight
+// in Q K^T a third less: every product reads 128 rows of Q for 64 keys from shared memory) and by the last of four rounds of blocks, half
+// full.  A row tile that passed by the key tiles none of its tokens chose (a fifth) gained nothing, since both walk the same ring.
 // Few tokens fill few SMs: then the blocks of a cluster share a pair's list, a run of its key tiles each, and fold their results
 // through distributed shared memory behind two cluster barriers, each block writing out a share of the 256 rows.
 //
@@ -497,7 +498,7 @@ attention_pages_umma_kernel(const __grid_constant__ CUtensorMap map_q, const __g
           asm("fma.rn.f32x2 %0, %1, %2, %3;" : "=l"(e) : "l"(pair_f32(s0[i], s0[i + 1])), "l"(scale2), "l"(neg2));
           const float lo = fast_exp2(__uint_as_float((unsigned)e)), hi = fast_exp2(__uint_as_float((unsigned)(e >> 32)));
           asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sq[i / 2 & 3]) : "l"(pair_f32(lo, hi)));
-          pw[i / 2] = pack_bf16(lo, hi);                            // (2^-9 of each weight; their sum is of the weights before)
+          pw[i / 2] = pack_bf16(lo, hi);                            // (half a step, 2^-8 of each; their sum is of the weights before)
         }
       }
       asm("add.rn.f32x2 %0, %0, %1;" : "+l"(sq[0]) : "l"(sq[1]));

@@ -30,7 +30,9 @@ class PageAttention(Mixer):
     """params: ``num_heads``, ``num_kv_heads``, ``head_dim``, ``top`` (pages a token reads at most, per key/value head), optional ``page``
     (tokens of a page, 64), ``first`` (pages from the request's beginning that are always read, 1), ``recent`` (pages up to the token's
     own that are always read, itself included, 1), ``qk_norm`` (bool), ``eps``, ``position`` (a PartSpec), ``scale``, and the tensor
-    names ``q_proj``, ``k_proj``, ``v_proj``, ``o_proj``, ``q_norm``, ``k_norm`` (after the prefix)."""
+    names ``q_proj``, ``k_proj``, ``v_proj``, ``o_proj``, ``q_norm``, ``k_norm`` (after the prefix).  Heads of 64 and 128 in groups of up to
+    16 on pages of 16, 32, 64 or 128 tokens run on the tensor cores in bfloat16; other sizes, and the scores of the 32-bit engine, on
+    kernels for any sizes, many times slower.  An entry that reads another's cache has to have pages of the same size."""
 
     def __init__(self, params, env: BuildEnv, prefix=""):
         super().__init__(params, env, prefix)
