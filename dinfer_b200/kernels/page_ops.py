@@ -123,6 +123,16 @@ def _rows(what: str, name: str, t, width: int):
     return shape[0], stride[0]
 
 
+def _meet(a: int, lda: int, b: int, ldb: int, rows: int, width: int, size: int) -> bool:
+    """Whether rows of ``width`` elements at address ``a`` and others at ``b``, strides in elements, have memory in common (or lie among one
+    another with strides that differ, which is taken for the same)."""
+    wide, last = width * size, (rows - 1) * size
+    if a + last * lda + wide <= b or b + last * ldb + wide <= a:
+        return False
+    step = lda * size
+    return lda != ldb or step == 0 or (b - a) % step < wide or (a - b) % step < wide
+
+
 def _heads(what: str, num_heads: int, num_kv_heads: int, head_dim: int) -> None:
     if num_heads <= 0 or num_kv_heads <= 0 or num_heads % num_kv_heads or not 0 < head_dim <= 512:
         raise KernelError(f"{what}: {num_heads} heads of {head_dim} over {num_kv_heads} key/value heads")
@@ -269,7 +279,8 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     rows, ldo = _rows(what, "out", out, num_heads * D)
     if rows != T:
         raise KernelError(f"{what}: out [T, H * D] of q's shape")
-    if T and out.data_ptr() == q.data_ptr():
+    q_at, out_at = q.data_ptr(), out.data_ptr()
+    if T and _meet(q_at, ldq, out_at, ldo, T, num_heads * D, q.element_size()):
         raise KernelError(f"{what}: out must not be q's memory (a row may be made twice)")
     B, width = _batch(what, T, block_table, cu_seqlens, positions)
     _ints(what, "chosen", chosen)
@@ -277,7 +288,7 @@ def attention_pages(q: torch.Tensor, out: torch.Tensor, cache: torch.Tensor, blo
     if len(shape) != 3 or shape[0] != T or shape[1] != Hkv or shape[2] == 0:
         raise KernelError(f"{what}: chosen int32 [T, Hkv, top] with top > 0")
     top = shape[2]
-    head = (q.data_ptr(), ldq, out.data_ptr(), ldo, cache.data_ptr(), num_pages, block_table.data_ptr(), width, cu_seqlens.data_ptr(), B,
+    head = (q_at, ldq, out_at, ldo, cache.data_ptr(), num_pages, block_table.data_ptr(), width, cu_seqlens.data_ptr(), B,
             positions.data_ptr(), chosen.data_ptr(), top, T, num_heads, Hkv, D, page_size, scale)
     if dt == _BF16 and T and (T >= PORTION_TOKENS and T > B or num_heads > TOKEN_GROUP * Hkv or top > TOKEN_TOP):
         size = _portions(head)

@@ -62,3 +62,33 @@ def test_tokens_times_pages_beyond_31_bits(top, takes):
     f = library("attention_pages_umma").dinfer_attention_pages_umma_workspace
     f.argtypes, f.restype = [page_ops.c_int] * 9, page_ops.c_int64
     assert (f(1, 5000, top, 300, 1, 1, 64, 16, 0) > 0) is takes      # 256 tokens of one head
+
+
+@pytest.mark.parametrize("call,refused", [
+    ("the same", True), ("a row further", True), ("half a row further", True), ("half a row before", True), ("columns that meet", True),
+    ("columns side by side", False), ("columns the other way", False), ("behind", False), ("rows of another width", True), ("one token", True),
+    ("one token beside", False)])
+def test_outputs_over_queries(monkeypatch, call, refused):
+    """A row may be made twice, and blocks read queries while others write: no part of ``out`` may lie on ``q``."""
+    from dinfer_b200.kernels.lib import KernelError
+    H, G, D, page, T = 4, 2, 64, 16, 5
+    w, launched = H * D, []
+    monkeypatch.setattr(page_ops, "_here", lambda what, *tensors: None)
+    monkeypatch.setattr(page_ops, "_device", lambda: 0)
+    monkeypatch.setattr(page_ops, "_call", lambda lib, *args: launched.append(lib))
+    x = torch.zeros(T * 4 * w, dtype=BF16)
+    rows = lambda at, ld, n=T: x[at:].as_strided((n, w), (ld, 1), at)                # noqa: E731
+    q, out = {"the same": (rows(0, w), rows(0, w)), "a row further": (rows(0, w), rows(w, w)), "half a row further": (rows(0, w), rows(w // 2, w)),
+              "half a row before": (rows(w // 2, w), rows(0, w)), "columns that meet": (rows(0, 3 * w), rows(w - 8, 3 * w)),
+              "columns side by side": (rows(0, 2 * w), rows(w, 2 * w)), "columns the other way": (rows(2 * w, 3 * w), rows(w, 3 * w)),
+              "behind": (rows(0, w), rows(T * w, w)), "rows of another width": (rows(0, 2 * w), rows(w, 3 * w)),
+              "one token": (rows(0, 7, 1), rows(8, 9, 1)), "one token beside": (rows(0, w, 1), rows(w, w, 1))}[call]
+    n = q.shape[0]
+    i = lambda *s: torch.zeros(*s, dtype=torch.int32)                                # noqa: E731
+    args = (q, out, torch.zeros(2, 2, G, page, D, dtype=BF16), i(1, 3), i(2), i(n), i(n, G, 4), H, 0.1)
+    if refused:
+        with pytest.raises(KernelError, match="out must not be q's memory"):
+            page_ops.attention_pages(*args)
+    else:
+        page_ops.attention_pages(*args)
+    assert len(launched) == (not refused)
