@@ -72,3 +72,28 @@ def test_scores_of_whole_numbers(size, dtype, scale, form):  # noqa: F811
     assert bool((bound <= (0.08 if dtype == F32 else 0.09) * size_ + 1e-30).all())
     off = (got[:b.live].double() - want).abs()
     assert bool((off <= bound).all()), float((off / bound).max())
+
+
+@pytest.mark.parametrize("dtype", [BF16, F32])
+@pytest.mark.parametrize("size", SIZES, ids=str)
+def test_a_score_of_infinity(size, dtype, form):  # noqa: F811
+    """One key scores +inf with every query of a key head: infinity over infinity for the tokens that see it, nothing for the others."""
+    from dinfer_b200.kernels import page_ops
+    requests, P, H, G, D = size
+    g = gen(D + P + 2)
+    b = Batch(requests, P, seed=33, pad=1)
+    q = torch.randn(b.T, H, D, generator=g)
+    q[..., 3] = q[..., 3].abs() + 0.25
+    q = q.reshape(b.T, H * D).to(dtype)
+    cache = torch.randn(b.num_pages, 2, G, P, D, generator=g).to(dtype)
+    chosen = choices(b, G, 5, g, "usual")
+    finite = plain_attention(q, cache, b, chosen, H, 0.2)[2]
+    for r, (h, n) in enumerate(requests):
+        at = h + n // 2
+        cache[int(b.table[r, at // P]), 0, G - 1, at % P, 3] = math.inf
+    want, size_, _ = plain_attention(q, cache, b, chosen, H, 0.2)
+    got = page_ops.attention_pages(c(q), torch.full_like(c(q), 3.0), c(cache), c(b.table), c(b.cu), c(b.positions), c(chosen), H, 0.2).cpu()
+    assert (got[b.live:] == 3.0).all()
+    got, nan = got[:b.live].double(), torch.isnan(want)
+    assert bool(nan.any()) and torch.equal(torch.isnan(got), nan)
+    assert bool(((got - want).abs() <= attention_bound(dtype, D, want, size_, finite))[~nan].all())
