@@ -762,8 +762,8 @@ DINFER_API int64_t dinfer_attention_pages_umma_workspace(int num_reqs, int width
   Params p{};
   const int64_t bytes = workspace_of(num_reqs, width, top, T, H, Hkv, D, page_size, p);
   if (bytes == 0 || sms <= 0) return bytes;
-  const double keys = (double)(top < width ? top : width) * page_size, row = D * 4;
-  const double by_token = 7.0 + (H / Hkv > 16 || top > 1024 ? fmax(T * H * keys * row / 3e6, keys / 26) : T * Hkv * keys * row / 6.3e6);
+  const double tokens = T, keys = (double)(top < width ? top : width) * page_size, row = D * 4;
+  const double by_token = 7.0 + (H / Hkv > 16 || top > 1024 ? fmax(tokens * H * keys * row / 3e6, keys / 26) : tokens * Hkv * keys * row / 6.3e6);
   auto tiles = [&](double n) { return fmin((double)width, top * pow(fmax(n, 1.0), 0.4)) * page_size / BN; };
   const double most = 2.0 * p.tile_tokens, longest = fmin(T - num_reqs + 1.0, most), mean = fmin((double)T / num_reqs, most);
   const double lists = fmax((double)T / most, (double)(num_reqs < T ? num_reqs : T)) * Hkv;
